@@ -13,7 +13,8 @@
  *      reference's `mlk-kernel` JSON wire format, run over typed device or
  *      host buffers (f16 / f32 / f64), optionally sharded over GPUs.
  *   3. Direct kernel entry points (`mlkb_map_*`, `mlkb_softmax_*`,
- *      `mlkb_gemm_*`, `mlkb_qk_softmax_*`) over device pointers on a stream.
+ *      `mlkb_gemm_*`, `mlkb_qk_softmax_*`, `mlkb_norm_rope`,
+ *      `mlkb_attention_*`) over device pointers on a stream.
  *
  * Every entry point returns an mlkb status (0 = ok). Codes 1-4 keep the
  * meaning the reference artifact ABI gives them
@@ -47,6 +48,7 @@ extern "C" {
 #define MLKB_F16 1
 #define MLKB_F32 2
 #define MLKB_F64 3
+#define MLKB_BF16 4 /* bfloat16: mlkb_norm_rope and mlkb_attention_* only */
 
 /* ---- module classes (what the pattern matcher recognised) --------------- */
 #define MLKB_KIND_MAP 1        /* one or more 1-D Loop{Compute;Store} roots */
@@ -77,6 +79,21 @@ typedef struct mlkb_expr {
     int64_t b_index;
     double b_value;
 } mlkb_expr;
+
+/*
+ * A [rows, heads, d] operand of the norm_rope and attention entries: 16-bit
+ * elements in device memory, the last dimension contiguous. data is 16-byte
+ * aligned and the strides (in elements) are positive multiples of 8; the
+ * stride of a dimension with one entry is ignored. At most 2^30 rows. Views
+ * into a larger buffer (the q, k and v parts of one projection's output,
+ * [heads, rows, d] storage) are ordinary. An output's rows may not overlap.
+ */
+typedef struct mlkb_heads {
+    void* data;
+    int64_t rows;
+    int64_t row_stride;
+    int64_t head_stride;
+} mlkb_heads;
 
 typedef struct mlkb_module mlkb_module; /* opaque bound Kernel IR module */
 
@@ -374,6 +391,101 @@ int mlkb_qk_softmax_f16(const void* q, const void* k, float* y, int64_t batch,
  * in place as the tensor cores' MN-major operand; nothing is transposed. */
 int mlkb_qk_softmax_kt_f16(const void* q, const void* kt, float* y, int64_t batch,
                            int64_t m, int64_t s, int64_t d, double scale, void* stream);
+
+/*
+ * Head norms and position rotation of queries and keys in one pass. For each
+ * row x (d elements) of every head of q [tokens, heads, d] and k [tokens,
+ * kv_heads, d], in f32 and rounded once:
+ *   x = x * rsqrt(mean(x^2) + eps) * weight     (with weights)
+ *   (x_a, x_b) = (x_a c - x_b s, x_b c + x_a s)  for pair i of rot / 2
+ * where (a, b) is (i, i + rot/2), or (2i, 2i + 1) with `interleaved`, and the
+ * elements from rot on are only normed. c = table[p, i], s = table[p, rot/2 + i]
+ * for the token's position p on the pair's axis.
+ *   heads, kv_heads  1 to 65536; kv_heads 0 leaves k and k_out out
+ *   d, rot           multiples of 16, rot <= d <= 512
+ *   q_weight, k_weight  [d] in the element type, or both NULL: no norm
+ *   table            f32 [table_rows, rot]: cosines, then sines
+ *   positions        int32, axis a of token t at [a * position_stride + t];
+ *                    a token with a position outside the table is left as it
+ *                    is and raises MLKB_ERR_INVALID in the status word that
+ *                    mlkb_take_device_error returns
+ *   sections         (host) how many pairs each of the n_axes axes turns, in
+ *                    order; they add up to rot / 2. NULL with one axis
+ *   elem_dtype       MLKB_F16 or MLKB_BF16, of q, k, weights and outputs
+ * Outputs may be the inputs themselves (same address and strides) and may not
+ * overlap them otherwise. No counterpart in the reference, whose Kernel IR
+ * has neither operator; the same holds for the attention entries below.
+ */
+int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* q_out,
+                   const mlkb_heads* k_out, int64_t heads, int64_t kv_heads, int64_t d,
+                   int64_t rot, const void* q_weight, const void* k_weight, double eps,
+                   const float* table, int64_t table_rows, const int32_t* positions,
+                   int64_t position_stride, const int32_t* sections, int32_t n_axes,
+                   int32_t interleaved, int32_t elem_dtype, void* stream);
+
+/*
+ * Attention over packed sequences: y = softmax(scale * q k^T) v for each head,
+ * where head h reads kv head h / (heads / kv_heads). Sequence s has the
+ * queries q_starts[s] .. q_starts[s+1]-1 and the keys k_starts[s] ..
+ * k_starts[s+1]-1 (device arrays of n_seqs + 1 int32). With `causal` its last
+ * query sees its last key: query i of nq sees keys j <= i + nk - nq of nk.
+ * So a whole prompt (nq == nk), the next piece of one, and a single new token
+ * are the same call.
+ *   q, y     [rows, heads, d]; k, v [key rows, kv_heads, d]; heads a multiple
+ *            of kv_heads, at most 128 times it; d a multiple of 8, 8 to 128;
+ *            f16 or bf16 (elem_dtype), y in the same type
+ *   scale    positive
+ * Scores, row maxima, sums and outputs are held in f32; the probabilities are
+ * rounded to the element type before the product with v. A query that sees no
+ * key (or only scores of -inf) gets zeros. Rows of y outside every sequence
+ * are left as they were. Keys a query does not see have no effect on it,
+ * whatever they or their values hold. A sequence whose starts fall or leave
+ * the operands is skipped and raises MLKB_ERR_INVALID in the status word that
+ * mlkb_take_device_error returns. y may not overlap the inputs.
+ */
+int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* v,
+                          const mlkb_heads* y, int64_t heads, int64_t kv_heads, int64_t d,
+                          const int32_t* q_starts, const int32_t* k_starts, int64_t n_seqs,
+                          int32_t causal, double scale, int32_t elem_dtype, void* stream);
+
+/*
+ * Attention of a batch whose requests share a prefix: each request's `steps`
+ * newest tokens (q and y: [batch * steps, heads, d]) over prefix_rows keys
+ * that all requests have in common, then the request's own keys. The prefix
+ * is read once for the whole batch.
+ *   prefix_k, prefix_v  [prefix_rows, kv_heads, d]; prefix_rows may be 0
+ *   k_pages, v_pages    [n_pages * page_size, kv_heads, d]
+ *   pages               device int32 [batch, pages_per_request]: request b's
+ *                       key i lies in page pages[b, i / page_size]. page_size
+ *                       is a power of two from 16 on. Entries behind a
+ *                       request's last key are not read. NULL: pages_per_request
+ *                       is 1, page b is request b's, of any size
+ *   lens                device int32 [batch]: own keys of each request, its
+ *                       newest tokens' among them; token i of `steps` sees the
+ *                       own keys j <= i + lens[b] - steps (and the prefix)
+ *   workspace           device memory of at least
+ *                       mlkb_attention_prefix_workspace bytes, 16-byte aligned,
+ *                       in use until the call's work on `stream` is done: calls
+ *                       (and captured graphs) that may run at the same time
+ *                       need workspaces of their own. Its contents do not matter
+ * Types, sizes, rounding and masked keys as in mlkb_attention_packed. A
+ * length outside [0, page_size * pages_per_request] is taken as the nearer
+ * end, and a page index outside the pages reads as zeros; both raise
+ * MLKB_ERR_INVALID in the status word.
+ */
+int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* prefix_k,
+                          const mlkb_heads* prefix_v, const mlkb_heads* k_pages,
+                          const mlkb_heads* v_pages, const mlkb_heads* y, int64_t batch,
+                          int64_t steps, int64_t heads, int64_t kv_heads, int64_t d,
+                          int64_t page_size, int64_t pages_per_request, const int32_t* pages,
+                          const int32_t* lens, double scale, int32_t elem_dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace mlkb_attention_prefix needs for these shapes on the
+ * current device; negative for shapes it refuses. */
+int64_t mlkb_attention_prefix_workspace(int64_t batch, int64_t steps, int64_t heads,
+                                        int64_t kv_heads, int64_t d, int64_t prefix_rows,
+                                        int64_t page_size, int64_t pages_per_request);
 
 /* Deterministic synthetic inputs, generated on the device: a counter-based
  * SplitMix64 stream of (seed, stream_id, element index).

@@ -25,7 +25,7 @@ ERR_UNSUPPORTED = 7
 ERR_INVALID = 8
 ERR_NOT_BOUND = 9
 
-F16, F32, F64 = 1, 2, 3
+F16, F32, F64, BF16 = 1, 2, 3, 4  # BF16: norm_rope and attention_* only
 KIND_MAP, KIND_SOFTMAX, KIND_MATMUL, KIND_REDUCESUM, KIND_QK_SOFTMAX = 1, 2, 3, 4, 5
 
 

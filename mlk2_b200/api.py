@@ -11,7 +11,7 @@ from typing import Sequence
 
 import numpy as np
 
-from . import F16, F32, F64, check, kir, lib
+from . import BF16, F16, F32, F64, check, kir, lib
 
 ASSEMBLE_DEVICE0 = 1  # MLKB_ASSEMBLE_DEVICE0
 ASSEMBLE_VIA_NCCL = 2  # MLKB_ASSEMBLE_VIA_NCCL
@@ -120,6 +120,200 @@ def qk_softmax_kt(q, kt, y, scale: float, stream=None):
     assert tuple(kt.shape) == (batch, d, s) and tuple(y.shape) == (batch, m, s)
     check(lib().mlkb_qk_softmax_kt_f16(_ptr(q), _ptr(kt), _ptr(y), batch, m, s, d, float(scale),
                                        _stream(stream)))
+
+
+# ---- attention (device tensors, 16-bit elements) ----------------------------------
+# Unlike the entries above, these take strided views (only the last dimension
+# contiguous) and run on their tensors' device, whichever device is current.
+
+_HEADS = C.c_int64 * 24  # up to six mlkb_heads: data, rows, row stride, head stride
+_HALF_DT = None
+
+
+def _heads_args(tensors, names):
+    """The operands as consecutive mlkb_heads, and their element type. Each is
+    [rows, heads, d], or None."""
+    global _HALF_DT
+    if _HALF_DT is None:
+        import torch
+
+        _HALF_DT = {torch.float16: F16, torch.bfloat16: BF16}
+    flat = []
+    first = tensors[0]
+    dtype, device = first.dtype, first.device
+    if dtype not in _HALF_DT:
+        raise ValueError(f"{names[0]}: dtype must be float16 or bfloat16, got {dtype}")
+    for t, name in zip(tensors, names):
+        if t is None:
+            flat += (0, 0, 0, 0)
+            continue
+        if t.dtype is not dtype or t.device != device:
+            raise ValueError(f"{name}: {t.dtype} on {t.device}, but {names[0]} is {dtype} on {device}")
+        rows, heads, _ = t.shape
+        row, head, last = t.stride()
+        if last != 1 and t.shape[2] > 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous")
+        flat += (t.data_ptr(), rows, row, head)
+    return _HEADS(*flat), _HALF_DT[dtype]
+
+
+def _int32_ptr(t, name, device, shape):
+    import torch
+
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous int32 on {device} needed")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+    return t.data_ptr()
+
+
+def _on_device(device, stream, call):
+    """call(stream handle) with `device` current (the default stream is the
+    device's current one)."""
+    import torch
+
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {device}")
+    if device.index == torch.cuda.current_device():
+        check(call(_stream(stream)))
+    else:
+        with torch.cuda.device(device):
+            check(call(_stream(stream)))
+
+
+def norm_rope(q, k, q_out, k_out, table, positions, sections=None, q_weight=None, k_weight=None,
+              eps: float = 1e-6, interleaved: bool = False, stream=None):
+    """Head norms (where weights are given) and position rotation of q
+    [tokens, heads, d] and k [tokens, kv_heads, d] (k and k_out may be None)
+    into q_out and k_out, which may be q and k themselves.
+
+    table: f32 [positions, rot], cosines of the rot/2 angles, then sines.
+    positions: int32 [tokens], or [axes, tokens] with `sections`, the number
+    of pairs each axis turns. A token whose position is outside the table is
+    left as it is (take_device_error() then reports it)."""
+    import torch
+
+    tokens, heads, d = q.shape
+    kv = 0 if k is None else k.shape[1]
+    ops, dt = _heads_args((q, k, q_out, k_out), ("q", "k", "q_out", "k_out"))
+    device = q.device
+    if q_out.shape != q.shape or (k is None) != (k_out is None) or (
+            k is not None and (k_out.shape != k.shape or k.shape[0] != tokens or k.shape[2] != d)):
+        raise ValueError("q_out and k_out must have the shapes of q and k, of equal tokens and d")
+    if table.dtype is not torch.float32 or table.device != device or not table.is_contiguous() \
+            or table.dim() != 2:
+        raise ValueError("table: contiguous float32 [positions, rot] on the device of q needed")
+    axes = 1 if positions.dim() == 1 else positions.shape[0]
+    pos = _int32_ptr(positions, "positions", device,
+                     (tokens,) if positions.dim() == 1 else (axes, tokens))
+    if sections is not None and len(sections) != axes:
+        raise ValueError(f"sections: {len(sections)} given for {axes} position axes")
+    sec = (C.c_int32 * axes)(*sections) if sections is not None else None
+    ptrs = []
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None and (w.dtype is not q.dtype or w.device != device or not w.is_contiguous()
+                              or tuple(w.shape) != (d,)):
+            raise ValueError(f"{name}: contiguous [{d}] of {q.dtype} on {device} needed")
+        ptrs.append(None if w is None else w.data_ptr())
+    table_rows, rot = table.shape
+    _on_device(device, stream, lambda s: lib().mlkb_norm_rope(
+        ops, C.byref(ops, 32), C.byref(ops, 64), C.byref(ops, 96), heads, kv, d, rot, ptrs[0], ptrs[1],
+        eps, table.data_ptr(), table_rows, pos, tokens, sec, axes, int(interleaved), dt, s))
+
+
+def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool = True, stream=None):
+    """y = softmax(scale q k^T) v for each head, over packed sequences.
+
+    q, y [rows, heads, d]; k, v [key rows, kv_heads, d]; q_starts, k_starts
+    int32 [sequences + 1]: sequence s has the rows starts[s] .. starts[s+1]-1.
+    causal: the last query of a sequence sees its last key. Rows of y outside
+    the sequences are left as they were; a query that sees no key gets zeros."""
+    ops, dt = _heads_args((q, k, v, y), ("q", "k", "v", "y"))
+    rows, heads, d = q.shape
+    kv = k.shape[1]
+    if y.shape != q.shape or v.shape != k.shape or k.shape[2] != d:
+        raise ValueError("y must have the shape of q, v that of k, and all the same d")
+    device = q.device
+    n = q_starts.shape[0]
+    if n < 1:
+        raise ValueError("q_starts: sequences + 1 entries needed")
+    qs = _int32_ptr(q_starts, "q_starts", device, (n,))
+    ks = _int32_ptr(k_starts, "k_starts", device, (n,))
+    _on_device(device, stream, lambda s: lib().mlkb_attention_packed(
+        ops, C.byref(ops, 32), C.byref(ops, 64), C.byref(ops, 96), heads, kv, d, qs, ks, n - 1,
+        int(causal), scale, dt, s))
+
+
+def attention_prefix_workspace(q, prefix_k, k_pages, pages=None) -> int:
+    """Bytes of workspace attention_prefix needs for these operands."""
+    import torch
+
+    batch, steps, heads, d = q.shape
+    wide = pages.shape[1] if pages is not None else min(1, k_pages.shape[0])
+    with torch.cuda.device(q.device):
+        return lib().mlkb_attention_prefix_workspace(batch, steps, heads, prefix_k.shape[1], d,
+                                                     prefix_k.shape[0], k_pages.shape[1], wide)
+
+
+def attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale: float, pages=None,
+                     workspace=None, stream=None):
+    """Attention of a batch that shares a prefix: the newest tokens q [batch,
+    steps, heads, d] of each request over the common keys prefix_k, prefix_v
+    [prefix, kv_heads, d], then the request's own lens[b] keys, its newest
+    tokens' among them and causal over those.
+
+    k_pages, v_pages [pages, page size, kv_heads, d]; pages int32 [batch,
+    pages a request may have] names them in order, or None: page b is request
+    b's. lens int32 [batch]. workspace: a CUDA tensor of at least
+    attention_prefix_workspace bytes, allocated here (on the current stream)
+    when None."""
+    import torch
+
+    batch, steps, heads, d = q.shape
+    kv = prefix_k.shape[1]
+    page = k_pages.shape[1]
+    if y.shape != q.shape or prefix_v.shape != prefix_k.shape or v_pages.shape != k_pages.shape \
+            or prefix_k.shape[2] != d or tuple(k_pages.shape[2:]) != (kv, d):
+        raise ValueError("y must have the shape of q, v that of k, and all the same d and kv heads")
+    flat = [_flat2(t, n) for t, n in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (y, "y"))]
+    ops, dt = _heads_args((flat[0], prefix_k, prefix_v, flat[1], flat[2], flat[3]),
+                          ("q", "prefix_k", "prefix_v", "k_pages", "v_pages", "y"))
+    device = q.device
+    wide = pages.shape[1] if pages is not None else min(1, k_pages.shape[0])
+    if pages is None and k_pages.shape[0] not in (0, batch):
+        raise ValueError("without a page table there must be one page for each request")
+    table = _int32_ptr(pages, "pages", device, (batch, wide))
+    own = _int32_ptr(lens, "lens", device, (batch,))
+
+    def call(s):
+        L = lib()
+        ws = workspace
+        if ws is None:
+            need = L.mlkb_attention_prefix_workspace(batch, steps, heads, kv, d, prefix_k.shape[0],
+                                                     page, wide)
+            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=device)
+            if stream is not None:
+                # the memory returns to the pool on the current stream: not before `stream` is done
+                ws.record_stream(torch.cuda.ExternalStream(int(stream), device=device))
+        elif ws.device != device or not ws.is_contiguous():
+            raise ValueError(f"workspace: contiguous on {device} needed")
+        return L.mlkb_attention_prefix(
+            ops, C.byref(ops, 32), C.byref(ops, 64), C.byref(ops, 96), C.byref(ops, 128),
+            C.byref(ops, 160), batch, steps, heads, kv, d, page, wide, table, own, scale, dt,
+            ws.data_ptr(), ws.numel() * ws.element_size(), s)
+
+    _on_device(device, stream, call)
+
+
+def _flat2(t, name):
+    """[a, b, heads, d] as [a * b, heads, d] without a copy."""
+    a, b, heads, d = t.shape
+    if a > 1 and b > 1 and t.stride(0) != b * t.stride(1):
+        raise ValueError(f"{name}: its first two dimensions must have one common stride")
+    row = t.stride(1) if b > 1 else t.stride(0)
+    return t.as_strided((a * b, heads, d), (row, t.stride(2), t.stride(3)))
 
 
 def fill(out, seed: int, stream_id: int, dist: str, lo: float, hi: float, stream=None):

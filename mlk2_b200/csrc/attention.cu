@@ -1,0 +1,1181 @@
+// Attention over packed prompts (attention_packed) and of a batch whose
+// requests share a prefix (attention_prefix): y = softmax(scale q K^T) V per
+// head, without writing the scores.
+//
+// Both run one tcgen05 kernel over a list of items. Query heads that share a
+// kv head are rows of the same tile (row r of a tile: token r / G, head r % G
+// of the G heads of the kv head), so grouped heads read K and V once.
+//
+// One CTA per SM, persistent. Two streams of work per CTA, each with its own
+// 128-row query tile, score accumulator and softmax warps:
+//   warps 0-3    stream 0: softmax and epilogue, one thread per row
+//   warps 4-7    stream 1: the same
+//   warp 8       MMA issuer
+//   warp 9       TMA producer (Q tiles; K and V tiles of 128 keys in a ring)
+//   warp 10      scheduler: writes the items into a ring for the other warps
+//   warp 11      idle (register shares move by groups of four warps)
+// TMEM: two score tiles (128 f32 columns each; the tile's probabilities
+// overwrite its first half as 16-bit pairs and are the A operand of P V) and
+// two output accumulators (128 columns each). For one stream the issuer
+// alternates P V of key tile j and Q K^T of tile j + 1; the streams interleave,
+// so one's softmax runs under the other's products. An item's streams are
+// either two query tiles over the same keys (`paired`) or one query tile over
+// alternate key tiles.
+//
+// Softmax: running row maximum m (of the raw scores) and sum in f32;
+// p = 2^(c s - c m), c = scale log2 e. The accumulator is rescaled only when a
+// row's maximum has grown by more than 2^8 since the last rescale: until then
+// p stays within 2^8 of 1, far inside the 16-bit formats' range, and the
+// factor cancels in the final division. The commit that makes Q K^T of tile
+// j + 1 visible also covers P V of tile j (same issuing thread), so a rescale
+// finds the accumulator at rest without another barrier.
+//
+// p is rounded to the inputs' 16-bit type for the product with V (the tensor
+// cores take equal operand types); its row sum is taken before that rounding.
+//
+// Keys past an item's end are masked in the scores and zeroed in V's tile (a
+// zero probability times a NaN would be NaN). Values that only some rows of a
+// tile may see (the causal edge) cannot be zeroed: a row whose result has a
+// NaN is computed again key by key from its own keys (slowRow).
+//
+// Every mbarrier wait is bounded (2 s); on a timeout the CTA raises the device
+// status word, drains its copies, frees TMEM and returns.
+#include <cudaTypedefs.h>
+
+#include <atomic>
+#include <climits>
+#include <type_traits>
+
+#include "heads.cuh"
+#include "tc_common.cuh"
+
+namespace mlkb {
+int makeTmap3d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base,
+               const int64_t (&dims)[3], const int64_t (&strides)[2], const int (&box)[3],
+               CUtensorMapSwizzle swizzle);
+
+namespace {
+
+constexpr int kTile = 128;   // rows of a query tile, keys of a key tile
+constexpr int kItems = 3;    // item ring
+constexpr int kStages = 5;   // K / V ring
+constexpr int kThreads = 12 * 32;
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;  // 8 x 200 + 4 x 104 = 12 x 168 as launched
+constexpr int kConsumers = 10;  // warps that read an item
+constexpr uint64_t kLimitNs = 2000000000ull;
+constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
+constexpr int kMaxSlots = 64;     // partial results a row may have
+
+// What one pass through the pipeline computes. Keys are counted from the
+// item's first; row limits (how many keys token i of a stream sees) are
+// clamp(vis0 + i, 0, nk) when causal, nk otherwise.
+struct Item {
+    int32_t live;      // 0: no more items
+    int32_t paired;    // streams: two query tiles over all key tiles / one over alternate key tiles
+    int32_t causal;
+    int32_t src;       // key source: 0 = rows of map 0, 1 = rows or pages of map 1
+    int32_t kvh;
+    int32_t nk;        // keys
+    int32_t k_row;     // contiguous source: row of the first key
+    int32_t page_row;  // paged source: first entry of the request's page table
+    int32_t key0;      // paged source: first key's index in the request
+    int32_t q_row[2];  // first token row of each stream
+    int32_t tok[2];    // its tokens
+    int32_t n[2];      // its key tiles
+    int32_t vis0[2];
+    int32_t slot[2];   // partial-result slot (prefix)
+};
+
+struct KeySource {
+    const void* k;
+    const void* v;
+    int64_t k_row, k_head, v_row, v_head;  // strides, elements
+};
+
+struct Params {
+    int32_t heads, kv_heads, group, d, tt;  // tt: tokens of a query tile
+    float c2, grow;                         // scale * log2 e; kRescale / c2
+    int* status;
+    const void* q;
+    int64_t q_row, q_head;
+    KeySource src[2];
+    void* y;
+    int64_t y_row, y_head;
+    // packed
+    const int32_t* q_starts;
+    const int32_t* k_starts;
+    int32_t seqs, q_rows, k_rows, causal;
+    // prefix
+    const int32_t* lens;
+    const int32_t* pages;
+    int32_t batch, steps, prefix;
+    int32_t page, page_shift, wide, n_pages;  // page size; pages of a request; pages in all
+    int32_t pre_items, pre_tiles, pre_splits, pre_mt, pre_paired;  // prefix items
+    int32_t suf_items, suf_keys, suf_chunks, suf_mt;               // request items
+    float* part;
+    float* lse;
+    int64_t rows;  // result rows: batch * steps * heads
+};
+
+template <int D>
+struct Smem {
+    static constexpr int kHalves = D / 64;
+    static constexpr uint32_t kBox = kTile * 128;          // 16 KB: 128 rows x 64 elements
+    static constexpr uint32_t kTileBytes = kHalves * kBox;
+    uint8_t q[2][kTileBytes];
+    uint8_t kv[kStages][kTileBytes];
+    Item item[kItems];
+    uint64_t full[kStages], empty[kStages];
+    uint64_t qfull[2], qempty[2];
+    uint64_t sfull[2], pfull[2], ofull[2];
+    uint64_t ifull[kItems], iempty[kItems];
+    uint32_t tmem_base;
+    int abort;
+};
+
+__device__ __forceinline__ int ceilDiv(int a, int b) { return (a + b - 1) / b; }
+
+__device__ __forceinline__ int rowLimit(const Item& it, int st, int token) {
+    int v = it.causal ? it.vis0[st] + token : it.nk;
+    v = v < 0 ? 0 : v;
+    return v < it.nk ? v : it.nk;
+}
+
+// Key tiles of an item, and the tile of step u of its pipeline (stream u & 1).
+__device__ __forceinline__ int itemTiles(const Item& it) {
+    return it.paired ? (it.n[0] > it.n[1] ? it.n[0] : it.n[1]) : it.n[0] + it.n[1];
+}
+__device__ __forceinline__ bool stepLive(const Item& it, int u) {
+    return (u >> 1) < it.n[u & 1];
+}
+__device__ __forceinline__ int stepTile(const Item& it, int u) { return it.paired ? u >> 1 : u; }
+
+// ---- scheduling: packed prompts ------------------------------------------------------
+// Items are (sequence, pair of query tiles, kv head), dealt to the CTAs in
+// order of falling cost (key tiles of the pair), back and forth over the grid,
+// so that the CTAs' sums come out even and the long items start first. No
+// list is stored: the warp walks cost levels x groups of 32 sequences, each
+// lane counting its sequence's pairs of exactly that cost.
+struct Walker {
+    int level, base;     // cost level; first sequence of the current group
+    int64_t before;      // items before (level, group)
+};
+
+struct Seq {
+    int q0, nq, k0, nk;
+};
+
+__device__ __forceinline__ Seq loadSeq(const Params& p, int s) {
+    Seq r = {0, 0, 0, 0};
+    if (s < p.seqs) {
+        const int a = p.q_starts[s], b = p.q_starts[s + 1];
+        const int c = p.k_starts[s], e = p.k_starts[s + 1];
+        if (a < 0 || b < a || b > p.q_rows || c < 0 || e < c || e > p.k_rows) {
+            if (p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
+        } else {
+            r = {a, b - a, c, e - c};
+        }
+    }
+    return r;
+}
+
+// Pairs of a sequence whose cost is at least `c` key tiles (they are its last).
+__device__ __forceinline__ int pairsFrom(const Params& p, const Seq& s, int c) {
+    const int w = 2 * p.tt;
+    const int np = ceilDiv(s.nq, w);
+    if (c <= 0) return np;
+    const int need = kTile * (c - 1) + 1;  // keys
+    if (s.nk < need) return 0;
+    if (!p.causal) return np;
+    const int tokens = need - (s.nk - s.nq);  // the pair's last token is at least this one
+    const int first = tokens <= 0 ? 0 : (tokens - 1) / w;
+    return np - first;
+}
+
+__device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, int lane) {
+    for (;;) {
+        const Seq s = loadSeq(p, w.base + lane);
+        const int ge = pairsFrom(p, s, w.level), gt = pairsFrom(p, s, w.level + 1);
+        const int64_t mine = static_cast<int64_t>(ge - gt) * p.kv_heads;
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+        if (idx < w.before + total) {
+            const int64_t at = idx - w.before;
+            const unsigned hit = __ballot_sync(0xffffffffu, at < upto);
+            const int src = __ffs(hit) - 1;
+            const int rem = static_cast<int>(at - (upto - mine));
+            if (lane == src) {
+                const int pair = ceilDiv(s.nq, 2 * p.tt) - ge + rem / p.kv_heads;
+                it.live = 1;
+                it.paired = 1;
+                it.causal = p.causal;
+                it.src = 0;
+                it.kvh = rem % p.kv_heads;
+                it.nk = s.nk;
+                it.k_row = s.k0;
+                it.page_row = 0;
+                it.key0 = 0;
+                for (int st = 0; st < 2; ++st) {
+                    const int t0 = (2 * pair + st) * p.tt;
+                    int n = s.nq - t0;
+                    n = n < 0 ? 0 : n < p.tt ? n : p.tt;
+                    it.q_row[st] = s.q0 + t0;
+                    it.tok[st] = n;
+                    it.vis0[st] = s.nk - s.nq + t0 + 1;
+                    it.n[st] = 0;
+                    it.slot[st] = 0;
+                    if (n > 0) it.n[st] = ceilDiv(rowLimit(it, st, n - 1), kTile);
+                }
+            }
+            return true;
+        }
+        w.before += total;
+        w.base += 32;
+        if (w.base >= p.seqs) {
+            w.base = 0;
+            if (--w.level < 0) return false;
+        }
+    }
+}
+
+// ---- scheduling: a shared prefix ------------------------------------------------------
+// Items 0 .. pre_items-1: (key split, kv head, query tile or pair) over the
+// prefix, all tokens of the batch as rows; then (request, key chunk, kv head,
+// query tile) over the requests' own keys. Every item writes its slots.
+__device__ void prefixItem(const Params& p, int idx, Item& it) {
+    it.live = 1;
+    it.page_row = 0;
+    it.key0 = 0;
+    if (idx < p.pre_items) {
+        const int mt = idx % p.pre_mt;
+        const int r = idx / p.pre_mt;
+        const int split = r / p.kv_heads;
+        it.kvh = r % p.kv_heads;
+        const int first = split * p.pre_tiles * kTile;
+        int last = first + p.pre_tiles * kTile;
+        last = last < p.prefix ? last : p.prefix;
+        it.paired = p.pre_paired;
+        it.causal = 0;
+        it.src = 0;
+        it.k_row = first;
+        it.nk = last - first;
+        const int tiles = ceilDiv(it.nk, kTile), tokens = p.batch * p.steps;
+        for (int st = 0; st < 2; ++st) {
+            const int t0 = (p.pre_paired ? 2 * mt + st : mt) * p.tt;
+            int n = tokens - t0;
+            n = n < 0 ? 0 : n < p.tt ? n : p.tt;
+            it.q_row[st] = t0;
+            it.tok[st] = n;
+            it.vis0[st] = 0;
+            it.n[st] = n <= 0 ? 0 : p.pre_paired ? tiles : (tiles + 1 - st) / 2;
+            it.slot[st] = p.pre_paired ? split : 2 * split + st;
+        }
+        return;
+    }
+    idx -= p.pre_items;
+    const int mt = idx % p.suf_mt;
+    int r = idx / p.suf_mt;
+    it.kvh = r % p.kv_heads;
+    r /= p.kv_heads;
+    const int chunk = r % p.suf_chunks, b = r / p.suf_chunks;
+    const int cap = p.wide * p.page;
+    int len = p.lens[b];
+    if (len < 0 || len > cap) {
+        if (p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
+        len = len < 0 ? 0 : cap;
+    }
+    const int c0 = chunk * p.suf_keys;
+    int nk = len - c0;
+    nk = nk < 0 ? 0 : nk < p.suf_keys ? nk : p.suf_keys;
+    it.paired = 0;
+    it.causal = 1;
+    it.src = 1;
+    it.nk = nk;
+    it.k_row = p.pages == nullptr ? b * cap + c0 : 0;
+    it.page_row = b * p.wide;
+    it.key0 = c0;
+    const int t0 = mt * p.tt;
+    int n = p.steps - t0;
+    n = n < p.tt ? n : p.tt;
+    it.vis0[0] = it.vis0[1] = len - p.steps + t0 + 1 - c0;
+    const int tiles = ceilDiv(rowLimit(it, 0, n - 1), kTile);
+    const int slot = (p.pre_paired ? 1 : 2) * p.pre_splits + 2 * chunk;
+    for (int st = 0; st < 2; ++st) {
+        it.q_row[st] = b * p.steps + t0;
+        it.tok[st] = n;
+        it.n[st] = (tiles + 1 - st) / 2;
+        it.slot[st] = slot + st;
+    }
+}
+
+// ---- one row, key by key ----------------------------------------------------------------
+__device__ __forceinline__ int pageRow(const Params& p, const Item& it, int key) {
+    const int at = it.key0 + key;
+    const int pg = p.pages[it.page_row + (at >> p.page_shift)];
+    // an index outside the pages reads rows past the map's end, which load as zeros
+    return (pg < 0 || pg >= p.n_pages) ? -1 : (pg << p.page_shift) + (at & (p.page - 1));
+}
+
+// Row `row` of the query tile from the definition, over the keys its stream
+// has and the row sees: o (normalised) and the log2 of its sum.
+template <int D, typename T>
+__device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, int row, float* o) {
+    const int token = row / p.group, head = it.kvh * p.group + row % p.group;
+    const T* q = static_cast<const T*>(p.q) + (it.q_row[st] + token) * p.q_row + head * p.q_head;
+    const KeySource& src = p.src[it.src];
+    const int lim = rowLimit(it, st, token);
+    float m = -INFINITY, l = 0.0f;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int c = 0; c < D; ++c) o[c] = 0.0f;
+        for (int key = 0; key < lim; ++key) {
+            if (!it.paired && ((key / kTile) & 1) != st) continue;
+            int64_t krow = it.k_row + static_cast<int64_t>(key);
+            if (it.src == 1 && p.pages != nullptr) krow = pageRow(p, it, key);
+            const T* k = static_cast<const T*>(src.k) + krow * src.k_row + it.kvh * src.k_head;
+            const T* v = static_cast<const T*>(src.v) + krow * src.v_row + it.kvh * src.v_head;
+            float s = 0.0f;
+            if (krow >= 0) {
+                for (int c = 0; c < p.d; c += 8) {
+                    float a[8], b[8];
+                    unpack8<T>(*reinterpret_cast<const uint4*>(q + c), a);
+                    unpack8<T>(*reinterpret_cast<const uint4*>(k + c), b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
+                }
+            }
+            if (pass == 0) {
+                m = (s > m || s != s) ? s : m;  // a NaN score stays
+                if (m != m) break;
+                continue;
+            }
+            const float e = tc::ex2((s - m) * p.c2);
+            l += e;
+            if (krow >= 0) {
+                for (int c = 0; c < p.d; c += 8) {
+                    float b[8];
+                    unpack8<T>(*reinterpret_cast<const uint4*>(v + c), b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[c + i] = fmaf(e, b[i], o[c + i]);
+                }
+            }
+        }
+        if (m == -INFINITY) return -INFINITY;  // nothing to see: zeros
+    }
+    const float inv = 1.0f / l;
+    for (int c = 0; c < D; ++c) o[c] *= inv;
+    return fmaf(m, p.c2, log2f(l));
+}
+
+// ---- the kernel ---------------------------------------------------------------------------
+template <int D, typename T, bool kPrefix>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
+                  const __grid_constant__ CUtensorMap map_k0,
+                  const __grid_constant__ CUtensorMap map_v0,
+                  const __grid_constant__ CUtensorMap map_k1,
+                  const __grid_constant__ CUtensorMap map_v1, const __grid_constant__ Params p) {
+    using Sm = Smem<D>;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
+    if ((tc::smem_u32(smem_raw) & 1023u) != 0) {  // uniform: the swizzled tiles need this base
+        if (threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            tc::mbar_init(&sm.full[i], 1);
+            tc::mbar_init(&sm.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&sm.qfull[i], 1);
+            tc::mbar_init(&sm.qempty[i], 1);
+            tc::mbar_init(&sm.sfull[i], 1);
+            tc::mbar_init(&sm.pfull[i], 4);
+            tc::mbar_init(&sm.ofull[i], 1);
+        }
+        for (int i = 0; i < kItems; ++i) {
+            tc::mbar_init(&sm.ifull[i], 1);
+            tc::mbar_init(&sm.iempty[i], kConsumers);
+        }
+        sm.abort = 0;
+        tc::fence_barrier_init();
+        tc::fence_proxy_async();
+    }
+    if (warp == 8) tc::tmem_alloc(&sm.tmem_base, 512);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    // Set-up overlaps the tail of the preceding grid; everything global waits for it.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = sm.tmem_base;
+    volatile int* abort = &sm.abort;
+
+    // Item `i` of this CTA (waits for the scheduler); false: no more, or aborted.
+    auto take = [&](uint32_t i, Item& it) -> bool {
+        const uint32_t r = i % kItems;
+        if (!tc::mbar_wait(&sm.ifull[r], (i / kItems) & 1u, abort, kLimitNs)) return false;
+        it = sm.item[r];
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.iempty[r]);
+        return it.live != 0;
+    };
+
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+      if (warp == 10) {
+        // ---------------- scheduler ----------------
+        Walker w = {0, 0, 0};
+        if constexpr (!kPrefix) {
+            int most = 0;
+            for (int s = lane; s - lane < p.seqs; s += 32) {
+                const Seq q = loadSeq(p, s);
+                if (q.nq > 0 && q.nk > most) most = q.nk;
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            w.level = ceilDiv(most, kTile);
+        }
+        for (uint32_t i = 0;; ++i) {
+            const uint32_t r = i % kItems;
+            if (i >= kItems &&
+                !tc::mbar_wait(&sm.iempty[r], ((i / kItems) - 1) & 1u, abort, kLimitNs)) {
+                break;
+            }
+            // back and forth over the grid: even rounds ascending, odd descending
+            const int64_t at = static_cast<int64_t>(i) * gridDim.x +
+                               ((i & 1u) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            bool live;
+            if constexpr (kPrefix) {
+                live = at < p.pre_items + p.suf_items;
+                if (live && lane == 0) prefixItem(p, static_cast<int>(at), sm.item[r]);
+            } else {
+                live = nextPacked(p, w, at, sm.item[r], lane);
+            }
+            if (!live && lane == 0) sm.item[r].live = 0;
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sm.ifull[r]);
+            if (!live) break;
+        }
+      } else if (warp == 9) {
+        // ---------------- TMA producer ----------------
+        uint32_t ring = 0, qn[2] = {0, 0};
+        Item it;
+        bool ok = true;
+        auto load_q = [&](int st) -> bool {
+            if (qn[st] > 0 && !tc::mbar_wait(&sm.qempty[st], (qn[st] - 1) & 1u, abort, kLimitNs)) {
+                return false;
+            }
+            ++qn[st];
+            if (lane == 0) {
+                tc::mbar_arrive_expect_tx(&sm.qfull[st], Sm::kHalves * 128u * p.group * p.tt);
+                for (int h = 0; h < Sm::kHalves; ++h) {
+                    tc::tma_load_3d(sm.q[st] + h * Sm::kBox, &map_q, &sm.qfull[st], h * 64,
+                                    it.kvh * p.group, it.q_row[st]);
+                }
+            }
+            __syncwarp();
+            return true;
+        };
+        auto load_kv = [&](const CUtensorMap* map, int tile) -> bool {
+            const uint32_t st = ring % kStages;
+            if (!tc::mbar_wait(&sm.empty[st], ((ring / kStages) & 1u) ^ 1u, abort, kLimitNs)) {
+                return false;
+            }
+            ++ring;
+            if (kPrefix && it.src == 1 && p.pages != nullptr) {
+                // one box per page (or one tile of a larger page); pages past the last key stay out
+                const int box = p.page < kTile ? p.page : kTile;
+                int keys = it.nk - tile * kTile;
+                keys = keys < kTile ? keys : kTile;
+                const int boxes = ceilDiv(keys, box);
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(&sm.full[st], Sm::kHalves * 128u * box * boxes);
+                }
+                __syncwarp();
+                if (lane < boxes) {
+                    int row = pageRow(p, it, tile * kTile + lane * box);
+                    if (row < 0) {
+                        row = p.n_pages << p.page_shift;
+                        if (p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
+                    }
+                    for (int h = 0; h < Sm::kHalves; ++h) {
+                        tc::tma_load_3d(sm.kv[st] + h * Sm::kBox + lane * box * 128, map,
+                                        &sm.full[st], h * 64, it.kvh, row);
+                    }
+                }
+                __syncwarp();
+            } else if (lane == 0) {
+                tc::mbar_arrive_expect_tx(&sm.full[st], Sm::kTileBytes);
+                for (int h = 0; h < Sm::kHalves; ++h) {
+                    tc::tma_load_3d(sm.kv[st] + h * Sm::kBox, map, &sm.full[st], h * 64, it.kvh,
+                                    it.k_row + tile * kTile);
+                }
+            }
+            __syncwarp();
+            return true;
+        };
+        for (uint32_t i = 0; ok && take(i, it); ++i) {
+            const int tiles = itemTiles(it);
+            const CUtensorMap* mk = kPrefix && it.src == 1 ? &map_k1 : &map_k0;
+            const CUtensorMap* mv = kPrefix && it.src == 1 ? &map_v1 : &map_v0;
+            if (tiles > 0 && (it.n[0] > 0 || !it.paired)) ok = load_q(0);
+            for (int t = 0; ok && t < tiles; ++t) {
+                ok = load_kv(mk, t);
+                if (ok && t == 0 && it.paired && it.n[1] > 0) ok = load_q(1);
+                ok = ok && load_kv(mv, t);
+            }
+        }
+        if (*abort) {  // copies in flight land before the CTA may exit
+            int never = 0;
+            for (uint32_t j = ring > kStages ? ring - kStages : 0; j < ring; ++j) {
+                (void)tc::mbar_wait(&sm.full[j % kStages], (j / kStages) & 1u, &never, kLimitNs);
+            }
+            for (int st = 0; st < 2; ++st) {
+                if (qn[st] > 0) {
+                    (void)tc::mbar_wait(&sm.qfull[st], (qn[st] - 1) & 1u, &never, kLimitNs);
+                }
+            }
+        }
+      } else if (warp == 8) {
+        // ---------------- MMA issuer ----------------
+        const int ksteps = ceilDiv(p.d, 16);
+        const uint32_t idesc_s = tc::idesc_f16_f32(kTile, kTile, 0, 0, kBf16);
+        const uint32_t idesc_o = tc::idesc_f16_f32(kTile, ksteps * 16, 0, 1, kBf16);
+        uint32_t ring = 0, qn[2] = {0, 0}, pn[2] = {0, 0};
+        Item it;
+        int tiles = 0;
+        // Scores of step u: S[stream] = Q[stream] K[tile]^T.
+        auto scores = [&](int u) -> bool {
+            if (!stepLive(it, u)) return true;
+            const int st = u & 1, tile = stepTile(it, u), qs = it.paired ? st : 0;
+            const uint32_t j = ring + 2 * tile, stage = j % kStages;
+            if ((it.paired ? tile == 0 : u == 0)) {
+                if (!tc::mbar_wait(&sm.qfull[qs], qn[qs] & 1u, abort, kLimitNs)) return false;
+                ++qn[qs];
+            }
+            if (!tc::mbar_wait(&sm.full[stage], (j / kStages) & 1u, abort, kLimitNs)) return false;
+            tc::tc_fence_after();
+            if (lane == 0) {
+                const uint32_t q0 = tc::smem_u32(sm.q[qs]), k0 = tc::smem_u32(sm.kv[stage]);
+                for (int kk = 0; kk < ksteps; ++kk) {
+                    const uint32_t off = (kk >> 2) * Sm::kBox + (kk & 3) * 32;
+                    tc::mma_f16(tmem + st * kTile, tc::smem_desc_sw128(q0 + off, 16, 1024),
+                                tc::smem_desc_sw128(k0 + off, 16, 1024), idesc_s, kk > 0);
+                }
+                // the tile's last reader releases it
+                const bool last = !it.paired || st == 1 || tile >= it.n[1];
+                if (last) tc::mma_commit(&sm.empty[stage]);
+                if (it.paired ? tile == it.n[st] - 1 : u == tiles - 1) tc::mma_commit(&sm.qempty[qs]);
+                tc::mma_commit(&sm.sfull[st]);
+            }
+            __syncwarp();
+            return true;
+        };
+        // Step u: O[stream] (+)= P[stream] V[tile].
+        auto values = [&](int u) -> bool {
+            if (!stepLive(it, u)) return true;
+            const int st = u & 1, tile = stepTile(it, u);
+            const uint32_t j = ring + 2 * tile + 1, stage = j % kStages;
+            if (!tc::mbar_wait(&sm.full[stage], (j / kStages) & 1u, abort, kLimitNs)) return false;
+            const int valid = it.nk - tile * kTile;
+            const bool first = !it.paired || st == 0 || tile >= it.n[0];
+            if (valid < kTile && first) {
+                for (int h = 0; h < Sm::kHalves; ++h) {
+                    uint4* z = reinterpret_cast<uint4*>(sm.kv[stage] + h * Sm::kBox);
+                    for (int x = valid * 8 + lane; x < kTile * 8; x += 32) z[x] = make_uint4(0, 0, 0, 0);
+                }
+                tc::fence_proxy_async();
+                __syncwarp();
+            }
+            if (!tc::mbar_wait(&sm.pfull[st], pn[st] & 1u, abort, kLimitNs)) return false;
+            ++pn[st];
+            tc::tc_fence_after();
+            if (lane == 0) {
+                const uint32_t v0 = tc::smem_u32(sm.kv[stage]);
+                const int jj = u >> 1;  // the stream's own tile count
+                for (int kk = 0; kk < kTile / 16; ++kk) {
+                    tc::mma_f16_ts(tmem + 2 * kTile + st * kTile, tmem + st * kTile + kk * 8,
+                                   tc::smem_desc_sw128(v0 + kk * 2048, Sm::kBox, 1024), idesc_o,
+                                   jj > 0 || kk > 0);
+                }
+                const bool last = !it.paired || st == 1 || tile >= it.n[1];
+                if (last) tc::mma_commit(&sm.empty[stage]);
+                if (jj == it.n[st] - 1) tc::mma_commit(&sm.ofull[st]);
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = true;
+        for (uint32_t i = 0; ok && take(i, it); ++i) {
+            tiles = itemTiles(it);
+            const int steps = it.paired ? 2 * tiles : tiles;
+            ok = scores(0) && scores(1);
+            for (int u = 0; ok && u < steps; ++u) ok = values(u) && scores(u + 2);
+            ring += 2 * tiles;
+        }
+      }
+    } else {
+        // ---------------- softmax and epilogue ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int st = warp >> 2, quarter = warp & 3;
+        const int row = quarter * 32 + lane;
+        const int token = row / p.group, head_in = row - token * p.group;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + st * kTile;
+        const uint32_t o_addr = tmem + lanes + 2 * kTile + st * kTile;
+        const int dcols = (p.d + 31) / 32;  // 32-column groups of the accumulator
+        uint32_t sn = 0, on = 0;
+        Item it;
+        bool ok = true;
+        for (uint32_t i = 0; ok && take(i, it); ++i) {
+            const int lim = rowLimit(it, st, token);
+            const bool mine = token < it.tok[st] && token < p.tt;
+            float m = -INFINITY, l = 0.0f;
+            for (int jj = 0; jj < it.n[st]; ++jj, ++sn) {
+                const int left = lim - (it.paired ? jj : 2 * jj + st) * kTile;  // keys the row sees
+                if (!tc::mbar_wait(&sm.sfull[st], sn & 1u, abort, kLimitNs)) {
+                    ok = false;
+                    break;
+                }
+                tc::tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_addr + c * 32, s[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc::tmem_ld_wait(s[c]);
+                if (__any_sync(0xffffffffu, left < kTile)) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) {
+                            if (c * 32 + x >= left) s[c][x] = __float_as_uint(-INFINITY);
+                        }
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        mx[c] = tc::max3(mx[c], __uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1]));
+                    }
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool grow = top > m + p.grow;
+                const bool any_grow = __any_sync(0xffffffffu, grow);
+                const float f = grow ? tc::ex2((m - top) * p.c2) : 1.0f;
+                m = grow ? top : m;
+                l *= f;
+                const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
+                float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) {
+                        const int y = 2 * x;
+                        const float a = tc::ex2(fmaf(__uint_as_float(s[2 * c + y / 32][y % 32]), p.c2, nm));
+                        const float b = tc::ex2(fmaf(__uint_as_float(s[2 * c + y / 32][y % 32 + 1]), p.c2, nm));
+                        sum[0] += a;
+                        sum[1] += b;
+                        w[x] = pack2<T>(a, b);
+                    }
+                    tc::tmem_st32(s_addr + c * 32, w);
+                }
+                l += sum[0] + sum[1];
+                if (any_grow && jj > 0) {  // after the probabilities: their registers are free now
+                    for (int c = 0; c < dcols; ++c) {
+                        uint32_t o[32];
+                        tc::tmem_ld32(o_addr + c * 32, o);
+                        tc::tmem_ld_wait(o);
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                        tc::tmem_st32(o_addr + c * 32, o);
+                    }
+                }
+                tc::tmem_st_wait();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sm.pfull[st]);
+            }
+            if (!ok) break;
+            // ---- the row's result ----
+            if (it.n[st] > 0) {
+                if (!tc::mbar_wait(&sm.ofull[st], on & 1u, abort, kLimitNs)) break;
+                ++on;
+                tc::tc_fence_after();
+            }
+            const int64_t tok_row = it.q_row[st] + token;
+            const int head = it.kvh * p.group + head_in;
+            const float inv = l > 0.0f ? 1.0f / l : l;  // 0 for a row that sees nothing; NaN stays
+            bool nan = l != l;
+            float* part = nullptr;
+            T* y = nullptr;
+            if constexpr (kPrefix) {
+                part = p.part + (it.slot[st] * p.rows + tok_row * p.heads + head) * p.d;
+            } else {
+                y = static_cast<T*>(p.y) + tok_row * p.y_row + head * p.y_head;
+            }
+            for (int c = 0; c < dcols; ++c) {
+                uint32_t o[32];
+                if (it.n[st] > 0) {
+                    tc::tmem_ld32(o_addr + c * 32, o);
+                    tc::tmem_ld_wait(o);
+                }
+#pragma unroll
+                for (int x = 0; x < 32; ++x) {
+                    // a row with no visible key: zeros, whatever the accumulator holds
+                    const float f = l == 0.0f ? 0.0f : __uint_as_float(o[x]) * inv;
+                    nan = nan || (f != f && c * 32 + x < p.d);
+                    o[x] = __float_as_uint(f);
+                }
+                if (mine) {
+#pragma unroll
+                    for (int x = 0; x < 32; x += 8) {
+                        if (c * 32 + x < p.d) {
+                            float f[8];
+#pragma unroll
+                            for (int z = 0; z < 8; ++z) f[z] = __uint_as_float(o[x + z]);
+                            if constexpr (kPrefix) {
+                                if (l != 0.0f) {
+                                    float4* out = reinterpret_cast<float4*>(part + c * 32 + x);
+                                    out[0] = make_float4(f[0], f[1], f[2], f[3]);
+                                    out[1] = make_float4(f[4], f[5], f[6], f[7]);
+                                }
+                            } else {
+                                *reinterpret_cast<uint4*>(y + c * 32 + x) = pack8<T>(f);
+                            }
+                        }
+                    }
+                }
+            }
+            float lse = l > 0.0f ? fmaf(m, p.c2, log2f(l)) : -INFINITY;
+            if (mine && nan) {
+                float o[D];
+                const Item again = it;
+                lse = slowRow<D, T>(p, again, st, row, o);
+                for (int c = 0; c < p.d; c += 2) {
+                    if constexpr (kPrefix) {
+                        *reinterpret_cast<float2*>(part + c) = make_float2(o[c], o[c + 1]);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(y + c) = pack2<T>(o[c], o[c + 1]);
+                    }
+                }
+            }
+            if (kPrefix && mine) p.lse[it.slot[st] * p.rows + tok_row * p.heads + head] = lse;
+            tc::tc_fence_before();  // the reads above come before the next item's products
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, 512);
+    }
+    if (threadIdx.x == 0 && sm.abort && p.status != nullptr) atomicExch(p.status, MLKB_ERR_TIMEOUT);
+}
+
+// ---- joining the partial results of attention_prefix ----------------------------------------
+// One warp per result row: y = sum_i 2^(lse_i - top) o_i / sum_i 2^(lse_i - top)
+// over the row's slots; slots that saw no key have lse = -inf and are not read.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join(const float* __restrict__ part,
+                                                      const float* __restrict__ lse, int slots,
+                                                      int64_t rows, int heads, int d, T* y,
+                                                      int64_t y_row, int64_t y_head) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    float e[kMaxSlots / 32];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMaxSlots / 32; ++i) {
+        e[i] = lane + 32 * i < slots ? lse[(lane + 32 * i) * rows + row] : -INFINITY;
+        top = fmaxf(top, e[i]);
+    }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxSlots / 32; ++i) {
+        e[i] = e[i] == -INFINITY ? 0.0f : tc::ex2(e[i] - top);
+        sum += e[i];
+    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const bool live = 4 * lane < d;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kMaxSlots / 32; ++i) {
+#pragma unroll 8
+        for (int s = 0; s < 32; ++s) {
+            if (32 * i + s >= slots) break;
+            const float w = __shfl_sync(0xffffffffu, e[i], s);
+            if (w == 0.0f) continue;  // no key seen there, or nothing beside the others
+            if (live) {
+                const float4 v = *reinterpret_cast<const float4*>(
+                    part + ((32 * i + s) * rows + row) * d + 4 * lane);
+                acc.x = fmaf(w, v.x, acc.x);
+                acc.y = fmaf(w, v.y, acc.y);
+                acc.z = fmaf(w, v.z, acc.z);
+                acc.w = fmaf(w, v.w, acc.w);
+            }
+        }
+    }
+    if (live) {
+        T* out = y + (row / heads) * y_row + (row % heads) * y_head + 4 * lane;
+        *reinterpret_cast<uint2*>(out) =
+            make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------
+struct Maps {
+    CUtensorMap q, k0, v0, k1, v1;
+};
+
+// [rows, heads, d] view as a 3-D map, box [box_rows, box_heads, 64]. A view
+// without rows is never loaded from: it gets a stand-in address.
+int headsMap(CUtensorMap* map, const mlkb_heads& t, int64_t heads, int64_t d, int dtype,
+             int box_heads, int box_rows, const void* standin) {
+    const int64_t dims[3] = {d, heads, t.rows > 0 ? t.rows : 1};
+    const int64_t strides[2] = {t.head_stride, t.row_stride};
+    const int box[3] = {64, box_heads, box_rows};
+    return makeTmap3d(map,
+                      dtype == MLKB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                      2, t.rows > 0 ? t.data : standin, dims, strides, box,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int D, typename T, bool kPrefix>
+int launchKernel(const Maps& m, const Params& p, int grid, cudaStream_t s) {
+    static std::atomic<bool> attr[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    auto kernel = attention_tcgen05<D, T, kPrefix>;
+    if (dev >= 0 && dev < 64 && !attr[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(sizeof(Smem<D>)));
+        if (e != cudaSuccess) return setCudaError(MLKB_ERR_LAUNCH, e, "attention smem attribute");
+        // The register shares are taken from what the block is launched with:
+        // a build that gave the kernel fewer would wait for them for good.
+        cudaFuncAttributes fa;
+        const cudaError_t ea = cudaFuncGetAttributes(&fa, kernel);
+        if (ea != cudaSuccess) return setCudaError(MLKB_ERR_LAUNCH, ea, "attention attributes");
+        if (fa.numRegs * 12 < 8 * kSoftmaxRegs + 4 * kOtherRegs) {
+            return setError(MLKB_ERR_LAUNCH, "attention: kernel built with too few registers");
+        }
+        attr[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = sizeof(Smem<D>);
+    cfg.stream = s;
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, m.q, m.k0, m.v0, m.k1, m.v1, p);
+    return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention launch");
+}
+
+template <bool kPrefix>
+int launchAttention(const Maps& m, const Params& p, int dtype, int grid, cudaStream_t s) {
+    if (dtype == MLKB_F16) {
+        return p.d <= 64 ? launchKernel<64, __half, kPrefix>(m, p, grid, s)
+                         : launchKernel<128, __half, kPrefix>(m, p, grid, s);
+    }
+    return p.d <= 64 ? launchKernel<64, __nv_bfloat16, kPrefix>(m, p, grid, s)
+                     : launchKernel<128, __nv_bfloat16, kPrefix>(m, p, grid, s);
+}
+
+// Checks what both entries share.
+int checkShape(int64_t heads, int64_t kv_heads, int64_t d, double scale, int32_t dtype) {
+    if (dtype != MLKB_F16 && dtype != MLKB_BF16) {
+        return setError(MLKB_ERR_INVALID, "attention: dtype must be f16 or bf16");
+    }
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads / kv_heads > kTile ||
+        kv_heads > 65536) {
+        return setError(MLKB_ERR_INVALID,
+                        "attention: heads must be a multiple of kv heads, at most 128 to each");
+    }
+    if (d < 8 || d > 128 || d % 8 != 0) {
+        return setError(MLKB_ERR_INVALID, "attention: d must be a multiple of 8, 8 to 128");
+    }
+    const float c2 = static_cast<float>(scale * 1.4426950408889634);
+    if (!(scale > 0) || !std::isfinite(c2) || c2 < 1e-30f) {
+        return setError(MLKB_ERR_INVALID, "attention: scale must be positive and finite");
+    }
+    return MLKB_OK;
+}
+
+void setShape(Params& p, int64_t heads, int64_t kv_heads, int64_t d, double scale) {
+    p.heads = static_cast<int32_t>(heads);
+    p.kv_heads = static_cast<int32_t>(kv_heads);
+    p.group = static_cast<int32_t>(heads / kv_heads);
+    p.d = static_cast<int32_t>(d);
+    p.tt = kTile / p.group;
+    p.c2 = static_cast<float>(scale * 1.4426950408889634);
+    p.grow = kRescale / p.c2;
+    p.status = deviceStatusPtr();
+}
+
+KeySource keySource(const mlkb_heads& k, const mlkb_heads& v) {
+    return {k.data, v.data, k.row_stride, k.head_stride, v.row_stride, v.head_stride};
+}
+
+// How attention_prefix cuts its work, from shapes alone (the lengths are on
+// the device).
+struct PrefixPlan {
+    int64_t group, tt, tokens, rows;
+    int64_t paired, mt, tiles, splits, slots_pre, pre_items;
+    int64_t chunk, chunks, suf_mt, suf_items, slots;
+};
+
+PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_heads,
+                      int64_t prefix, int64_t cap) {
+    PrefixPlan r = {};
+    r.group = heads / kv_heads;
+    r.tt = kTile / r.group;
+    r.tokens = batch * steps;
+    r.rows = r.tokens * heads;
+    const int64_t sms = smCount();
+    const int64_t qt = (r.tokens + r.tt - 1) / r.tt;
+    r.paired = qt > 1;
+    r.mt = r.paired ? (qt + 1) / 2 : 1;
+    const int64_t tiles = (prefix + kTile - 1) / kTile;
+    if (tiles > 0) {
+        // About one item per SM, but no item shorter than 4 tiles and at most 16 splits.
+        const int64_t units = r.mt * kv_heads;
+        int64_t splits = (sms + units - 1) / units;
+        splits = splits < 16 ? splits : 16;
+        int64_t per = (tiles + splits - 1) / splits;
+        per = per > 4 ? per : 4;
+        r.tiles = per;
+        r.splits = (tiles + per - 1) / per;
+    }
+    r.slots_pre = r.splits * (r.paired ? 1 : 2);
+    r.pre_items = r.splits * kv_heads * r.mt;
+    r.suf_mt = (steps + r.tt - 1) / r.tt;
+    if (cap > 0) {
+        const int64_t units = batch * kv_heads * r.suf_mt;
+        const int64_t ctiles = (cap + kTile - 1) / kTile;
+        int64_t n = (2 * sms + units - 1) / units;
+        n = n < 16 ? n : 16;
+        int64_t per = (ctiles + n - 1) / n;
+        per = per > 4 ? per : 4;
+        r.chunk = per * kTile;
+        r.chunks = (ctiles + per - 1) / per;
+    }
+    r.suf_items = batch * kv_heads * r.suf_mt * r.chunks;
+    r.slots = r.slots_pre + 2 * r.chunks;
+    return r;
+}
+
+}  // namespace
+}  // namespace mlkb
+
+extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* v,
+                                     const mlkb_heads* y, int64_t heads, int64_t kv_heads,
+                                     int64_t d, const int32_t* q_starts, const int32_t* k_starts,
+                                     int64_t n_seqs, int32_t causal, double scale,
+                                     int32_t elem_dtype, void* stream) {
+    using namespace mlkb;
+    if (int st = checkShape(heads, kv_heads, d, scale, elem_dtype)) return st;
+    mlkb_heads hq = {}, hk = {}, hv = {}, hy = {};
+    if (int st = checkHeads(q, heads, d, false, "attention q", &hq)) return st;
+    if (int st = checkHeads(k, kv_heads, d, false, "attention k", &hk)) return st;
+    if (int st = checkHeads(v, kv_heads, d, false, "attention v", &hv)) return st;
+    if (int st = checkHeads(y, heads, d, true, "attention y", &hy)) return st;
+    if (hk.rows != hv.rows || hq.rows != hy.rows) {
+        return setError(MLKB_ERR_INVALID, "attention: k and v, and q and y, must have equal rows");
+    }
+    if (n_seqs < 0 || n_seqs > kMaxHeadRows) {
+        return setError(MLKB_ERR_INVALID, "attention: bad number of sequences");
+    }
+    if (n_seqs == 0 || hq.rows == 0) return okStatus();
+    if (q_starts == nullptr || k_starts == nullptr ||
+        ((reinterpret_cast<uintptr_t>(q_starts) | reinterpret_cast<uintptr_t>(k_starts)) & 3u) != 0) {
+        return setError(MLKB_ERR_INVALID, "attention: q_starts and k_starts needed");
+    }
+    if (int st = needDevice()) return st;
+    Params p = {};
+    setShape(p, heads, kv_heads, d, scale);
+    p.q = hq.data;
+    p.q_row = hq.row_stride;
+    p.q_head = hq.head_stride;
+    p.src[0] = keySource(hk, hv);
+    p.y = hy.data;
+    p.y_row = hy.row_stride;
+    p.y_head = hy.head_stride;
+    p.q_starts = q_starts;
+    p.k_starts = k_starts;
+    p.seqs = static_cast<int32_t>(n_seqs);
+    p.q_rows = static_cast<int32_t>(hq.rows);
+    p.k_rows = static_cast<int32_t>(hk.rows);
+    p.causal = causal != 0;
+    Maps m;
+    if (int st = headsMap(&m.q, hq, heads, d, elem_dtype, p.group, p.tt, nullptr)) return st;
+    if (int st = headsMap(&m.k0, hk, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
+    if (int st = headsMap(&m.v0, hv, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
+    m.k1 = m.k0;
+    m.v1 = m.v0;
+    // Most pairs of query tiles there can be: every sequence may end inside one.
+    const int64_t pairs = hq.rows / (2 * p.tt) + (n_seqs < hq.rows ? n_seqs : hq.rows);
+    const int64_t items = pairs * kv_heads;
+    const int grid = static_cast<int>(items < smCount() ? items : smCount());
+    return launchAttention<false>(m, p, elem_dtype, grid, asStream(stream));
+}
+
+extern "C" int64_t mlkb_attention_prefix_workspace(int64_t batch, int64_t steps, int64_t heads,
+                                                   int64_t kv_heads, int64_t d, int64_t prefix_rows,
+                                                   int64_t page_size, int64_t pages_per_request) {
+    using namespace mlkb;
+    if (batch < 0 || steps < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
+        heads / kv_heads > kTile || d < 8 || d > 128 || prefix_rows < 0 || page_size < 0 ||
+        pages_per_request < 0 || batch > kMaxHeadRows || steps > kMaxHeadRows || heads > (1 << 23) ||
+        prefix_rows > kMaxHeadRows || page_size > kMaxHeadRows || pages_per_request > kMaxHeadRows) {
+        return -1;
+    }
+    const PrefixPlan r =
+        planPrefix(batch, steps, heads, kv_heads, prefix_rows, page_size * pages_per_request);
+    return r.slots * r.rows * (d + 1) * 4;
+}
+
+extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* prefix_k,
+                                     const mlkb_heads* prefix_v, const mlkb_heads* k_pages,
+                                     const mlkb_heads* v_pages, const mlkb_heads* y, int64_t batch,
+                                     int64_t steps, int64_t heads, int64_t kv_heads, int64_t d,
+                                     int64_t page_size, int64_t pages_per_request,
+                                     const int32_t* pages, const int32_t* lens, double scale,
+                                     int32_t elem_dtype, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+    using namespace mlkb;
+    if (int st = checkShape(heads, kv_heads, d, scale, elem_dtype)) return st;
+    mlkb_heads hq = {}, hpk = {}, hpv = {}, hk = {}, hv = {}, hy = {};
+    if (int st = checkHeads(q, heads, d, false, "attention q", &hq)) return st;
+    if (int st = checkHeads(prefix_k, kv_heads, d, false, "attention prefix_k", &hpk)) return st;
+    if (int st = checkHeads(prefix_v, kv_heads, d, false, "attention prefix_v", &hpv)) return st;
+    if (int st = checkHeads(k_pages, kv_heads, d, false, "attention k_pages", &hk)) return st;
+    if (int st = checkHeads(v_pages, kv_heads, d, false, "attention v_pages", &hv)) return st;
+    if (int st = checkHeads(y, heads, d, true, "attention y", &hy)) return st;
+    if (batch < 0 || steps < 1 || batch > kMaxHeadRows || steps > kMaxHeadRows ||
+        hq.rows != batch * steps || hy.rows != hq.rows) {
+        return setError(MLKB_ERR_INVALID, "attention: q and y must have batch * steps rows");
+    }
+    if (hpk.rows != hpv.rows || hk.rows != hv.rows) {
+        return setError(MLKB_ERR_INVALID, "attention: k and v must have equal rows");
+    }
+    if (page_size < 0 || pages_per_request < 0 || page_size > kMaxHeadRows ||
+        pages_per_request > kMaxHeadRows) {
+        return setError(MLKB_ERR_INVALID, "attention: bad page size or page count");
+    }
+    const int64_t cap = page_size * pages_per_request;
+    if (cap > kMaxHeadRows) return setError(MLKB_ERR_INVALID, "attention: a request may hold 2^30 keys");
+    if (pages != nullptr) {
+        if (page_size < 16 || (page_size & (page_size - 1)) != 0 || hk.rows % page_size != 0) {
+            return setError(MLKB_ERR_INVALID,
+                            "attention: page size must be a power of two from 16 on, and the pages "
+                            "whole");
+        }
+        if (batch * pages_per_request > INT_MAX) {
+            return setError(MLKB_ERR_INVALID, "attention: page table too large");
+        }
+    } else if (cap > 0 && (pages_per_request != 1 || hk.rows != batch * page_size)) {
+        return setError(MLKB_ERR_INVALID,
+                        "attention: without a page table each request has one page, in order");
+    }
+    if (hq.rows == 0) return okStatus();
+    if (cap > 0 && (lens == nullptr || ((reinterpret_cast<uintptr_t>(lens) |
+                                         reinterpret_cast<uintptr_t>(pages)) & 3u) != 0)) {
+        return setError(MLKB_ERR_INVALID, "attention: lens needed");
+    }
+    const PrefixPlan r = planPrefix(batch, steps, heads, kv_heads, hpk.rows, cap);
+    if (r.pre_items + r.suf_items > INT_MAX || r.slots > kMaxSlots) {
+        return setError(MLKB_ERR_INVALID, "attention: too much work for one call");
+    }
+    if (workspace_bytes < r.slots * r.rows * (d + 1) * 4 ||
+        (r.slots > 0 && (workspace == nullptr || !aligned16(workspace)))) {
+        return setError(MLKB_ERR_INVALID,
+                        "attention: workspace (16-byte aligned) smaller than "
+                        "mlkb_attention_prefix_workspace says");
+    }
+    if (int st = needDevice()) return st;
+    Params p = {};
+    setShape(p, heads, kv_heads, d, scale);
+    p.q = hq.data;
+    p.q_row = hq.row_stride;
+    p.q_head = hq.head_stride;
+    p.src[0] = keySource(hpk, hpv);
+    p.src[1] = keySource(hk, hv);
+    p.lens = lens;
+    p.pages = pages;
+    p.batch = static_cast<int32_t>(batch);
+    p.steps = static_cast<int32_t>(steps);
+    p.prefix = static_cast<int32_t>(hpk.rows);
+    p.page = static_cast<int32_t>(page_size);
+    p.wide = static_cast<int32_t>(pages_per_request);
+    if (pages != nullptr) {
+        while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
+        p.n_pages = static_cast<int32_t>(hk.rows / page_size);
+    }
+    p.pre_items = static_cast<int32_t>(r.pre_items);
+    p.pre_tiles = static_cast<int32_t>(r.tiles);
+    p.pre_splits = static_cast<int32_t>(r.splits);
+    p.pre_mt = static_cast<int32_t>(r.mt);
+    p.pre_paired = static_cast<int32_t>(r.paired);
+    p.suf_items = static_cast<int32_t>(r.suf_items);
+    p.suf_keys = static_cast<int32_t>(r.chunk);
+    p.suf_chunks = static_cast<int32_t>(r.chunks);
+    p.suf_mt = static_cast<int32_t>(r.suf_mt);
+    p.rows = r.rows;
+    p.part = static_cast<float*>(workspace);
+    p.lse = p.part + r.slots * r.rows * d;
+    Maps m;
+    const int box = pages != nullptr && page_size < kTile ? static_cast<int>(page_size) : kTile;
+    if (int st = headsMap(&m.q, hq, heads, d, elem_dtype, p.group, p.tt, nullptr)) return st;
+    if (int st = headsMap(&m.k0, hpk, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
+    if (int st = headsMap(&m.v0, hpv, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
+    if (int st = headsMap(&m.k1, hk, kv_heads, d, elem_dtype, 1, box, hq.data)) return st;
+    if (int st = headsMap(&m.v1, hv, kv_heads, d, elem_dtype, 1, box, hq.data)) return st;
+    const int64_t items = r.pre_items + r.suf_items;
+    cudaStream_t s = asStream(stream);
+    if (items > 0) {
+        const int grid = static_cast<int>(items < smCount() ? items : smCount());
+        if (int st = launchAttention<true>(m, p, elem_dtype, grid, s)) return st;
+    }
+    const int64_t blocks = (r.rows + 7) / 8;
+    if (blocks > INT_MAX) return setError(MLKB_ERR_INVALID, "attention: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    const float* part = p.part;
+    const float* lse = p.lse;
+    const int slots = static_cast<int>(r.slots);
+    const cudaError_t e =
+        elem_dtype == MLKB_F16
+            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, slots, r.rows, p.heads, p.d,
+                                 static_cast<__half*>(hy.data), hy.row_stride, hy.head_stride)
+            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, slots, r.rows,
+                                 p.heads, p.d, static_cast<__nv_bfloat16*>(hy.data), hy.row_stride,
+                                 hy.head_stride);
+    return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention join launch");
+}

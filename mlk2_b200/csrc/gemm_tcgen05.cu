@@ -472,6 +472,26 @@ int makeTmap2d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const
     return r == CUDA_SUCCESS ? okStatus() : setError(MLKB_ERR_INVALID, "tensor map encode failed");
 }
 
+// 3-D tensor map, dims and box innermost first; strides of the two outer
+// dimensions in elements. Out-of-range elements load as zero.
+int makeTmap3d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base,
+               const int64_t (&dims)[3], const int64_t (&strides)[2], const int (&box)[3],
+               CUtensorMapSwizzle swizzle) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = encodeFn();
+    if (enc == nullptr) return setError(MLKB_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t d[3] = {static_cast<cuuint64_t>(dims[0]), static_cast<cuuint64_t>(dims[1]),
+                             static_cast<cuuint64_t>(dims[2])};
+    const cuuint64_t st[2] = {static_cast<cuuint64_t>(strides[0]) * elem_bytes,
+                              static_cast<cuuint64_t>(strides[1]) * elem_bytes};
+    const cuuint32_t b[3] = {static_cast<cuuint32_t>(box[0]), static_cast<cuuint32_t>(box[1]),
+                             static_cast<cuuint32_t>(box[2])};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, type, 3, const_cast<void*>(base), d, st, b, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? okStatus() : setError(MLKB_ERR_INVALID, "tensor map encode failed");
+}
+
 // 2-D f16 tensor map, 128-byte swizzle (box_cols * 2 must be 128).
 int makeTmapF16(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows,
                 int box_cols) {

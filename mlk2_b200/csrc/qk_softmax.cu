@@ -84,18 +84,8 @@ struct QkSmem {
 
 constexpr size_t kSmemBytes = sizeof(QkSmem);
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// max of three (NaN-avoiding like fmaxf: a NaN operand never wins).
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
+using tc::ex2;
+using tc::max3;
 
 // Lane-0 arrive after the whole warp is done with the guarded resource.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
