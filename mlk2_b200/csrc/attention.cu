@@ -64,6 +64,7 @@ constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;  // 8 x 200 + 4 x 104 = 12 x
 constexpr int kConsumers = 10;  // warps that read an item
 constexpr uint64_t kLimitNs = 2000000000ull;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
+constexpr int kPoly = 0;          // of 8 pairs of exponentials, how many go to the FMA pipe
 constexpr int kMaxSlots = 64;     // partial results a row may have
 
 // What one pass through the pipeline computes. Keys are counted from the
@@ -127,7 +128,7 @@ struct Smem {
     Item item[kItems];
     uint64_t full[kStages], empty[kStages];
     uint64_t qfull[2], qempty[2];
-    uint64_t sfull[2], pfull[2], ofull[2];
+    uint64_t sfull[2], pfull[2][2], ofull[2];  // pfull: [stream][half of the key tile]
     uint64_t ifull[kItems], iempty[kItems];
     uint32_t tmem_base;
     int abort;
@@ -136,7 +137,7 @@ struct Smem {
 __device__ __forceinline__ int ceilDiv(int a, int b) { return (a + b - 1) / b; }
 
 __device__ __forceinline__ int rowLimit(const Item& it, int st, int token) {
-    int v = it.causal ? it.vis0[st] + token : it.nk;
+    int v = it.causal ? (st == 0 ? it.vis0[0] : it.vis0[1]) + token : it.nk;
     v = v < 0 ? 0 : v;
     return v < it.nk ? v : it.nk;
 }
@@ -398,7 +399,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             tc::mbar_init(&sm.qfull[i], 1);
             tc::mbar_init(&sm.qempty[i], 1);
             tc::mbar_init(&sm.sfull[i], 1);
-            tc::mbar_init(&sm.pfull[i], 4);
+            tc::mbar_init(&sm.pfull[i][0], 4);
+            tc::mbar_init(&sm.pfull[i][1], 4);
             tc::mbar_init(&sm.ofull[i], 1);
         }
         for (int i = 0; i < kItems; ++i) {
@@ -563,17 +565,22 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             }
             if (!tc::mbar_wait(&sm.full[stage], (j / kStages) & 1u, abort, kLimitNs)) return false;
             tc::tc_fence_after();
-            if (lane == 0) {
-                const uint32_t q0 = tc::smem_u32(sm.q[qs]), k0 = tc::smem_u32(sm.kv[stage]);
-                for (int kk = 0; kk < ksteps; ++kk) {
-                    const uint32_t off = (kk >> 2) * Sm::kBox + (kk & 3) * 32;
-                    tc::mma_f16(tmem + st * kTile, tc::smem_desc_sw128(q0 + off, 16, 1024),
-                                tc::smem_desc_sw128(k0 + off, 16, 1024), idesc_s, kk > 0);
+            if (tc::elect_one()) {
+                const uint64_t q0 = tc::smem_desc_sw128(tc::smem_u32(sm.q[qs]), 16, 1024);
+                const uint64_t k0 = tc::smem_desc_sw128(tc::smem_u32(sm.kv[stage]), 16, 1024);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = ((kk >> 2) * Sm::kBox + (kk & 3) * 32) >> 4;
+                    if (kk < ksteps) {
+                        tc::mma_f16(tmem + st * kTile, q0 + off, k0 + off, idesc_s, kk > 0);
+                    }
                 }
                 // the tile's last reader releases it
                 const bool last = !it.paired || st == 1 || tile >= it.n[1];
                 if (last) tc::mma_commit(&sm.empty[stage]);
-                if (it.paired ? tile == it.n[st] - 1 : u == tiles - 1) tc::mma_commit(&sm.qempty[qs]);
+                if (it.paired ? tile == (st == 0 ? it.n[0] : it.n[1]) - 1 : u == tiles - 1) {
+                    tc::mma_commit(&sm.qempty[qs]);
+                }
                 tc::mma_commit(&sm.sfull[st]);
             }
             __syncwarp();
@@ -595,22 +602,29 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 tc::fence_proxy_async();
                 __syncwarp();
             }
-            if (!tc::mbar_wait(&sm.pfull[st], pn[st] & 1u, abort, kLimitNs)) return false;
-            ++pn[st];
-            tc::tc_fence_after();
-            if (lane == 0) {
-                const uint32_t v0 = tc::smem_u32(sm.kv[stage]);
-                const int jj = u >> 1;  // the stream's own tile count
-                for (int kk = 0; kk < kTile / 16; ++kk) {
-                    tc::mma_f16_ts(tmem + 2 * kTile + st * kTile, tmem + st * kTile + kk * 8,
-                                   tc::smem_desc_sw128(v0 + kk * 2048, Sm::kBox, 1024), idesc_o,
-                                   jj > 0 || kk > 0);
+            const int jj = u >> 1;  // the stream's own tile count
+            for (int half = 0; half < 2; ++half) {
+                if (!tc::mbar_wait(&sm.pfull[st][half], pn[st] & 1u, abort, kLimitNs)) return false;
+                tc::tc_fence_after();
+                if (tc::elect_one()) {
+                    const uint64_t v0 =
+                        tc::smem_desc_sw128(tc::smem_u32(sm.kv[stage]), Sm::kBox, 1024) + half * 512;
+                    const uint32_t p0 = tmem + st * kTile + half * 32;
+                    const uint32_t o0 = tmem + 2 * kTile + st * kTile;
+                    tc::mma_f16_ts(o0, p0, v0, idesc_o, jj > 0 || half > 0);
+#pragma unroll
+                    for (int q = 1; q < 4; ++q) {  // 16 keys: 2 KB of V
+                        tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, 1);
+                    }
+                    if (half == 1) {
+                        const bool last = !it.paired || st == 1 || tile >= it.n[1];
+                        if (last) tc::mma_commit(&sm.empty[stage]);
+                        if (jj == (st == 0 ? it.n[0] : it.n[1]) - 1) tc::mma_commit(&sm.ofull[st]);
+                    }
                 }
-                const bool last = !it.paired || st == 1 || tile >= it.n[1];
-                if (last) tc::mma_commit(&sm.empty[stage]);
-                if (jj == it.n[st] - 1) tc::mma_commit(&sm.ofull[st]);
+                __syncwarp();
             }
-            __syncwarp();
+            ++pn[st];
             return true;
         };
         bool ok = true;
@@ -637,10 +651,13 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         bool ok = true;
         for (uint32_t i = 0; ok && take(i, it); ++i) {
             const int lim = rowLimit(it, st, token);
-            const bool mine = token < it.tok[st] && token < p.tt;
+            const int n = st == 0 ? it.n[0] : it.n[1];
+            // keys the row sees from the stream's current tile on, and a tile's step
+            int left = lim - (it.paired ? 0 : st * kTile);
+            const int stride = it.paired ? kTile : 2 * kTile;
+            const bool mine = token < (st == 0 ? it.tok[0] : it.tok[1]) && token < p.tt;
             float m = -INFINITY, l = 0.0f;
-            for (int jj = 0; jj < it.n[st]; ++jj, ++sn) {
-                const int left = lim - (it.paired ? jj : 2 * jj + st) * kTile;  // keys the row sees
+            for (int jj = 0; jj < n; ++jj, ++sn, left -= stride) {
                 if (!tc::mbar_wait(&sm.sfull[st], sn & 1u, abort, kLimitNs)) {
                     ok = false;
                     break;
@@ -651,7 +668,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_addr + c * 32, s[c]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tc::tmem_ld_wait(s[c]);
-                if (__any_sync(0xffffffffu, left < kTile)) {
+                const bool masked = __any_sync(0xffffffffu, left < kTile);
+                if (masked) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -670,63 +688,87 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 const bool grow = top > m + p.grow;
-                const bool any_grow = __any_sync(0xffffffffu, grow);
-                const float f = grow ? tc::ex2((m - top) * p.c2) : 1.0f;
-                m = grow ? top : m;
-                l *= f;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? tc::ex2((m - top) * p.c2) : 1.0f;
+                    m = grow ? top : m;
+                    l *= f;
+                    if (jj > 0) {
+                        for (int c = 0; c < p.d; c += 16) {
+                            uint32_t o[16];
+                            tc::tmem_ld16(o_addr + c, o);
+                            tc::tmem_ld_wait(o);
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            tc::tmem_st16(o_addr + c, o);
+                        }
+                    }
+                }
                 const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
-                float sum[2] = {0.0f, 0.0f};
+                const uint64_t c2 = tc::pair(p.c2, p.c2), nm2 = tc::pair(nm, nm);
+                uint64_t sum[2] = {0, 0};
+                // Probabilities of the tile in two halves: the product with V
+                // starts on the first while the second is computed.
+                auto probabilities = [&](auto poly) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[32];
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[32];
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) {
-                        const int y = 2 * x;
-                        const float a = tc::ex2(fmaf(__uint_as_float(s[2 * c + y / 32][y % 32]), p.c2, nm));
-                        const float b = tc::ex2(fmaf(__uint_as_float(s[2 * c + y / 32][y % 32 + 1]), p.c2, nm));
-                        sum[0] += a;
-                        sum[1] += b;
-                        w[x] = pack2<T>(a, b);
+                        for (int x = 0; x < 32; ++x) {
+                            const int y = 2 * x;
+                            uint64_t v = tc::fma2(tc::pair(__uint_as_float(s[2 * c + y / 32][y % 32]),
+                                                           __uint_as_float(s[2 * c + y / 32][y % 32 + 1])),
+                                                  c2, nm2);
+                            if (poly.value && x % 8 < kPoly) {
+                                v = tc::ex2_poly(v);
+                            } else {
+                                const float2 z = tc::unpair(v);
+                                v = tc::pair(tc::ex2(z.x), tc::ex2(z.y));
+                            }
+                            sum[x & 1] = tc::add2(sum[x & 1], v);
+                            const float2 z = tc::unpair(v);
+                            w[x] = pack2<T>(z.x, z.y);
+                        }
+                        tc::tmem_st32(s_addr + c * 32, w);
+                        tc::tmem_st_wait();
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&sm.pfull[st][c]);
                     }
-                    tc::tmem_st32(s_addr + c * 32, w);
+                };
+                // Masked scores are -inf, which only ex2 takes to an exact 0.
+                if (masked) {
+                    probabilities(std::false_type{});
+                } else {
+                    probabilities(std::true_type{});
                 }
-                l += sum[0] + sum[1];
-                if (any_grow && jj > 0) {  // after the probabilities: their registers are free now
-                    for (int c = 0; c < dcols; ++c) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(o_addr + c * 32, o);
-                        tc::tmem_ld_wait(o);
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                        tc::tmem_st32(o_addr + c * 32, o);
-                    }
-                }
-                tc::tmem_st_wait();
-                tc::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&sm.pfull[st]);
+                const float2 z = tc::unpair(tc::add2(sum[0], sum[1]));
+                l += z.x + z.y;
             }
             if (!ok) break;
+            // No score above -inf: the row sees nothing. (A NaN score shows in l.)
+            if (m == -INFINITY && l < 0x1p60f) l = 0.0f;
             // ---- the row's result ----
-            if (it.n[st] > 0) {
+            if (n > 0) {
                 if (!tc::mbar_wait(&sm.ofull[st], on & 1u, abort, kLimitNs)) break;
                 ++on;
                 tc::tc_fence_after();
             }
-            const int64_t tok_row = it.q_row[st] + token;
+            const int64_t tok_row = (st == 0 ? it.q_row[0] : it.q_row[1]) + token;
+            const int slot = st == 0 ? it.slot[0] : it.slot[1];
             const int head = it.kvh * p.group + head_in;
             const float inv = l > 0.0f ? 1.0f / l : l;  // 0 for a row that sees nothing; NaN stays
-            bool nan = l != l;
+            // NaN somewhere: also seen as a sum no tile can have (ex2_poly)
+            bool nan = !(l < 0x1p60f);
             float* part = nullptr;
             T* y = nullptr;
             if constexpr (kPrefix) {
-                part = p.part + (it.slot[st] * p.rows + tok_row * p.heads + head) * p.d;
+                part = p.part + (slot * p.rows + tok_row * p.heads + head) * p.d;
             } else {
                 y = static_cast<T*>(p.y) + tok_row * p.y_row + head * p.y_head;
             }
             for (int c = 0; c < dcols; ++c) {
                 uint32_t o[32];
-                if (it.n[st] > 0) {
+                if (n > 0) {
                     tc::tmem_ld32(o_addr + c * 32, o);
                     tc::tmem_ld_wait(o);
                 }
@@ -770,7 +812,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     }
                 }
             }
-            if (kPrefix && mine) p.lse[it.slot[st] * p.rows + tok_row * p.heads + head] = lse;
+            if (kPrefix && mine) p.lse[slot * p.rows + tok_row * p.heads + head] = lse;
             tc::tc_fence_before();  // the reads above come before the next item's products
         }
     }

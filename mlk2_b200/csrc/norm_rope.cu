@@ -19,7 +19,8 @@ namespace {
 
 constexpr int kMaxAxes = 4;
 constexpr int kThreads = 256;
-constexpr int kSteps = 4;  // head-row steps a warp has in flight
+constexpr int kSteps = 2;   // head-row steps a warp has in flight
+constexpr int kBlocks = 4;  // blocks of an SM
 
 struct RopeParams {
     mlkb_heads q, k, qo, ko;
@@ -37,20 +38,40 @@ struct RopeParams {
 };
 
 template <typename T, int L, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocks) norm_rope_kernel(const RopeParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
-    const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-    const int64_t tok = warp / p.chunks;
+    const unsigned warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t tok = warp / static_cast<unsigned>(p.chunks);
     if (tok >= p.tokens) return;
-    const int step0 = static_cast<int>(warp - tok * p.chunks) * p.spw;
+    const int step0 = static_cast<int>(warp - static_cast<unsigned>(tok) * p.chunks) * p.spw;
     const int c = lane % L, sub = lane / L;
     const int half = p.rot >> 1, nrot = p.rot >> 4;
     const bool live = c < p.d / 16, turned = c < nrot;
     // element offsets of the lane's two vectors
     const int e0 = turned ? 8 * c : p.rot + 16 * (c - nrot);
     const int e1 = turned ? half + 8 * c : e0 + 8;
+    constexpr int kRowsPerStep = 32 / L;
+
+    uint4 va[kSteps], vb[kSteps];
+    int row[kSteps];
+    auto load = [&](int st) {
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+            row[u] = (st + u < step0 + p.spw) ? (st + u) * kRowsPerStep + sub : p.rows;
+            va[u] = vb[u] = make_uint4(0, 0, 0, 0);
+            if (live && row[u] < p.rows) {
+                const bool isq = row[u] < p.heads;
+                const mlkb_heads& v = isq ? p.q : p.k;
+                const T* x = static_cast<const T*>(v.data) + tok * v.row_stride +
+                             (isq ? row[u] : row[u] - p.heads) * v.head_stride;
+                va[u] = *reinterpret_cast<const uint4*>(x + e0);
+                vb[u] = *reinterpret_cast<const uint4*>(x + e1);
+            }
+        }
+    };
+    load(step0);  // in flight under the position and the table row below
 
     // The lane's cosines and sines: for split pairs (i, i + half), pairs 8c..8c+7
     // serve both vectors; for neighbours (2i, 2i + 1), vector 0 holds pairs
@@ -98,23 +119,8 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeParams p)
         return;
     }
 
-    constexpr int kRowsPerStep = 32 / L;
     for (int st = step0; st < step0 + p.spw; st += kSteps) {
-        uint4 va[kSteps], vb[kSteps];
-        int row[kSteps];
-#pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            row[u] = (st + u < step0 + p.spw) ? (st + u) * kRowsPerStep + sub : p.rows;
-            va[u] = vb[u] = make_uint4(0, 0, 0, 0);
-            if (live && row[u] < p.rows) {
-                const bool isq = row[u] < p.heads;
-                const mlkb_heads& v = isq ? p.q : p.k;
-                const T* x = static_cast<const T*>(v.data) + tok * v.row_stride +
-                             (isq ? row[u] : row[u] - p.heads) * v.head_stride;
-                va[u] = *reinterpret_cast<const uint4*>(x + e0);
-                vb[u] = *reinterpret_cast<const uint4*>(x + e1);
-            }
-        }
+        if (st > step0) load(st);
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
             const bool isq = row[u] < p.heads;
@@ -189,10 +195,10 @@ int launchNormRope(RopeParams& p, bool interleaved, cudaStream_t s) {
     // Few tokens: a warp takes one step, so that they spread over the SMs. Many:
     // kSteps, whose loads are in flight together and share the table row.
     const int64_t all = static_cast<int64_t>(p.tokens) * steps;
-    p.spw = all <= static_cast<int64_t>(smCount()) * 32 ? 1 : kSteps;
-    p.chunks = (steps + p.spw - 1) / p.spw;
+    p.chunks = all <= static_cast<int64_t>(smCount()) * 32 ? steps : (steps + kSteps - 1) / kSteps;
+    p.spw = (steps + p.chunks - 1) / p.chunks;
     const int64_t blocks = (static_cast<int64_t>(p.tokens) * p.chunks + kThreads / 32 - 1) / (kThreads / 32);
-    if (blocks > 0x7fffffff) return setError(MLKB_ERR_INVALID, "norm_rope: too many head rows");
+    if (blocks > 0x7fffffff / (kThreads / 32)) return setError(MLKB_ERR_INVALID, "norm_rope: too many head rows");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks));
     cfg.blockDim = dim3(kThreads);
