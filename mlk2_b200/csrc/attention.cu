@@ -8,12 +8,15 @@
 //
 // One CTA per SM, persistent. Two streams of work per CTA, each with its own
 // 128-row query tile, score accumulator and softmax warps:
-//   warps 0-3    stream 0: softmax and epilogue, one thread per row
-//   warps 4-7    stream 1: the same
-//   warp 8       MMA issuer
-//   warp 9       TMA producer (Q tiles; K and V tiles of 128 keys in a ring)
-//   warp 10      scheduler: writes the items into a ring for the other warps
-//   warp 11      idle (register shares move by groups of four warps)
+//   warps 0-7    stream 0: softmax and epilogue. Two threads share a row, one
+//                for each half of a tile's 64 + 64 keys; they exchange the
+//                half maxima through shared memory (a row in one thread made
+//                the softmax twice as long a chain between two products)
+//   warps 8-15   stream 1: the same
+//   warp 16      MMA issuer
+//   warp 17      TMA producer (Q tiles; K and V tiles of 128 keys in a ring)
+//   warp 18      scheduler: writes the items into a ring for the other warps
+//   warp 19      idle (register shares move by groups of four warps)
 // TMEM: two score tiles (128 f32 columns each; the tile's probabilities
 // overwrite its first half as 16-bit pairs and are the A operand of P V) and
 // two output accumulators (128 columns each). For one stream the issuer
@@ -60,19 +63,20 @@ constexpr int kTile = 128;   // rows of a query tile, keys of a key tile
 constexpr int kItems = 3;    // item ring
 constexpr int kStages = 5;   // K / V ring
 constexpr int kThreads = 12 * 32;
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;  // 8 x 200 + 4 x 104 = 12 x 168 as launched
-constexpr int kConsumers = 10;  // warps that read an item
+constexpr int kMma = 8, kTma = 9, kSched = 10;  // warps; 0 to 7 are softmax warps, 11 is idle
+constexpr int kConsumers = 10;                  // warps that read an item
+constexpr int kFirst = 6;  // 16-key steps of a tile's probabilities that are handed on first
 constexpr uint64_t kLimitNs = 2000000000ull;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
 constexpr int kPoly = 0;          // of 8 pairs of exponentials, how many go to the FMA pipe
-constexpr int kMaxSlots = 64;     // partial results a row may have
+constexpr int kMaxSlots = 32;     // partial results a row may have
 
 // What one pass through the pipeline computes. Keys are counted from the
 // item's first; row limits (how many keys token i of a stream sees) are
 // clamp(vis0 + i, 0, nk) when causal, nk otherwise.
 struct Item {
     int32_t live;      // 0: no more items
-    int32_t paired;    // streams: two query tiles over all key tiles / one over alternate key tiles
+    int32_t paired;    // streams: two query tiles over all keys / one, over alternate key tiles
     int32_t causal;
     int32_t src;       // key source: 0 = rows of map 0, 1 = rows or pages of map 1
     int32_t kvh;
@@ -84,7 +88,7 @@ struct Item {
     int32_t tok[2];    // its tokens
     int32_t n[2];      // its key tiles
     int32_t vis0[2];
-    int32_t slot[2];   // partial-result slot (prefix)
+    int32_t slot;      // partial-result slot (prefix)
 };
 
 struct KeySource {
@@ -128,11 +132,16 @@ struct Smem {
     Item item[kItems];
     uint64_t full[kStages], empty[kStages];
     uint64_t qfull[2], qempty[2];
-    uint64_t sfull[2], pfull[2][2], ofull[2];  // pfull: [stream][half of the key tile]
+    uint64_t sfull[2], ofull[2];        // [stream]
+    uint64_t pfull[2][2];               // [stream][first part of the tile's keys, rest]
+    uint64_t xbar[4];                   // [lane quarter]: the streams' warps meet
     uint64_t ifull[kItems], iempty[kItems];
+    float2 xch[2][kTile];               // [stream][row]: maximum and sum
     uint32_t tmem_base;
     int abort;
 };
+
+static_assert(sizeof(Smem<128>) <= 227 * 1024, "shared memory of a block");
 
 __device__ __forceinline__ int ceilDiv(int a, int b) { return (a + b - 1) / b; }
 
@@ -142,14 +151,17 @@ __device__ __forceinline__ int rowLimit(const Item& it, int st, int token) {
     return v < it.nk ? v : it.nk;
 }
 
-// Key tiles of an item, and the tile of step u of its pipeline (stream u & 1).
+// Key tiles of an item.
 __device__ __forceinline__ int itemTiles(const Item& it) {
     return it.paired ? (it.n[0] > it.n[1] ? it.n[0] : it.n[1]) : it.n[0] + it.n[1];
 }
-__device__ __forceinline__ bool stepLive(const Item& it, int u) {
-    return (u >> 1) < it.n[u & 1];
+
+// Key tiles of the two streams of one query tile whose rows see at most `keys` keys.
+__device__ __forceinline__ void splitTiles(Item& it, int keys) {
+    const int tiles = ceilDiv(keys, kTile);
+    it.n[0] = (tiles + 1) / 2;
+    it.n[1] = tiles / 2;
 }
-__device__ __forceinline__ int stepTile(const Item& it, int u) { return it.paired ? u >> 1 : u; }
 
 // ---- scheduling: packed prompts ------------------------------------------------------
 // Items are (sequence, pair of query tiles, kv head), dealt to the CTAs in
@@ -213,7 +225,6 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
             if (lane == src) {
                 const int pair = ceilDiv(s.nq, 2 * p.tt) - ge + rem / p.kv_heads;
                 it.live = 1;
-                it.paired = 1;
                 it.causal = p.causal;
                 it.src = 0;
                 it.kvh = rem % p.kv_heads;
@@ -221,6 +232,7 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
                 it.k_row = s.k0;
                 it.page_row = 0;
                 it.key0 = 0;
+                it.slot = 0;
                 for (int st = 0; st < 2; ++st) {
                     const int t0 = (2 * pair + st) * p.tt;
                     int n = s.nq - t0;
@@ -228,9 +240,14 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
                     it.q_row[st] = s.q0 + t0;
                     it.tok[st] = n;
                     it.vis0[st] = s.nk - s.nq + t0 + 1;
-                    it.n[st] = 0;
-                    it.slot[st] = 0;
-                    if (n > 0) it.n[st] = ceilDiv(rowLimit(it, st, n - 1), kTile);
+                    it.n[st] = n > 0 ? ceilDiv(rowLimit(it, st, n - 1), kTile) : 0;
+                }
+                it.paired = it.tok[1] > 0;
+                if (!it.paired) {
+                    it.q_row[1] = it.q_row[0];
+                    it.tok[1] = it.tok[0];
+                    it.vis0[1] = it.vis0[0];
+                    splitTiles(it, rowLimit(it, 0, it.tok[0] - 1));
                 }
             }
             return true;
@@ -265,7 +282,8 @@ __device__ void prefixItem(const Params& p, int idx, Item& it) {
         it.src = 0;
         it.k_row = first;
         it.nk = last - first;
-        const int tiles = ceilDiv(it.nk, kTile), tokens = p.batch * p.steps;
+        const int tokens = p.batch * p.steps;
+        it.slot = split;
         for (int st = 0; st < 2; ++st) {
             const int t0 = (p.pre_paired ? 2 * mt + st : mt) * p.tt;
             int n = tokens - t0;
@@ -273,9 +291,9 @@ __device__ void prefixItem(const Params& p, int idx, Item& it) {
             it.q_row[st] = t0;
             it.tok[st] = n;
             it.vis0[st] = 0;
-            it.n[st] = n <= 0 ? 0 : p.pre_paired ? tiles : (tiles + 1 - st) / 2;
-            it.slot[st] = p.pre_paired ? split : 2 * split + st;
+            it.n[st] = n > 0 ? ceilDiv(it.nk, kTile) : 0;
         }
+        if (!it.paired) splitTiles(it, it.nk);
         return;
     }
     idx -= p.pre_items;
@@ -304,14 +322,12 @@ __device__ void prefixItem(const Params& p, int idx, Item& it) {
     int n = p.steps - t0;
     n = n < p.tt ? n : p.tt;
     it.vis0[0] = it.vis0[1] = len - p.steps + t0 + 1 - c0;
-    const int tiles = ceilDiv(rowLimit(it, 0, n - 1), kTile);
-    const int slot = (p.pre_paired ? 1 : 2) * p.pre_splits + 2 * chunk;
+    it.slot = p.pre_splits + chunk;
     for (int st = 0; st < 2; ++st) {
         it.q_row[st] = b * p.steps + t0;
         it.tok[st] = n;
-        it.n[st] = (tiles + 1 - st) / 2;
-        it.slot[st] = slot + st;
     }
+    splitTiles(it, rowLimit(it, 0, n - 1));
 }
 
 // ---- one row, key by key ----------------------------------------------------------------
@@ -322,8 +338,8 @@ __device__ __forceinline__ int pageRow(const Params& p, const Item& it, int key)
     return (pg < 0 || pg >= p.n_pages) ? -1 : (pg << p.page_shift) + (at & (p.page - 1));
 }
 
-// Row `row` of the query tile from the definition, over the keys its stream
-// has and the row sees: o (normalised) and the log2 of its sum.
+// Row `row` of the query tile from the definition, over the item's keys that
+// the row sees: o (normalised) and the log2 of its sum.
 template <int D, typename T>
 __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, int row, float* o) {
     const int token = row / p.group, head = it.kvh * p.group + row % p.group;
@@ -334,7 +350,6 @@ __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, i
     for (int pass = 0; pass < 2; ++pass) {
         for (int c = 0; c < D; ++c) o[c] = 0.0f;
         for (int key = 0; key < lim; ++key) {
-            if (!it.paired && ((key / kTile) & 1) != st) continue;
             int64_t krow = it.k_row + static_cast<int64_t>(key);
             if (it.src == 1 && p.pages != nullptr) krow = pageRow(p, it, key);
             const T* k = static_cast<const T*>(src.k) + krow * src.k_row + it.kvh * src.k_head;
@@ -372,6 +387,26 @@ __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, i
     return fmaf(m, p.c2, log2f(l));
 }
 
+// Among each four lanes, lane q's v[i] becomes lane i's v[q].
+__device__ __forceinline__ void swap4(uint4& a, uint4& b, bool upper, int mask) {
+    uint4 x = upper ? a : b;
+    x.x = __shfl_xor_sync(0xffffffffu, x.x, mask);
+    x.y = __shfl_xor_sync(0xffffffffu, x.y, mask);
+    x.z = __shfl_xor_sync(0xffffffffu, x.z, mask);
+    x.w = __shfl_xor_sync(0xffffffffu, x.w, mask);
+    if (upper) {
+        a = x;
+    } else {
+        b = x;
+    }
+}
+__device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
+    swap4(v[0], v[1], (lane & 1) != 0, 1);
+    swap4(v[2], v[3], (lane & 1) != 0, 1);
+    swap4(v[0], v[2], (lane & 2) != 0, 2);
+    swap4(v[1], v[3], (lane & 2) != 0, 2);
+}
+
 // ---- the kernel ---------------------------------------------------------------------------
 template <int D, typename T, bool kPrefix>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -399,9 +434,11 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             tc::mbar_init(&sm.qfull[i], 1);
             tc::mbar_init(&sm.qempty[i], 1);
             tc::mbar_init(&sm.sfull[i], 1);
-            tc::mbar_init(&sm.pfull[i][0], 4);
-            tc::mbar_init(&sm.pfull[i][1], 4);
             tc::mbar_init(&sm.ofull[i], 1);
+            for (int j = 0; j < 2; ++j) {
+                tc::mbar_init(&sm.pfull[i][j], 4);
+                tc::mbar_init(&sm.xbar[2 * i + j], 2);
+            }
         }
         for (int i = 0; i < kItems; ++i) {
             tc::mbar_init(&sm.ifull[i], 1);
@@ -411,7 +448,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         tc::fence_barrier_init();
         tc::fence_proxy_async();
     }
-    if (warp == 8) tc::tmem_alloc(&sm.tmem_base, 512);
+    if (warp == kMma) tc::tmem_alloc(&sm.tmem_base, 512);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -421,19 +458,19 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
     const uint32_t tmem = sm.tmem_base;
     volatile int* abort = &sm.abort;
 
-    // Item `i` of this CTA (waits for the scheduler); false: no more, or aborted.
-    auto take = [&](uint32_t i, Item& it) -> bool {
-        const uint32_t r = i % kItems;
-        if (!tc::mbar_wait(&sm.ifull[r], (i / kItems) & 1u, abort, kLimitNs)) return false;
-        it = sm.item[r];
+    // Item `i` of this CTA once the scheduler has written it; null: no more, or
+    // aborted. It stays in the ring until drop(i).
+    auto take = [&](uint32_t i) -> const Item* {
+        const Item& it = sm.item[i % kItems];
+        if (!tc::mbar_wait(&sm.ifull[i % kItems], (i / kItems) & 1u, abort, kLimitNs)) return nullptr;
+        return it.live != 0 ? &it : nullptr;
+    };
+    auto drop = [&](uint32_t i) {
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.iempty[r]);
-        return it.live != 0;
+        if (lane == 0) tc::mbar_arrive(&sm.iempty[i % kItems]);
     };
 
-    if (warp >= 8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-      if (warp == 10) {
+    if (warp == kSched) {
         // ---------------- scheduler ----------------
         Walker w = {0, 0, 0};
         if constexpr (!kPrefix) {
@@ -466,10 +503,10 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             if (lane == 0) tc::mbar_arrive(&sm.ifull[r]);
             if (!live) break;
         }
-      } else if (warp == 9) {
+    } else if (warp == kTma) {
         // ---------------- TMA producer ----------------
         uint32_t ring = 0, qn[2] = {0, 0};
-        Item it;
+        Item it;  // a copy
         bool ok = true;
         auto load_q = [&](int st) -> bool {
             if (qn[st] > 0 && !tc::mbar_wait(&sm.qempty[st], (qn[st] - 1) & 1u, abort, kLimitNs)) {
@@ -480,7 +517,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 tc::mbar_arrive_expect_tx(&sm.qfull[st], Sm::kHalves * 128u * p.group * p.tt);
                 for (int h = 0; h < Sm::kHalves; ++h) {
                     tc::tma_load_3d(sm.q[st] + h * Sm::kBox, &map_q, &sm.qfull[st], h * 64,
-                                    it.kvh * p.group, it.q_row[st]);
+                                    it.kvh * p.group, st == 0 ? it.q_row[0] : it.q_row[1]);
                 }
             }
             __syncwarp();
@@ -524,11 +561,15 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             __syncwarp();
             return true;
         };
-        for (uint32_t i = 0; ok && take(i, it); ++i) {
+        for (uint32_t i = 0; ok; ++i) {
+            const Item* next = take(i);
+            if (next == nullptr) break;
+            it = *next;
+            drop(i);
             const int tiles = itemTiles(it);
             const CUtensorMap* mk = kPrefix && it.src == 1 ? &map_k1 : &map_k0;
             const CUtensorMap* mv = kPrefix && it.src == 1 ? &map_v1 : &map_v0;
-            if (tiles > 0 && (it.n[0] > 0 || !it.paired)) ok = load_q(0);
+            if (it.n[0] > 0) ok = load_q(0);
             for (int t = 0; ok && t < tiles; ++t) {
                 ok = load_kv(mk, t);
                 if (ok && t == 0 && it.paired && it.n[1] > 0) ok = load_q(1);
@@ -546,28 +587,40 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
             }
         }
-      } else if (warp == 8) {
+    } else if (warp == kMma) {
         // ---------------- MMA issuer ----------------
+        // Everything an issue needs is in registers before its wait ends: the
+        // time between two issues is time the tensor core may stand idle.
         const int ksteps = ceilDiv(p.d, 16);
         const uint32_t idesc_s = tc::idesc_f16_f32(kTile, kTile, 0, 0, kBf16);
         const uint32_t idesc_o = tc::idesc_f16_f32(kTile, ksteps * 16, 0, 1, kBf16);
-        uint32_t ring = 0, qn[2] = {0, 0}, pn[2] = {0, 0};
-        Item it;
-        int tiles = 0;
-        // Scores of step u: S[stream] = Q[stream] K[tile]^T.
-        auto scores = [&](int u) -> bool {
-            if (!stepLive(it, u)) return true;
-            const int st = u & 1, tile = stepTile(it, u), qs = it.paired ? st : 0;
-            const uint32_t j = ring + 2 * tile, stage = j % kStages;
-            if ((it.paired ? tile == 0 : u == 0)) {
-                if (!tc::mbar_wait(&sm.qfull[qs], qn[qs] & 1u, abort, kLimitNs)) return false;
-                ++qn[qs];
+        const uint64_t kdesc = tc::smem_desc_sw128(tc::smem_u32(sm.kv[0]), 16, 1024);
+        const uint64_t vdesc = tc::smem_desc_sw128(tc::smem_u32(sm.kv[0]), Sm::kBox, 1024);
+        const uint64_t qdesc = tc::smem_desc_sw128(tc::smem_u32(sm.q[0]), 16, 1024);
+        constexpr uint32_t kStep = Sm::kTileBytes >> 4;  // a tile in descriptor units
+        uint32_t qphase[2] = {0, 0}, pphase[2] = {0, 0};
+        // A place in the K / V ring: stage and parity.
+        struct Place {
+            uint32_t stage, parity;
+            __device__ __forceinline__ void move(uint32_t by) {  // by < kStages
+                stage += by;
+                if (stage >= kStages) {
+                    stage -= kStages;
+                    parity ^= 1u;
+                }
             }
-            if (!tc::mbar_wait(&sm.full[stage], (j / kStages) & 1u, abort, kLimitNs)) return false;
+        };
+        // S[st] = Q[slot] K^T from the tile at `k`.
+        auto scores = [&](auto stream, uint32_t slot, const Place& k, bool first, bool release,
+                          bool last) -> bool {
+            constexpr int st = decltype(stream)::value;
+            if (first) {
+                if (!tc::mbar_wait(&sm.qfull[slot], qphase[st], abort, kLimitNs)) return false;
+            }
+            const uint64_t q0 = qdesc + slot * kStep, k0 = kdesc + k.stage * kStep;
+            if (!tc::mbar_wait(&sm.full[k.stage], k.parity, abort, kLimitNs)) return false;
             tc::tc_fence_after();
             if (tc::elect_one()) {
-                const uint64_t q0 = tc::smem_desc_sw128(tc::smem_u32(sm.q[qs]), 16, 1024);
-                const uint64_t k0 = tc::smem_desc_sw128(tc::smem_u32(sm.kv[stage]), 16, 1024);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t off = ((kk >> 2) * Sm::kBox + (kk & 3) * 32) >> 4;
@@ -575,115 +628,164 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                         tc::mma_f16(tmem + st * kTile, q0 + off, k0 + off, idesc_s, kk > 0);
                     }
                 }
-                // the tile's last reader releases it
-                const bool last = !it.paired || st == 1 || tile >= it.n[1];
-                if (last) tc::mma_commit(&sm.empty[stage]);
-                if (it.paired ? tile == (st == 0 ? it.n[0] : it.n[1]) - 1 : u == tiles - 1) {
-                    tc::mma_commit(&sm.qempty[qs]);
-                }
                 tc::mma_commit(&sm.sfull[st]);
+                if (release) tc::mma_commit(&sm.empty[k.stage]);
+                if (last) tc::mma_commit(&sm.qempty[slot]);
             }
             __syncwarp();
             return true;
         };
-        // Step u: O[stream] (+)= P[stream] V[tile].
-        auto values = [&](int u) -> bool {
-            if (!stepLive(it, u)) return true;
-            const int st = u & 1, tile = stepTile(it, u);
-            const uint32_t j = ring + 2 * tile + 1, stage = j % kStages;
-            if (!tc::mbar_wait(&sm.full[stage], (j / kStages) & 1u, abort, kLimitNs)) return false;
-            const int valid = it.nk - tile * kTile;
-            const bool first = !it.paired || st == 0 || tile >= it.n[0];
-            if (valid < kTile && first) {
+        // O[st] (+)= P[st] V from the tile at `v`, of which `valid` keys count.
+        auto values = [&](auto stream, const Place& v, int valid, bool zero, bool first,
+                          bool release, bool last) -> bool {
+            constexpr int st = decltype(stream)::value;
+            if (!tc::mbar_wait(&sm.full[v.stage], v.parity, abort, kLimitNs)) return false;
+            if (valid < kTile && zero) {
                 for (int h = 0; h < Sm::kHalves; ++h) {
-                    uint4* z = reinterpret_cast<uint4*>(sm.kv[stage] + h * Sm::kBox);
+                    uint4* z = reinterpret_cast<uint4*>(sm.kv[v.stage] + h * Sm::kBox);
                     for (int x = valid * 8 + lane; x < kTile * 8; x += 32) z[x] = make_uint4(0, 0, 0, 0);
                 }
                 tc::fence_proxy_async();
                 __syncwarp();
             }
-            const int jj = u >> 1;  // the stream's own tile count
-            for (int half = 0; half < 2; ++half) {
-                if (!tc::mbar_wait(&sm.pfull[st][half], pn[st] & 1u, abort, kLimitNs)) return false;
-                tc::tc_fence_after();
+            const uint32_t o0 = tmem + 2 * kTile + st * kTile;
+            const uint32_t p0 = tmem + st * kTile;
+            const uint64_t v0 = vdesc + v.stage * kStep;  // 16 keys: 2 KB of V
+            if (!tc::mbar_wait(&sm.pfull[st][0], pphase[st], abort, kLimitNs)) return false;
+            tc::tc_fence_after();
+            if (kFirst < 8) {
                 if (tc::elect_one()) {
-                    const uint64_t v0 =
-                        tc::smem_desc_sw128(tc::smem_u32(sm.kv[stage]), Sm::kBox, 1024) + half * 512;
-                    const uint32_t p0 = tmem + st * kTile + half * 32;
-                    const uint32_t o0 = tmem + 2 * kTile + st * kTile;
-                    tc::mma_f16_ts(o0, p0, v0, idesc_o, jj > 0 || half > 0);
 #pragma unroll
-                    for (int q = 1; q < 4; ++q) {  // 16 keys: 2 KB of V
-                        tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, 1);
-                    }
-                    if (half == 1) {
-                        const bool last = !it.paired || st == 1 || tile >= it.n[1];
-                        if (last) tc::mma_commit(&sm.empty[stage]);
-                        if (jj == (st == 0 ? it.n[0] : it.n[1]) - 1) tc::mma_commit(&sm.ofull[st]);
+                    for (int q = 0; q < kFirst; ++q) {
+                        tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, q > 0 || !first);
                     }
                 }
                 __syncwarp();
+                if (!tc::mbar_wait(&sm.pfull[st][1], pphase[st], abort, kLimitNs)) return false;
+                tc::tc_fence_after();
             }
-            ++pn[st];
+            if (tc::elect_one()) {
+#pragma unroll
+                for (int q = kFirst < 8 ? kFirst : 0; q < 8; ++q) {
+                    tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, q > 0 || !first);
+                }
+                if (last) tc::mma_commit(&sm.ofull[st]);
+                if (release) tc::mma_commit(&sm.empty[v.stage]);
+            }
+            __syncwarp();
+            pphase[st] ^= 1u;
             return true;
         };
+        Place at = {0, 0};
         bool ok = true;
-        for (uint32_t i = 0; ok && take(i, it); ++i) {
-            tiles = itemTiles(it);
-            const int steps = it.paired ? 2 * tiles : tiles;
-            ok = scores(0) && scores(1);
-            for (int u = 0; ok && u < steps; ++u) ok = values(u) && scores(u + 2);
-            ring += 2 * tiles;
+        for (uint32_t i = 0; ok; ++i) {
+            const Item* it = take(i);
+            if (it == nullptr) break;
+            const int n0 = it->n[0], n1 = it->n[1], nk = it->nk, tiles = itemTiles(*it);
+            const bool paired = it->paired != 0;
+            drop(i);
+            const uint32_t step = paired ? 2 : 4;  // ring places a stream's next tile is ahead
+            const uint32_t slot1 = paired ? 1 : 0;
+            std::integral_constant<int, 0> s0;
+            std::integral_constant<int, 1> s1;
+            Place k0 = at, v0 = at, k1 = at, v1;
+            if (!paired) k1.move(2);
+            v0.move(1);
+            v1 = k1;
+            v1.move(1);
+            // In a pair the second stream, where it reads a tile, is the tile's last
+            // reader; alternate tiles have one reader each. Q's last reader is the
+            // stream that owns it, or the item's last tile.
+            if (n0 > 0) ok = scores(s0, 0, k0, true, !paired || n1 <= 0, paired ? n0 == 1 : n1 <= 0);
+            if (ok && n1 > 0) ok = scores(s1, slot1, k1, paired, true, n1 == 1 && (paired || n0 == 1));
+            for (int t = 0; ok && (t < n0 || t < n1); ++t) {
+                const int tile0 = paired ? t : 2 * t, tile1 = paired ? t : 2 * t + 1;
+                k0.move(step);
+                k1.move(step);
+                if (t < n0) {
+                    ok = values(s0, v0, nk - tile0 * kTile, true, t == 0, !paired || t >= n1, t + 1 == n0);
+                    if (ok && t + 1 < n0) {
+                        ok = scores(s0, 0, k0, false, !paired || t + 1 >= n1,
+                                    t + 2 == n0 && (paired || n1 < n0));
+                    }
+                }
+                if (ok && t < n1) {
+                    ok = values(s1, v1, nk - tile1 * kTile, !paired || t >= n0, t == 0, true, t + 1 == n1);
+                    if (ok && t + 1 < n1) {
+                        ok = scores(s1, slot1, k1, false, true, t + 2 == n1 && (paired || n1 == n0));
+                    }
+                }
+                v0.move(step);
+                v1.move(step);
+            }
+            if (n0 > 0) qphase[0] ^= 1u;
+            if (paired && n1 > 0) qphase[1] ^= 1u;
+            const uint32_t next = at.stage + 2 * tiles;
+            at.parity ^= (next / kStages) & 1u;
+            at.stage = next % kStages;
         }
-      }
-    } else {
+    } else if (warp < kMma) {
         // ---------------- softmax and epilogue ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int st = warp >> 2, quarter = warp & 3;
         const int row = quarter * 32 + lane;
         const int token = row / p.group, head_in = row - token * p.group;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_addr = tmem + lanes + st * kTile;
-        const uint32_t o_addr = tmem + lanes + 2 * kTile + st * kTile;
-        const int dcols = (p.d + 31) / 32;  // 32-column groups of the accumulator
-        uint32_t sn = 0, on = 0;
-        Item it;
+        const uint32_t o_addr = tmem + lanes + 2 * kTile;  // stream 1's is kTile further
+        uint32_t sn = 0, on[2] = {0, 0}, xn = 0;  // tiles; accumulators, by stream; meetings
+        // Meets the other stream's warp of the same rows.
+        auto meet = [&]() -> bool {
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sm.xbar[quarter]);
+            return tc::mbar_wait(&sm.xbar[quarter], xn++ & 1u, abort, kLimitNs);
+        };
         bool ok = true;
-        for (uint32_t i = 0; ok && take(i, it); ++i) {
+        for (uint32_t i = 0; ok; ++i) {
+            const Item* item = take(i);  // kept in the ring: a copy would not fit the registers
+            if (item == nullptr) break;
+            const Item& it = *item;
             const int lim = rowLimit(it, st, token);
-            const int n = st == 0 ? it.n[0] : it.n[1];
-            // keys the row sees from the stream's current tile on, and a tile's step
+            const int n = st == 0 ? it.n[0] : it.n[1], theirs = st == 0 ? it.n[1] : it.n[0];
+            // keys the row sees from the stream's current tile on
             int left = lim - (it.paired ? 0 : st * kTile);
             const int stride = it.paired ? kTile : 2 * kTile;
             const bool mine = token < (st == 0 ? it.tok[0] : it.tok[1]) && token < p.tt;
+            const bool idle = !__any_sync(0xffffffffu, mine);  // no row of the warp is wanted
             float m = -INFINITY, l = 0.0f;
             for (int jj = 0; jj < n; ++jj, ++sn, left -= stride) {
                 if (!tc::mbar_wait(&sm.sfull[st], sn & 1u, abort, kLimitNs)) {
                     ok = false;
                     break;
                 }
-                tc::tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_addr + c * 32, s[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc::tmem_ld_wait(s[c]);
-                const bool masked = __any_sync(0xffffffffu, left < kTile);
-                if (masked) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) {
-                            if (c * 32 + x >= left) s[c][x] = __float_as_uint(-INFINITY);
-                        }
+                if (idle) {
+                    if (lane == 0) {
+                        tc::mbar_arrive(&sm.pfull[st][0]);
+                        if (kFirst < 8) tc::mbar_arrive(&sm.pfull[st][1]);
                     }
+                    continue;
                 }
+                tc::tc_fence_after();
+                // The tile's scores are read twice, 32 at a time, for the row maximum
+                // and for the probabilities: held whole they would spill.
+                const bool masked = __any_sync(0xffffffffu, left < kTile);
+                uint32_t s[2][32];
+                auto hide = [&](uint32_t (&v)[32], int c) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) {
+                        if (c * 32 + x >= left) v[x] = __float_as_uint(-INFINITY);
+                    }
+                };
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tc::tmem_ld32(s_addr, s[0]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
+                    tc::tmem_ld_wait(s[c & 1]);
+                    tc::tmem_ld32(s_addr + ((c + 1) & 3) * 32, s[(c + 1) & 1]);  // last: the first again
+                    if (masked) hide(s[c & 1], c);
 #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        mx[c] = tc::max3(mx[c], __uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1]));
+                        mx[x / 2 % 4] = tc::max3(mx[x / 2 % 4], __uint_as_float(s[c & 1][x]),
+                                                 __uint_as_float(s[c & 1][x + 1]));
                     }
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
@@ -693,32 +795,34 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     m = grow ? top : m;
                     l *= f;
                     if (jj > 0) {
-                        for (int c = 0; c < p.d; c += 16) {
+                        for (int x = 0; x < p.d; x += 16) {
                             uint32_t o[16];
-                            tc::tmem_ld16(o_addr + c, o);
+                            tc::tmem_ld16(o_addr + st * kTile + x, o);
                             tc::tmem_ld_wait(o);
 #pragma unroll
-                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                            tc::tmem_st16(o_addr + c, o);
+                            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                            tc::tmem_st16(o_addr + st * kTile + x, o);
                         }
                     }
                 }
                 const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
                 const uint64_t c2 = tc::pair(p.c2, p.c2), nm2 = tc::pair(nm, nm);
                 uint64_t sum[2] = {0, 0};
-                // Probabilities of the tile in two halves: the product with V
-                // starts on the first while the second is computed.
-                auto probabilities = [&](auto poly) {
+                // Probabilities, handed on in two parts: the product with V starts
+                // on the first while the last is computed.
+                auto probabilities = [&](auto plain) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t w[32];
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[16];
+                        tc::tmem_ld_wait(s[c & 1]);
+                        if (c < 3) tc::tmem_ld32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
+                        if (!plain.value) hide(s[c & 1], c);
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) {
-                            const int y = 2 * x;
-                            uint64_t v = tc::fma2(tc::pair(__uint_as_float(s[2 * c + y / 32][y % 32]),
-                                                           __uint_as_float(s[2 * c + y / 32][y % 32 + 1])),
+                        for (int x = 0; x < 16; ++x) {
+                            uint64_t v = tc::fma2(tc::pair(__uint_as_float(s[c & 1][2 * x]),
+                                                           __uint_as_float(s[c & 1][2 * x + 1])),
                                                   c2, nm2);
-                            if (poly.value && x % 8 < kPoly) {
+                            if (plain.value && x % 8 < kPoly) {
                                 v = tc::ex2_poly(v);
                             } else {
                                 const float2 z = tc::unpair(v);
@@ -728,11 +832,13 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                             const float2 z = tc::unpair(v);
                             w[x] = pack2<T>(z.x, z.y);
                         }
-                        tc::tmem_st32(s_addr + c * 32, w);
-                        tc::tmem_st_wait();
-                        tc::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) tc::mbar_arrive(&sm.pfull[st][c]);
+                        tc::tmem_st16(s_addr + c * 16, w);
+                        if (c == kFirst / 2 - 1 || c == 3) {
+                            tc::tmem_st_wait();
+                            tc::tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) tc::mbar_arrive(&sm.pfull[st][kFirst < 8 && c == 3]);
+                        }
                     }
                 };
                 // Masked scores are -inf, which only ex2 takes to an exact 0.
@@ -745,80 +851,132 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 l += z.x + z.y;
             }
             if (!ok) break;
-            // No score above -inf: the row sees nothing. (A NaN score shows in l.)
+            // Accumulators done with this item, of either stream.
+            const uint32_t o_own = on[st], o_other = on[st ^ 1];
+            on[st] += n > 0;
+            on[st ^ 1] += theirs > 0;
+            if (idle) {
+                drop(i);
+                continue;
+            }
+            // No score above -inf: nothing was seen. (A NaN score shows in l.)
             if (m == -INFINITY && l < 0x1p60f) l = 0.0f;
             // ---- the row's result ----
-            if (n > 0) {
-                if (!tc::mbar_wait(&sm.ofull[st], on & 1u, abort, kLimitNs)) break;
-                ++on;
-                tc::tc_fence_after();
+            // A pair's streams have rows of their own. Otherwise both have seen
+            // half of the same rows' keys: each joins the two results for half
+            // of the columns.
+            if (n > 0 && !tc::mbar_wait(&sm.ofull[st], o_own & 1u, abort, kLimitNs)) break;
+            float f0 = 1.0f, f1 = 0.0f;  // shares of this stream's and the other's accumulator
+            int from = 0, to = D;
+            if (!it.paired) {
+                sm.xch[st][row] = make_float2(m, l);
+                if (!meet()) break;
+                const float2 o = sm.xch[st ^ 1][row];
+                if (theirs > 0 && !tc::mbar_wait(&sm.ofull[st ^ 1], o_other & 1u, abort, kLimitNs)) break;
+                const float both = fmaxf(m, o.x);
+                f0 = l == 0.0f ? 0.0f : tc::ex2((m - both) * p.c2);
+                f1 = o.y == 0.0f ? 0.0f : tc::ex2((o.x - both) * p.c2);
+                l = l * f0 + o.y * f1;
+                m = both;
+                from = st * (D / 2);
+                to = from + D / 2;
             }
+            tc::tc_fence_after();
             const int64_t tok_row = (st == 0 ? it.q_row[0] : it.q_row[1]) + token;
-            const int slot = st == 0 ? it.slot[0] : it.slot[1];
             const int head = it.kvh * p.group + head_in;
-            const float inv = l > 0.0f ? 1.0f / l : l;  // 0 for a row that sees nothing; NaN stays
-            // NaN somewhere: also seen as a sum no tile can have (ex2_poly)
+            // 0 for a row that sees nothing; NaN stays
+            const float inv = l > 0.0f ? 1.0f / l : l;
+            f0 *= inv;
+            f1 *= inv;
+            // NaN somewhere: also seen as a sum no row can have (ex2_poly)
             bool nan = !(l < 0x1p60f);
-            float* part = nullptr;
-            T* y = nullptr;
-            if constexpr (kPrefix) {
-                part = p.part + (slot * p.rows + tok_row * p.heads + head) * p.d;
-            } else {
-                y = static_cast<T*>(p.y) + tok_row * p.y_row + head * p.y_head;
+            using Out = typename std::conditional<kPrefix, float, T>::type;
+            constexpr int kVec = 16 / sizeof(Out);  // elements of a 16-byte store
+            constexpr int kPass = 4 * kVec;         // columns at a time: 64 bytes of a row
+            Out* out = kPrefix
+                ? reinterpret_cast<Out*>(p.part) + (it.slot * p.rows + tok_row * p.heads + head) * p.d
+                : static_cast<Out*>(p.y) + tok_row * p.y_row + head * p.y_head;
+            // Four lanes store four rows together, 64 bytes of one row at a time.
+            const bool store = mine && !(kPrefix && l == 0.0f);
+            Out* rows[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int src = (lane & ~3) + r;
+                const int64_t addr = __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(out), src);
+                rows[r] = __shfl_sync(0xffffffffu, static_cast<int>(store), src) != 0
+                    ? reinterpret_cast<Out*>(addr) + (lane & 3) * kVec
+                    : nullptr;
             }
-            for (int c = 0; c < dcols; ++c) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tc::tmem_ld32(o_addr + c * 32, o);
-                    tc::tmem_ld_wait(o);
-                }
+            for (int x = from; x < to && x < p.d; x += kPass) {
+                uint4 v[4];
 #pragma unroll
-                for (int x = 0; x < 32; ++x) {
-                    // a row with no visible key: zeros, whatever the accumulator holds
-                    const float f = l == 0.0f ? 0.0f : __uint_as_float(o[x]) * inv;
-                    nan = nan || (f != f && c * 32 + x < p.d);
-                    o[x] = __float_as_uint(f);
-                }
-                if (mine) {
+                for (int g = 0; g < kPass / 16; ++g) {
+                    uint32_t o[16];
+                    float f[16];
+                    // An accumulator without steps holds what an earlier item left.
+                    if (n > 0) {
+                        tc::tmem_ld16(o_addr + st * kTile + x + g * 16, o);
+                        tc::tmem_ld_wait(o);
+                    }
 #pragma unroll
-                    for (int x = 0; x < 32; x += 8) {
-                        if (c * 32 + x < p.d) {
-                            float f[8];
+                    for (int y = 0; y < 16; ++y) f[y] = f0 == 0.0f ? 0.0f : __uint_as_float(o[y]) * f0;
+                    if (!it.paired && theirs > 0) {
+                        tc::tmem_ld16(o_addr + (st ^ 1) * kTile + x + g * 16, o);
+                        tc::tmem_ld_wait(o);
 #pragma unroll
-                            for (int z = 0; z < 8; ++z) f[z] = __uint_as_float(o[x + z]);
-                            if constexpr (kPrefix) {
-                                if (l != 0.0f) {
-                                    float4* out = reinterpret_cast<float4*>(part + c * 32 + x);
-                                    out[0] = make_float4(f[0], f[1], f[2], f[3]);
-                                    out[1] = make_float4(f[4], f[5], f[6], f[7]);
-                                }
-                            } else {
-                                *reinterpret_cast<uint4*>(y + c * 32 + x) = pack8<T>(f);
-                            }
+                        for (int y = 0; y < 16; ++y) {
+                            if (f1 != 0.0f) f[y] = fmaf(__uint_as_float(o[y]), f1, f[y]);
                         }
+                    }
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) nan = nan || (f[y] != f[y] && x + g * 16 + y < p.d);
+                    if constexpr (kPrefix) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            v[y] = make_uint4(__float_as_uint(f[4 * y]), __float_as_uint(f[4 * y + 1]),
+                                              __float_as_uint(f[4 * y + 2]), __float_as_uint(f[4 * y + 3]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            v[2 * g + y] = make_uint4(pack2<T>(f[8 * y], f[8 * y + 1]),
+                                                      pack2<T>(f[8 * y + 2], f[8 * y + 3]),
+                                                      pack2<T>(f[8 * y + 4], f[8 * y + 5]),
+                                                      pack2<T>(f[8 * y + 6], f[8 * y + 7]));
+                        }
+                    }
+                }
+                transpose4(v, lane);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (rows[r] != nullptr && x + (lane & 3) * kVec < p.d) {
+                        *reinterpret_cast<uint4*>(rows[r] + x) = v[r];
                     }
                 }
             }
             float lse = l > 0.0f ? fmaf(m, p.c2, log2f(l)) : -INFINITY;
+            __syncwarp();  // a row written again below was stored by other lanes
             if (mine && nan) {
                 float o[D];
-                const Item again = it;
-                lse = slowRow<D, T>(p, again, st, row, o);
-                for (int c = 0; c < p.d; c += 2) {
+                lse = slowRow<D, T>(p, it, st, row, o);
+                for (int x = from; x < to && x < p.d; ++x) {
                     if constexpr (kPrefix) {
-                        *reinterpret_cast<float2*>(part + c) = make_float2(o[c], o[c + 1]);
+                        out[x] = o[x];
                     } else {
-                        *reinterpret_cast<uint32_t*>(y + c) = pack2<T>(o[c], o[c + 1]);
+                        out[x] = static_cast<T>(o[x]);
                     }
                 }
             }
-            if (kPrefix && mine) p.lse[slot * p.rows + tok_row * p.heads + head] = lse;
+            if (kPrefix && mine && from == 0) p.lse[it.slot * p.rows + tok_row * p.heads + head] = lse;
             tc::tc_fence_before();  // the reads above come before the next item's products
+            const bool together = !it.paired;
+            drop(i);
+            if (together && !meet()) break;
         }
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kMma) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, 512);
     }
@@ -909,14 +1067,6 @@ int launchKernel(const Maps& m, const Params& p, int grid, cudaStream_t s) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    static_cast<int>(sizeof(Smem<D>)));
         if (e != cudaSuccess) return setCudaError(MLKB_ERR_LAUNCH, e, "attention smem attribute");
-        // The register shares are taken from what the block is launched with:
-        // a build that gave the kernel fewer would wait for them for good.
-        cudaFuncAttributes fa;
-        const cudaError_t ea = cudaFuncGetAttributes(&fa, kernel);
-        if (ea != cudaSuccess) return setCudaError(MLKB_ERR_LAUNCH, ea, "attention attributes");
-        if (fa.numRegs * 12 < 8 * kSoftmaxRegs + 4 * kOtherRegs) {
-            return setError(MLKB_ERR_LAUNCH, "attention: kernel built with too few registers");
-        }
         attr[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -982,7 +1132,7 @@ KeySource keySource(const mlkb_heads& k, const mlkb_heads& v) {
 // the device).
 struct PrefixPlan {
     int64_t group, tt, tokens, rows;
-    int64_t paired, mt, tiles, splits, slots_pre, pre_items;
+    int64_t paired, mt, tiles, splits, pre_items;
     int64_t chunk, chunks, suf_mt, suf_items, slots;
 };
 
@@ -1008,7 +1158,6 @@ PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_he
         r.tiles = per;
         r.splits = (tiles + per - 1) / per;
     }
-    r.slots_pre = r.splits * (r.paired ? 1 : 2);
     r.pre_items = r.splits * kv_heads * r.mt;
     r.suf_mt = (steps + r.tt - 1) / r.tt;
     if (cap > 0) {
@@ -1022,7 +1171,7 @@ PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_he
         r.chunks = (ctiles + per - 1) / per;
     }
     r.suf_items = batch * kv_heads * r.suf_mt * r.chunks;
-    r.slots = r.slots_pre + 2 * r.chunks;
+    r.slots = r.splits + r.chunks;
     return r;
 }
 
