@@ -65,10 +65,9 @@ constexpr int kStages = 5;   // K / V ring
 constexpr int kThreads = 12 * 32;
 constexpr int kMma = 8, kTma = 9, kSched = 10;  // warps; 0 to 7 are softmax warps, 11 is idle
 constexpr int kConsumers = 10;                  // warps that read an item
-constexpr int kFirst = 6;  // 16-key steps of a tile's probabilities that are handed on first
 constexpr uint64_t kLimitNs = 2000000000ull;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
-constexpr int kPoly = 0;          // of 8 pairs of exponentials, how many go to the FMA pipe
+constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe
 constexpr int kMaxSlots = 32;     // partial results a row may have
 
 // What one pass through the pipeline computes. Keys are counted from the
@@ -132,8 +131,7 @@ struct Smem {
     Item item[kItems];
     uint64_t full[kStages], empty[kStages];
     uint64_t qfull[2], qempty[2];
-    uint64_t sfull[2], ofull[2];        // [stream]
-    uint64_t pfull[2][2];               // [stream][first part of the tile's keys, rest]
+    uint64_t sfull[2], pfull[2], ofull[2];  // [stream]
     uint64_t xbar[4];                   // [lane quarter]: the streams' warps meet
     uint64_t ifull[kItems], iempty[kItems];
     float2 xch[2][kTile];               // [stream][row]: maximum and sum
@@ -435,10 +433,9 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             tc::mbar_init(&sm.qempty[i], 1);
             tc::mbar_init(&sm.sfull[i], 1);
             tc::mbar_init(&sm.ofull[i], 1);
-            for (int j = 0; j < 2; ++j) {
-                tc::mbar_init(&sm.pfull[i][j], 4);
-                tc::mbar_init(&sm.xbar[2 * i + j], 2);
-            }
+            tc::mbar_init(&sm.pfull[i], 4);
+            tc::mbar_init(&sm.xbar[2 * i], 2);
+            tc::mbar_init(&sm.xbar[2 * i + 1], 2);
         }
         for (int i = 0; i < kItems; ++i) {
             tc::mbar_init(&sm.ifull[i], 1);
@@ -610,116 +607,113 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
             }
         };
-        // S[st] = Q[slot] K^T from the tile at `k`.
-        auto scores = [&](auto stream, uint32_t slot, const Place& k, bool first, bool release,
-                          bool last) -> bool {
-            constexpr int st = decltype(stream)::value;
-            if (first) {
-                if (!tc::mbar_wait(&sm.qfull[slot], qphase[st], abort, kLimitNs)) return false;
-            }
-            const uint64_t q0 = qdesc + slot * kStep, k0 = kdesc + k.stage * kStep;
-            if (!tc::mbar_wait(&sm.full[k.stage], k.parity, abort, kLimitNs)) return false;
-            tc::tc_fence_after();
-            if (tc::elect_one()) {
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * Sm::kBox + (kk & 3) * 32) >> 4;
-                    if (kk < ksteps) {
-                        tc::mma_f16(tmem + st * kTile, q0 + off, k0 + off, idesc_s, kk > 0);
-                    }
-                }
-                tc::mma_commit(&sm.sfull[st]);
-                if (release) tc::mma_commit(&sm.empty[k.stage]);
-                if (last) tc::mma_commit(&sm.qempty[slot]);
-            }
-            __syncwarp();
-            return true;
+        auto wait = [&](const Place& x) {
+            return tc::mbar_wait(&sm.full[x.stage], x.parity, abort, kLimitNs);
         };
-        // O[st] (+)= P[st] V from the tile at `v`, of which `valid` keys count.
-        auto values = [&](auto stream, const Place& v, int valid, bool zero, bool first,
-                          bool release, bool last) -> bool {
-            constexpr int st = decltype(stream)::value;
-            if (!tc::mbar_wait(&sm.full[v.stage], v.parity, abort, kLimitNs)) return false;
-            if (valid < kTile && zero) {
-                for (int h = 0; h < Sm::kHalves; ++h) {
-                    uint4* z = reinterpret_cast<uint4*>(sm.kv[v.stage] + h * Sm::kBox);
-                    for (int x = valid * 8 + lane; x < kTile * 8; x += 32) z[x] = make_uint4(0, 0, 0, 0);
-                }
-                tc::fence_proxy_async();
-                __syncwarp();
-            }
-            const uint32_t o0 = tmem + 2 * kTile + st * kTile;
-            const uint32_t p0 = tmem + st * kTile;
-            const uint64_t v0 = vdesc + v.stage * kStep;  // 16 keys: 2 KB of V
-            if (!tc::mbar_wait(&sm.pfull[st][0], pphase[st], abort, kLimitNs)) return false;
-            tc::tc_fence_after();
-            if (kFirst < 8) {
-                if (tc::elect_one()) {
+        auto loaded = [&](const Place& x) { return tc::mbar_test(&sm.full[x.stage], x.parity); };
+        // S[st] = Q[slot] K^T, by one thread.
+        auto scores = [&](int st, uint32_t slot, const Place& k, bool release, bool q_done) {
+            const uint64_t q0 = qdesc + slot * kStep, k0 = kdesc + k.stage * kStep;
+            const uint32_t s0 = tmem + st * kTile;
 #pragma unroll
-                    for (int q = 0; q < kFirst; ++q) {
-                        tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, q > 0 || !first);
-                    }
-                }
-                __syncwarp();
-                if (!tc::mbar_wait(&sm.pfull[st][1], pphase[st], abort, kLimitNs)) return false;
-                tc::tc_fence_after();
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = ((kk >> 2) * Sm::kBox + (kk & 3) * 32) >> 4;
+                if (kk < ksteps) tc::mma_f16(s0, q0 + off, k0 + off, idesc_s, kk > 0);
             }
-            if (tc::elect_one()) {
-#pragma unroll
-                for (int q = kFirst < 8 ? kFirst : 0; q < 8; ++q) {
-                    tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, q > 0 || !first);
-                }
-                if (last) tc::mma_commit(&sm.ofull[st]);
-                if (release) tc::mma_commit(&sm.empty[v.stage]);
-            }
-            __syncwarp();
-            pphase[st] ^= 1u;
-            return true;
+            tc::mma_commit(&sm.sfull[st]);
+            if (release) tc::mma_commit(&sm.empty[k.stage]);
+            if (q_done) tc::mma_commit(&sm.qempty[slot]);
         };
         Place at = {0, 0};
         bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
             const Item* it = take(i);
             if (it == nullptr) break;
-            const int n0 = it->n[0], n1 = it->n[1], nk = it->nk, tiles = itemTiles(*it);
+            const int n[2] = {it->n[0], it->n[1]}, nk = it->nk, tiles = itemTiles(*it);
             const bool paired = it->paired != 0;
             drop(i);
             const uint32_t step = paired ? 2 : 4;  // ring places a stream's next tile is ahead
-            const uint32_t slot1 = paired ? 1 : 0;
-            std::integral_constant<int, 0> s0;
-            std::integral_constant<int, 1> s1;
-            Place k0 = at, v0 = at, k1 = at, v1;
-            if (!paired) k1.move(2);
-            v0.move(1);
-            v1 = k1;
-            v1.move(1);
-            // In a pair the second stream, where it reads a tile, is the tile's last
-            // reader; alternate tiles have one reader each. Q's last reader is the
-            // stream that owns it, or the item's last tile.
-            if (n0 > 0) ok = scores(s0, 0, k0, true, !paired || n1 <= 0, paired ? n0 == 1 : n1 <= 0);
-            if (ok && n1 > 0) ok = scores(s1, slot1, k1, paired, true, n1 == 1 && (paired || n0 == 1));
-            for (int t = 0; ok && (t < n0 || t < n1); ++t) {
-                const int tile0 = paired ? t : 2 * t, tile1 = paired ? t : 2 * t + 1;
-                k0.move(step);
-                k1.move(step);
-                if (t < n0) {
-                    ok = values(s0, v0, nk - tile0 * kTile, true, t == 0, !paired || t >= n1, t + 1 == n0);
-                    if (ok && t + 1 < n0) {
-                        ok = scores(s0, 0, k0, false, !paired || t + 1 >= n1,
-                                    t + 2 == n0 && (paired || n1 < n0));
-                    }
+            // Each stream's next K and V, and whether they are known to have landed.
+            Place k[2] = {at, at}, v[2];
+            if (!paired) k[1].move(2);
+            bool known[2] = {false, false};
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                v[st] = k[st];
+                v[st].move(1);
+                if (!ok || n[st] == 0) continue;
+                const uint32_t slot = paired ? st : 0;
+                if (paired || st == 0) ok = tc::mbar_wait(&sm.qfull[slot], qphase[slot], abort, kLimitNs);
+                ok = ok && wait(k[st]);
+                tc::tc_fence_after();
+                // In a pair the second stream, where it reads a tile, is the tile's
+                // last reader; alternate tiles have one reader each. Q's last reader
+                // is the stream that owns it, or the item's last tile.
+                if (ok && tc::elect_one()) {
+                    scores(st, slot, k[st], !paired || st == 1 || n[1] == 0,
+                           n[st] == 1 && (paired || (st == 0 ? n[1] == 0 : n[0] == 1)));
                 }
-                if (ok && t < n1) {
-                    ok = values(s1, v1, nk - tile1 * kTile, !paired || t >= n0, t == 0, true, t + 1 == n1);
-                    if (ok && t + 1 < n1) {
-                        ok = scores(s1, slot1, k1, false, true, t + 2 == n1 && (paired || n1 == n0));
-                    }
-                }
-                v0.move(step);
-                v1.move(step);
+                __syncwarp();
             }
-            if (n0 > 0) qphase[0] ^= 1u;
-            if (paired && n1 > 0) qphase[1] ^= 1u;
+            for (int t = 0; ok && (t < n[0] || t < n[1]); ++t) {
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    // O (+)= P V of the stream's tile t, then S of its tile t + 1.
+                    if (!ok || t >= n[st]) continue;
+                    const bool more = t + 1 < n[st];
+                    const uint32_t slot = paired ? st : 0;
+                    const Place vp = v[st];
+                    k[st].move(step);
+                    v[st].move(step);
+                    const Place kp = k[st];
+                    if (!known[st]) ok = wait(vp);
+                    const int valid = nk - (paired ? t : 2 * t + st) * kTile;
+                    if (valid < kTile && (!paired || st == 0 || t >= n[0])) {  // its first reader
+                        for (int h = 0; h < Sm::kHalves; ++h) {
+                            uint4* z = reinterpret_cast<uint4*>(sm.kv[vp.stage] + h * Sm::kBox);
+                            for (int x = valid * 8 + lane; x < kTile * 8; x += 32) z[x] = make_uint4(0, 0, 0, 0);
+                        }
+                        tc::fence_proxy_async();
+                        __syncwarp();
+                    }
+                    ok = ok && tc::mbar_wait(&sm.pfull[st], pphase[st], abort, kLimitNs);
+                    pphase[st] ^= 1u;
+                    if (!ok) continue;
+                    const bool k_known = known[st];
+                    // Look ahead for the other stream's next step: the answer comes
+                    // while this step's products are issued. A pair shares its tiles.
+                    if (paired && st == 0) {
+                        known[1] = more || t + 1 >= n[1];
+                    } else {
+                        Place vn = v[st ^ 1], kn = k[st ^ 1];
+                        kn.move(step);
+                        known[st ^ 1] = loaded(vn) && loaded(kn);
+                    }
+                    const bool k_done = !paired || st == 1 || t + 1 >= n[1];
+                    const bool q_done = t + 2 == n[st] && (paired || (st == 0 ? n[1] < n[0] : n[1] == n[0]));
+                    tc::tc_fence_after();
+                    if (tc::elect_one()) {
+                        const uint32_t o0 = tmem + 2 * kTile + st * kTile, p0 = tmem + st * kTile;
+                        const uint64_t v0 = vdesc + vp.stage * kStep;  // 16 keys: 2 KB of V
+#pragma unroll
+                        for (int q = 0; q < kTile / 16; ++q) {
+                            tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, q > 0 || t > 0);
+                        }
+                        if (!more) tc::mma_commit(&sm.ofull[st]);
+                        if (!paired || st == 1 || t >= n[1]) tc::mma_commit(&sm.empty[vp.stage]);
+                        if (more && k_known) scores(st, slot, kp, k_done, q_done);
+                    }
+                    __syncwarp();
+                    if (more && !k_known) {
+                        ok = wait(kp);
+                        tc::tc_fence_after();
+                        if (ok && tc::elect_one()) scores(st, slot, kp, k_done, q_done);
+                        __syncwarp();
+                    }
+                }
+            }
+            if (n[0] > 0) qphase[0] ^= 1u;
+            if (paired && n[1] > 0) qphase[1] ^= 1u;
             const uint32_t next = at.stage + 2 * tiles;
             at.parity ^= (next / kStages) & 1u;
             at.stage = next % kStages;
@@ -758,10 +752,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     break;
                 }
                 if (idle) {
-                    if (lane == 0) {
-                        tc::mbar_arrive(&sm.pfull[st][0]);
-                        if (kFirst < 8) tc::mbar_arrive(&sm.pfull[st][1]);
-                    }
+                    if (lane == 0) tc::mbar_arrive(&sm.pfull[st]);
                     continue;
                 }
                 tc::tc_fence_after();
@@ -808,8 +799,6 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
                 const uint64_t c2 = tc::pair(p.c2, p.c2), nm2 = tc::pair(nm, nm);
                 uint64_t sum[2] = {0, 0};
-                // Probabilities, handed on in two parts: the product with V starts
-                // on the first while the last is computed.
                 auto probabilities = [&](auto plain) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
@@ -833,12 +822,6 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                             w[x] = pack2<T>(z.x, z.y);
                         }
                         tc::tmem_st16(s_addr + c * 16, w);
-                        if (c == kFirst / 2 - 1 || c == 3) {
-                            tc::tmem_st_wait();
-                            tc::tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) tc::mbar_arrive(&sm.pfull[st][kFirst < 8 && c == 3]);
-                        }
                     }
                 };
                 // Masked scores are -inf, which only ex2 takes to an exact 0.
@@ -847,6 +830,10 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 } else {
                     probabilities(std::true_type{});
                 }
+                tc::tmem_st_wait();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sm.pfull[st]);
                 const float2 z = tc::unpair(tc::add2(sum[0], sum[1]));
                 l += z.x + z.y;
             }
@@ -888,16 +875,15 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             const float inv = l > 0.0f ? 1.0f / l : l;
             f0 *= inv;
             f1 *= inv;
-            // NaN somewhere: also seen as a sum no row can have (ex2_poly)
-            bool nan = !(l < 0x1p60f);
             using Out = typename std::conditional<kPrefix, float, T>::type;
             constexpr int kVec = 16 / sizeof(Out);  // elements of a 16-byte store
             constexpr int kPass = 4 * kVec;         // columns at a time: 64 bytes of a row
             Out* out = kPrefix
                 ? reinterpret_cast<Out*>(p.part) + (it.slot * p.rows + tok_row * p.heads + head) * p.d
                 : static_cast<Out*>(p.y) + tok_row * p.y_row + head * p.y_head;
-            // Four lanes store four rows together, 64 bytes of one row at a time.
-            const bool store = mine && !(kPrefix && l == 0.0f);
+            // Four lanes store four rows together, 64 bytes of one row at a time. A
+            // row that sees nothing is left to the end.
+            const bool store = mine && l != 0.0f;
             Out* rows[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -907,65 +893,73 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     ? reinterpret_cast<Out*>(addr) + (lane & 3) * kVec
                     : nullptr;
             }
-            for (int x = from; x < to && x < p.d; x += kPass) {
-                uint4 v[4];
+            const int end = to < p.d ? to : p.d;
+            const uint64_t f02 = tc::pair(f0, f0), f12 = tc::pair(f1, f1);
+            uint64_t bad2 = 0;  // 0 times every value: NaN when one is infinite or NaN
+#pragma unroll 1
+            for (int x = from; x < end; x += kPass) {
+                uint4 v[4] = {};
 #pragma unroll
                 for (int g = 0; g < kPass / 16; ++g) {
+                    if (x + g * 16 >= end) break;  // columns there are not computed
                     uint32_t o[16];
-                    float f[16];
-                    // An accumulator without steps holds what an earlier item left.
+                    uint64_t f[8] = {};
                     if (n > 0) {
                         tc::tmem_ld16(o_addr + st * kTile + x + g * 16, o);
                         tc::tmem_ld_wait(o);
-                    }
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) f[y] = f0 == 0.0f ? 0.0f : __uint_as_float(o[y]) * f0;
+                        for (int y = 0; y < 8; ++y) {
+                            f[y] = tc::fma2(tc::pair(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])),
+                                            f02, 0);
+                        }
+                    }
                     if (!it.paired && theirs > 0) {
                         tc::tmem_ld16(o_addr + (st ^ 1) * kTile + x + g * 16, o);
                         tc::tmem_ld_wait(o);
 #pragma unroll
-                        for (int y = 0; y < 16; ++y) {
-                            if (f1 != 0.0f) f[y] = fmaf(__uint_as_float(o[y]), f1, f[y]);
+                        for (int y = 0; y < 8; ++y) {
+                            f[y] = tc::fma2(tc::pair(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])),
+                                            f12, f[y]);
+                        }
+                    }
+                    uint32_t w[16];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        bad2 = tc::fma2(f[y], 0, bad2);
+                        const float2 z = tc::unpair(f[y]);
+                        if constexpr (kPrefix) {
+                            w[2 * y] = __float_as_uint(z.x);
+                            w[2 * y + 1] = __float_as_uint(z.y);
+                        } else {
+                            w[y] = pack2<T>(z.x, z.y);
                         }
                     }
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) nan = nan || (f[y] != f[y] && x + g * 16 + y < p.d);
-                    if constexpr (kPrefix) {
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            v[y] = make_uint4(__float_as_uint(f[4 * y]), __float_as_uint(f[4 * y + 1]),
-                                              __float_as_uint(f[4 * y + 2]), __float_as_uint(f[4 * y + 3]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            v[2 * g + y] = make_uint4(pack2<T>(f[8 * y], f[8 * y + 1]),
-                                                      pack2<T>(f[8 * y + 2], f[8 * y + 3]),
-                                                      pack2<T>(f[8 * y + 4], f[8 * y + 5]),
-                                                      pack2<T>(f[8 * y + 6], f[8 * y + 7]));
-                        }
+                    for (int y = 0; y < (kPrefix ? 4 : 2); ++y) {
+                        v[(kPrefix ? 0 : 2 * g) + y] = make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
                     }
                 }
                 transpose4(v, lane);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (rows[r] != nullptr && x + (lane & 3) * kVec < p.d) {
+                    if (rows[r] != nullptr && x + (lane & 3) * kVec < end) {
                         *reinterpret_cast<uint4*>(rows[r] + x) = v[r];
                     }
                 }
             }
             float lse = l > 0.0f ? fmaf(m, p.c2, log2f(l)) : -INFINITY;
-            __syncwarp();  // a row written again below was stored by other lanes
-            if (mine && nan) {
+            // A NaN somewhere, also seen as a sum no row can have (ex2_poly), or an infinity.
+            const float2 bad = tc::unpair(bad2);
+            const bool again = mine && l != 0.0f && (!(l < 0x1p60f) || bad.x != 0.0f || bad.y != 0.0f);
+            const bool zeros = !kPrefix && mine && l == 0.0f;
+            if (__any_sync(0xffffffffu, again || zeros)) {  // (ordered after the other lanes' stores)
                 float o[D];
-                lse = slowRow<D, T>(p, it, st, row, o);
-                for (int x = from; x < to && x < p.d; ++x) {
-                    if constexpr (kPrefix) {
-                        out[x] = o[x];
-                    } else {
-                        out[x] = static_cast<T>(o[x]);
-                    }
+                if (again) {
+                    lse = slowRow<D, T>(p, it, st, row, o);
+                } else {
+                    for (int x = from; x < end; ++x) o[x] = 0.0f;
                 }
+                for (int x = from; x < end && (again || zeros); ++x) out[x] = static_cast<Out>(o[x]);
             }
             if (kPrefix && mine && from == 0) p.lse[it.slot * p.rows + tok_row * p.heads + head] = lse;
             tc::tc_fence_before();  // the reads above come before the next item's products
