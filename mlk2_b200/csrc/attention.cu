@@ -6,7 +6,10 @@
 // kv head are rows of the same tile (row r of a tile: token r / G, head r % G
 // of the G heads of the kv head), so grouped heads read K and V once.
 //
-// One CTA per SM, persistent. Two streams of work per CTA, each with its own
+// One CTA per SM at a time, one item per CTA of the grid; a running CTA takes
+// the items of CTAs that are not launched yet (cluster launch control), so
+// uneven items spread by themselves and a CTA's set-up is paid once. Two
+// streams of work per CTA, each with its own
 // 128-row query tile, score accumulator and softmax warps:
 //   warps 0-7    stream 0: softmax and epilogue. Two threads share a row, one
 //                for each half of a tile's 64 + 64 keys; they exchange the
@@ -60,15 +63,16 @@ int makeTmap3d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const
 namespace {
 
 constexpr int kTile = 128;   // rows of a query tile, keys of a key tile
-constexpr int kItems = 3;    // item ring
-constexpr int kStages = 5;   // K / V ring
+constexpr int kItems = 2;    // item ring: the one in work and the next
 constexpr int kThreads = 12 * 32;
 constexpr int kMma = 8, kTma = 9, kSched = 10;  // warps; 0 to 7 are softmax warps, 11 is idle
 constexpr int kConsumers = 10;                  // warps that read an item
 constexpr uint64_t kLimitNs = 2000000000ull;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
 constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe
-constexpr int kMaxSlots = 32;     // partial results a row may have
+constexpr int kMaxSlots = 32;     // partial results a row may have: 16 of the prefix, 16 of its own keys
+constexpr int kOwnItems = 4;      // items of own keys an SM should get, and their most key tiles
+constexpr int kOwnTiles = 32;
 
 // What one pass through the pipeline computes. Keys are counted from the
 // item's first; row limits (how many keys token i of a stream sees) are
@@ -114,8 +118,9 @@ struct Params {
     const int32_t* pages;
     int32_t batch, steps, prefix;
     int32_t page, page_shift, wide, n_pages;  // page size; pages of a request; pages in all
-    int32_t pre_items, pre_tiles, pre_splits, pre_mt, pre_paired;  // prefix items
-    int32_t suf_items, suf_keys, suf_chunks, suf_mt;               // request items
+    int32_t pre_items, pre_tiles, pre_splits, pre_mt, pre_pairs;  // prefix items
+    int32_t suf_slots, suf_mt, tickets, sms;                      // request items
+    int32_t* chunk;                                               // keys of a chunk, for the join
     float* part;
     float* lse;
     int64_t rows;  // result rows: batch * steps * heads
@@ -126,20 +131,22 @@ struct Smem {
     static constexpr int kHalves = D / 64;
     static constexpr uint32_t kBox = kTile * 128;          // 16 KB: 128 rows x 64 elements
     static constexpr uint32_t kTileBytes = kHalves * kBox;
+    static constexpr int kStages = D == 64 ? 11 : 5;       // K / V ring: what fits
     uint8_t q[2][kTileBytes];
     uint8_t kv[kStages][kTileBytes];
     Item item[kItems];
+    alignas(16) uint4 cancel;
     uint64_t full[kStages], empty[kStages];
     uint64_t qfull[2], qempty[2];
     uint64_t sfull[2], pfull[2], ofull[2];  // [stream]
     uint64_t xbar[4];                   // [lane quarter]: the streams' warps meet
-    uint64_t ifull[kItems], iempty[kItems];
+    uint64_t ifull[kItems], iempty[kItems], cfull, cnext;
     float2 xch[2][kTile];               // [stream][row]: maximum and sum
     uint32_t tmem_base;
     int abort;
 };
 
-static_assert(sizeof(Smem<128>) <= 227 * 1024, "shared memory of a block");
+static_assert(sizeof(Smem<128>) <= 227 * 1024 && sizeof(Smem<64>) <= 227 * 1024, "shared memory of a block");
 
 __device__ __forceinline__ int ceilDiv(int a, int b) { return (a + b - 1) / b; }
 
@@ -162,9 +169,8 @@ __device__ __forceinline__ void splitTiles(Item& it, int keys) {
 }
 
 // ---- scheduling: packed prompts ------------------------------------------------------
-// Items are (sequence, pair of query tiles, kv head), dealt to the CTAs in
-// order of falling cost (key tiles of the pair), back and forth over the grid,
-// so that the CTAs' sums come out even and the long items start first. No
+// Items are (sequence, pair of query tiles, kv head), numbered in order of
+// falling cost (key tiles of the pair), so that the long ones start first. No
 // list is stored: the warp walks cost levels x groups of 32 sequences, each
 // lane counting its sequence's pairs of exactly that cost.
 struct Walker {
@@ -261,71 +267,135 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
 
 // ---- scheduling: a shared prefix ------------------------------------------------------
 // Items 0 .. pre_items-1: (key split, kv head, query tile or pair) over the
-// prefix, all tokens of the batch as rows; then (request, key chunk, kv head,
-// query tile) over the requests' own keys. Every item writes its slots.
-__device__ void prefixItem(const Params& p, int idx, Item& it) {
-    it.live = 1;
-    it.page_row = 0;
-    it.key0 = 0;
-    if (idx < p.pre_items) {
-        const int mt = idx % p.pre_mt;
-        const int r = idx / p.pre_mt;
-        const int split = r / p.kv_heads;
-        it.kvh = r % p.kv_heads;
-        const int first = split * p.pre_tiles * kTile;
-        int last = first + p.pre_tiles * kTile;
-        last = last < p.prefix ? last : p.prefix;
-        it.paired = p.pre_paired;
-        it.causal = 0;
-        it.src = 0;
-        it.k_row = first;
-        it.nk = last - first;
-        const int tokens = p.batch * p.steps;
-        it.slot = split;
-        for (int st = 0; st < 2; ++st) {
-            const int t0 = (p.pre_paired ? 2 * mt + st : mt) * p.tt;
-            int n = tokens - t0;
-            n = n < 0 ? 0 : n < p.tt ? n : p.tt;
-            it.q_row[st] = t0;
-            it.tok[st] = n;
-            it.vis0[st] = 0;
-            it.n[st] = n > 0 ? ceilDiv(it.nk, kTile) : 0;
-        }
-        if (!it.paired) splitTiles(it, it.nk);
-        return;
-    }
-    idx -= p.pre_items;
-    const int mt = idx % p.suf_mt;
-    int r = idx / p.suf_mt;
-    it.kvh = r % p.kv_heads;
-    r /= p.kv_heads;
-    const int chunk = r % p.suf_chunks, b = r / p.suf_chunks;
+// prefix, all tokens of the batch as rows; then the requests' own keys, cut
+// into chunks: (request and chunk, kv head, query tile).
+struct OwnKeys {
+    int keys;       // of a chunk; 0: not planned yet
+    int64_t items;  // chunks of all requests x kv heads x query tiles
+};
+
+__device__ __forceinline__ int ownLength(const Params& p, int b) {
     const int cap = p.wide * p.page;
     int len = p.lens[b];
     if (len < 0 || len > cap) {
         if (p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
         len = len < 0 ? 0 : cap;
     }
-    const int c0 = chunk * p.suf_keys;
-    int nk = len - c0;
-    nk = nk < 0 ? 0 : nk < p.suf_keys ? nk : p.suf_keys;
-    it.paired = 0;
-    it.causal = 1;
-    it.src = 1;
-    it.nk = nk;
-    it.k_row = p.pages == nullptr ? b * cap + c0 : 0;
-    it.page_row = b * p.wide;
-    it.key0 = c0;
-    const int t0 = mt * p.tt;
-    int n = p.steps - t0;
-    n = n < p.tt ? n : p.tt;
-    it.vis0[0] = it.vis0[1] = len - p.steps + t0 + 1 - c0;
-    it.slot = p.pre_splits + chunk;
-    for (int st = 0; st < 2; ++st) {
-        it.q_row[st] = b * p.steps + t0;
-        it.tok[st] = n;
+    return len;
+}
+
+// The chunk length, from the lengths on the device (the same in every block):
+// enough chunks for kOwnItems items on each SM, but none under 2 tiles or, where there
+// is work enough, over kOwnTiles, and at most suf_slots to a request.
+__device__ void planOwnKeys(const Params& p, OwnKeys& own, int lane) {
+    if (own.keys > 0) return;
+    int64_t tiles = 0;
+    int most = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+        const int n = ceilDiv(ownLength(p, b), kTile);
+        tiles += n;
+        most = n > most ? n : most;
     }
-    splitTiles(it, rowLimit(it, 0, n - 1));
+    most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    const int64_t unit = static_cast<int64_t>(p.kv_heads) * p.suf_mt;
+    const int64_t want = (tiles * unit + kOwnItems * p.sms - 1) / (kOwnItems * p.sms);
+    int per = want < 2 ? 2 : want < kOwnTiles ? static_cast<int>(want) : kOwnTiles;
+    const int least = ceilDiv(most, p.suf_slots);
+    per = per > least ? per : least;
+    int64_t chunks = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+        chunks += ceilDiv(ceilDiv(ownLength(p, b), kTile), per);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) chunks += __shfl_xor_sync(0xffffffffu, chunks, o);
+    own.keys = per * kTile;
+    own.items = chunks * unit;
+}
+
+__device__ bool nextPrefix(const Params& p, OwnKeys& own, Walker& w, int64_t idx, Item& it,
+                           int lane) {
+    if (idx < p.pre_items) {
+        if (lane == 0) {
+            const int mt = static_cast<int>(idx) % p.pre_mt;
+            const int r = static_cast<int>(idx) / p.pre_mt;
+            const int split = r / p.kv_heads;
+            const int first = split * p.pre_tiles * kTile;
+            const int last = min(first + p.pre_tiles * kTile, p.prefix);
+            const int tokens = p.batch * p.steps;
+            it.live = 1;
+            it.page_row = 0;
+            it.key0 = 0;
+            it.kvh = r % p.kv_heads;
+            it.paired = mt < p.pre_pairs;  // the last query tile may be alone
+            it.causal = 0;
+            it.src = 0;
+            it.k_row = first;
+            it.nk = last - first;
+            it.slot = split;
+            for (int st = 0; st < 2; ++st) {
+                const int t0 = (2 * mt + (it.paired ? st : 0)) * p.tt;
+                const int n = max(0, min(tokens - t0, p.tt));
+                it.q_row[st] = t0;
+                it.tok[st] = n;
+                it.vis0[st] = 0;
+                it.n[st] = n > 0 ? ceilDiv(it.nk, kTile) : 0;
+            }
+            if (!it.paired) splitTiles(it, it.nk);
+        }
+        return true;
+    }
+    if (p.suf_slots == 0) return false;
+    planOwnKeys(p, own, lane);
+    idx -= p.pre_items;
+    if (idx == 0 && lane == 0) *p.chunk = own.keys;  // one block meets this number
+    if (idx >= own.items) return false;
+    if (idx < w.before) w = {};  // a new number may stand for items before the last one's
+    const int unit = p.kv_heads * p.suf_mt;
+    for (;;) {  // groups of 32 requests, each lane counting its request's items
+        const int b = w.base + lane;
+        const int len = b < p.batch ? ownLength(p, b) : 0;
+        const int64_t mine = static_cast<int64_t>(ceilDiv(len, own.keys)) * unit;
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+        if (idx >= w.before + total) {
+            w.before += total;
+            w.base += 32;
+            if (w.base >= p.batch) return false;
+            continue;
+        }
+        const int64_t at = idx - w.before;
+        const unsigned hit = __ballot_sync(0xffffffffu, at < upto);
+        if (lane == __ffs(hit) - 1) {
+            const int rem = static_cast<int>(at - (upto - mine));
+            const int chunk = rem / unit, mt = rem % unit % p.suf_mt;
+            const int c0 = chunk * own.keys;
+            const int t0 = mt * p.tt, n = min(p.steps - t0, p.tt);
+            it.live = 1;
+            it.kvh = rem % unit / p.suf_mt;
+            it.paired = 0;
+            it.causal = 1;
+            it.src = 1;
+            it.nk = min(len - c0, own.keys);
+            it.k_row = p.pages == nullptr ? b * p.page + c0 : 0;
+            it.page_row = b * p.wide;
+            it.key0 = c0;
+            it.vis0[0] = it.vis0[1] = len - p.steps + t0 + 1 - c0;
+            it.slot = p.pre_splits + chunk;
+            for (int st = 0; st < 2; ++st) {
+                it.q_row[st] = b * p.steps + t0;
+                it.tok[st] = n;
+            }
+            splitTiles(it, rowLimit(it, 0, n - 1));
+        }
+        return true;
+    }
 }
 
 // ---- one row, key by key ----------------------------------------------------------------
@@ -414,6 +484,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_k1,
                   const __grid_constant__ CUtensorMap map_v1, const __grid_constant__ Params p) {
     using Sm = Smem<D>;
+    constexpr int kStages = Sm::kStages;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
@@ -441,6 +512,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             tc::mbar_init(&sm.ifull[i], 1);
             tc::mbar_init(&sm.iempty[i], kConsumers);
         }
+        tc::mbar_init(&sm.cfull, 1);
+        tc::mbar_init(&sm.cnext, 1);
         sm.abort = 0;
         tc::fence_barrier_init();
         tc::fence_proxy_async();
@@ -469,7 +542,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 
     if (warp == kSched) {
         // ---------------- scheduler ----------------
-        Walker w = {0, 0, 0};
+        Walker w = {};
+        OwnKeys own = {};
         if constexpr (!kPrefix) {
             int most = 0;
             for (int s = lane; s - lane < p.seqs; s += 32) {
@@ -479,26 +553,42 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             most = __reduce_max_sync(0xffffffffu, most);
             w.level = ceilDiv(most, kTile);
         }
-        for (uint32_t i = 0;; ++i) {
-            const uint32_t r = i % kItems;
-            if (i >= kItems &&
-                !tc::mbar_wait(&sm.iempty[r], ((i / kItems) - 1) & 1u, abort, kLimitNs)) {
+        int64_t at = blockIdx.x;  // the block's own item first, then those of blocks not yet launched
+        for (uint32_t n = 0, asked = 0;;) {
+            Item& slot = sm.item[n % kItems];
+            if (n >= kItems &&
+                !tc::mbar_wait(&sm.iempty[n % kItems], ((n / kItems) - 1) & 1u, abort, kLimitNs)) {
                 break;
             }
-            // back and forth over the grid: even rounds ascending, odd descending
-            const int64_t at = static_cast<int64_t>(i) * gridDim.x +
-                               ((i & 1u) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-            bool live;
-            if constexpr (kPrefix) {
-                live = at < p.pre_items + p.suf_items;
-                if (live && lane == 0) prefixItem(p, static_cast<int>(at), sm.item[r]);
-            } else {
-                live = nextPacked(p, w, at, sm.item[r], lane);
+            bool live = false;
+            if (at >= 0) {
+                if constexpr (kPrefix) {
+                    live = nextPrefix(p, own, w, at, slot, lane);
+                } else {
+                    live = nextPacked(p, w, at, slot, lane);
+                }
             }
-            if (!live && lane == 0) sm.item[r].live = 0;
+            if (live || at < 0) {
+                if (!live && lane == 0) slot.live = 0;
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sm.ifull[n % kItems]);
+                if (!live) break;
+                // The next number is asked for towards the end of this item's loads:
+                // earlier would take work that another block is free for.
+                if (!tc::mbar_wait(&sm.cnext, n++ & 1u, abort, kLimitNs)) break;
+                if (kPrefix && at >= p.pre_items) {  // every `tickets`-th item of the requests
+                    at += p.tickets;
+                    continue;
+                }
+            }
+            if (lane == 0) tc::cancel_ask(&sm.cancel, &sm.cfull);
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&sm.ifull[r]);
-            if (!live) break;
+            int never = 0;  // the answer lands before the block may exit
+            if (!tc::mbar_wait(&sm.cfull, asked++ & 1u, &never, kLimitNs)) {
+                if (lane == 0) *abort = 1;
+                break;
+            }
+            at = tc::cancel_answer(&sm.cancel);
         }
     } else if (warp == kTma) {
         // ---------------- TMA producer ----------------
@@ -568,10 +658,12 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             const CUtensorMap* mv = kPrefix && it.src == 1 ? &map_v1 : &map_v0;
             if (it.n[0] > 0) ok = load_q(0);
             for (int t = 0; ok && t < tiles; ++t) {
+                if (t == tiles - 1 && lane == 0) tc::mbar_arrive(&sm.cnext);
                 ok = load_kv(mk, t);
                 if (ok && t == 0 && it.paired && it.n[1] > 0) ok = load_q(1);
                 ok = ok && load_kv(mv, t);
             }
+            if (tiles == 0 && lane == 0) tc::mbar_arrive(&sm.cnext);
         }
         if (*abort) {  // copies in flight land before the CTA may exit
             int never = 0;
@@ -979,17 +1071,27 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 
 // ---- joining the partial results of attention_prefix ----------------------------------------
 // One warp per result row: y = sum_i 2^(lse_i - top) o_i / sum_i 2^(lse_i - top)
-// over the row's slots; slots that saw no key have lse = -inf and are not read.
+// over the row's slots; those that saw no key have lse = -inf and are not read.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_join(const float* __restrict__ part,
-                                                      const float* __restrict__ lse, int slots,
-                                                      int64_t rows, int heads, int d, T* y,
-                                                      int64_t y_row, int64_t y_head) {
+                                                      const float* __restrict__ lse, int splits,
+                                                      int own, const int32_t* __restrict__ chunk,
+                                                      const int32_t* __restrict__ lens, int cap,
+                                                      int64_t rows, int per_request, int heads,
+                                                      int d, T* y, int64_t y_row, int64_t y_head) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (row >= rows) return;
+    // The prefix' slots are all written; of its own keys those of chunks that exist.
+    int slots = splits;
+    if (own > 0) {
+        const int keys = *chunk;
+        int len = lens[row / per_request];
+        len = len < 0 ? 0 : len < cap ? len : cap;
+        slots += (len + keys - 1) / keys;
+    }
     float e[kMaxSlots / 32];
     float top = -INFINITY;
 #pragma unroll
@@ -1125,47 +1227,47 @@ KeySource keySource(const mlkb_heads& k, const mlkb_heads& v) {
 // How attention_prefix cuts its work, from shapes alone (the lengths are on
 // the device).
 struct PrefixPlan {
-    int64_t group, tt, tokens, rows;
-    int64_t paired, mt, tiles, splits, pre_items;
-    int64_t chunk, chunks, suf_mt, suf_items, slots;
+    int64_t tt, rows, pairs, mt, tiles, splits, pre_items;
+    int64_t suf_mt, suf_slots, tickets, slots;
+
+    // The partial results, their log-sums, and the chunk length.
+    int64_t bytes(int64_t d) const { return slots * rows * (d + 1) * 4 + 16; }
 };
 
 PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_heads,
                       int64_t prefix, int64_t cap) {
     PrefixPlan r = {};
-    r.group = heads / kv_heads;
-    r.tt = kTile / r.group;
-    r.tokens = batch * steps;
-    r.rows = r.tokens * heads;
+    r.tt = kTile / (heads / kv_heads);
+    r.rows = batch * steps * heads;
     const int64_t sms = smCount();
-    const int64_t qt = (r.tokens + r.tt - 1) / r.tt;
-    r.paired = qt > 1;
-    r.mt = r.paired ? (qt + 1) / 2 : 1;
+    const int64_t qt = (batch * steps + r.tt - 1) / r.tt;
+    r.pairs = qt / 2;
+    r.mt = (qt + 1) / 2;
     const int64_t tiles = (prefix + kTile - 1) / kTile;
     if (tiles > 0) {
-        // About one item per SM, but no item shorter than 4 tiles and at most 16 splits.
+        // At most 16 splits, none shorter than 2 tiles: the number for which the
+        // items' rounds over the SMs are shortest (an item costs about 2 tiles more).
         const int64_t units = r.mt * kv_heads;
-        int64_t splits = (sms + units - 1) / units;
-        splits = splits < 16 ? splits : 16;
-        int64_t per = (tiles + splits - 1) / splits;
-        per = per > 4 ? per : 4;
-        r.tiles = per;
-        r.splits = (tiles + per - 1) / per;
+        int64_t best = INT64_MAX;
+        for (int64_t s = 1; s <= 16 && s <= (tiles + 1) / 2; ++s) {
+            const int64_t per = (tiles + s - 1) / s, n = (tiles + per - 1) / per;
+            const int64_t cost = (units * n + sms - 1) / sms * (per + 2);
+            if (cost < best) {
+                best = cost;
+                r.tiles = per;
+                r.splits = n;
+            }
+        }
     }
     r.pre_items = r.splits * kv_heads * r.mt;
     r.suf_mt = (steps + r.tt - 1) / r.tt;
-    if (cap > 0) {
-        const int64_t units = batch * kv_heads * r.suf_mt;
-        const int64_t ctiles = (cap + kTile - 1) / kTile;
-        int64_t n = (2 * sms + units - 1) / units;
-        n = n < 16 ? n : 16;
-        int64_t per = (ctiles + n - 1) / n;
-        per = per > 4 ? per : 4;
-        r.chunk = per * kTile;
-        r.chunks = (ctiles + per - 1) / per;
-    }
-    r.suf_items = batch * kv_heads * r.suf_mt * r.chunks;
-    r.slots = r.splits + r.chunks;
+    const int64_t most = (cap + 2 * kTile - 1) / (2 * kTile);  // chunks of 2 tiles
+    r.suf_slots = most < 16 ? most : 16;
+    // The requests' items are numbered modulo the tickets: how many there are is
+    // known on the device only, and a block that finds none costs its launch.
+    const int64_t items = batch * kv_heads * r.suf_mt * r.suf_slots;
+    r.tickets = items < 8 * sms ? items : 8 * sms;
+    r.slots = r.splits + r.suf_slots;
     return r;
 }
 
@@ -1220,8 +1322,8 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
     // Most pairs of query tiles there can be: every sequence may end inside one.
     const int64_t pairs = hq.rows / (2 * p.tt) + (n_seqs < hq.rows ? n_seqs : hq.rows);
     const int64_t items = pairs * kv_heads;
-    const int grid = static_cast<int>(items < smCount() ? items : smCount());
-    return launchAttention<false>(m, p, elem_dtype, grid, asStream(stream));
+    if (items > INT_MAX) return setError(MLKB_ERR_INVALID, "attention: too much work for one call");
+    return launchAttention<false>(m, p, elem_dtype, static_cast<int>(items), asStream(stream));
 }
 
 extern "C" int64_t mlkb_attention_prefix_workspace(int64_t batch, int64_t steps, int64_t heads,
@@ -1236,7 +1338,7 @@ extern "C" int64_t mlkb_attention_prefix_workspace(int64_t batch, int64_t steps,
     }
     const PrefixPlan r =
         planPrefix(batch, steps, heads, kv_heads, prefix_rows, page_size * pages_per_request);
-    return r.slots * r.rows * (d + 1) * 4;
+    return r.bytes(d);
 }
 
 extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* prefix_k,
@@ -1288,11 +1390,11 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
         return setError(MLKB_ERR_INVALID, "attention: lens needed");
     }
     const PrefixPlan r = planPrefix(batch, steps, heads, kv_heads, hpk.rows, cap);
-    if (r.pre_items + r.suf_items > INT_MAX || r.slots > kMaxSlots) {
+    if (r.pre_items + r.tickets > INT_MAX || r.slots > kMaxSlots ||
+        kv_heads * r.suf_mt * r.suf_slots > INT_MAX) {
         return setError(MLKB_ERR_INVALID, "attention: too much work for one call");
     }
-    if (workspace_bytes < r.slots * r.rows * (d + 1) * 4 ||
-        (r.slots > 0 && (workspace == nullptr || !aligned16(workspace)))) {
+    if (workspace_bytes < r.bytes(d) || workspace == nullptr || !aligned16(workspace)) {
         return setError(MLKB_ERR_INVALID,
                         "attention: workspace (16-byte aligned) smaller than "
                         "mlkb_attention_prefix_workspace says");
@@ -1320,13 +1422,14 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     p.pre_tiles = static_cast<int32_t>(r.tiles);
     p.pre_splits = static_cast<int32_t>(r.splits);
     p.pre_mt = static_cast<int32_t>(r.mt);
-    p.pre_paired = static_cast<int32_t>(r.paired);
-    p.suf_items = static_cast<int32_t>(r.suf_items);
-    p.suf_keys = static_cast<int32_t>(r.chunk);
-    p.suf_chunks = static_cast<int32_t>(r.chunks);
+    p.pre_pairs = static_cast<int32_t>(r.pairs);
+    p.suf_slots = static_cast<int32_t>(r.suf_slots);
     p.suf_mt = static_cast<int32_t>(r.suf_mt);
+    p.tickets = static_cast<int32_t>(r.tickets);
+    p.sms = smCount();
     p.rows = r.rows;
-    p.part = static_cast<float*>(workspace);
+    p.chunk = static_cast<int32_t*>(workspace);
+    p.part = static_cast<float*>(workspace) + 4;
     p.lse = p.part + r.slots * r.rows * d;
     Maps m;
     const int box = pages != nullptr && page_size < kTile ? static_cast<int>(page_size) : kTile;
@@ -1335,11 +1438,10 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     if (int st = headsMap(&m.v0, hpv, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
     if (int st = headsMap(&m.k1, hk, kv_heads, d, elem_dtype, 1, box, hq.data)) return st;
     if (int st = headsMap(&m.v1, hv, kv_heads, d, elem_dtype, 1, box, hq.data)) return st;
-    const int64_t items = r.pre_items + r.suf_items;
+    const int64_t items = r.pre_items + r.tickets;
     cudaStream_t s = asStream(stream);
     if (items > 0) {
-        const int grid = static_cast<int>(items < smCount() ? items : smCount());
-        if (int st = launchAttention<true>(m, p, elem_dtype, grid, s)) return st;
+        if (int st = launchAttention<true>(m, p, elem_dtype, static_cast<int>(items), s)) return st;
     }
     const int64_t blocks = (r.rows + 7) / 8;
     if (blocks > INT_MAX) return setError(MLKB_ERR_INVALID, "attention: too many rows");
@@ -1354,13 +1456,15 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     cfg.numAttrs = 1;
     const float* part = p.part;
     const float* lse = p.lse;
-    const int slots = static_cast<int>(r.slots);
+    const int32_t* chunk = p.chunk;
+    const int per_request = p.steps * p.heads, cap32 = static_cast<int>(cap);
     const cudaError_t e =
         elem_dtype == MLKB_F16
-            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, slots, r.rows, p.heads, p.d,
+            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, p.pre_splits, p.suf_slots,
+                                 chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
                                  static_cast<__half*>(hy.data), hy.row_stride, hy.head_stride)
-            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, slots, r.rows,
-                                 p.heads, p.d, static_cast<__nv_bfloat16*>(hy.data), hy.row_stride,
-                                 hy.head_stride);
+            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, p.pre_splits,
+                                 p.suf_slots, chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
+                                 static_cast<__nv_bfloat16*>(hy.data), hy.row_stride, hy.head_stride);
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention join launch");
 }

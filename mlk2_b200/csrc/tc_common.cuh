@@ -339,6 +339,34 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint16_t cta_mask
         : "memory");
 }
 
+// ---- work taken from blocks not yet launched -------------------------------------
+// Asks for the launch of one more block of this grid to be cancelled; the
+// 16-byte answer (16-byte aligned shared memory) arrives on `bar`. Not to be
+// asked again once the answer was no.
+__device__ __forceinline__ void cancel_ask(uint4* answer, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128"
+        " [%0], [%1];" ::"r"(smem_u32(answer)),
+        "r"(smem_u32(bar))
+        : "memory");
+}
+
+// The x index of the block whose launch was cancelled, or -1.
+__device__ __forceinline__ int cancel_answer(const uint4* answer) {
+    int x = -1;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
+        "ld.shared.b128 h, [%1];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, h;\n\t}"
+        : "+r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
+    fence_proxy_async();  // the next answer is written by the async proxy
+    return x;
+}
+
 // ---- descriptors ---------------------------------------------------------------
 // Shared-memory matrix descriptor (sm_100 "version 1"), 128-byte swizzle.
 //   bits  0-13 start address >> 4      bits 16-29 leading byte offset >> 4
