@@ -125,62 +125,87 @@ def qk_softmax_kt(q, kt, y, scale: float, stream=None):
 # ---- attention (device tensors, 16-bit elements) ----------------------------------
 # Unlike the entries above, these take strided views (only the last dimension
 # contiguous) and run on their tensors' device, whichever device is current.
+# A decoding step calls them for microseconds of work, so what they do on the
+# host counts: torch's bindings are looked up once, operands go in one array.
 
-_HEADS = C.c_int64 * 24  # up to six mlkb_heads: data, rows, row stride, head stride
-_HALF_DT = None
+class _Torch:
+    """What the calls below use of torch, bound on first use."""
 
-
-def _heads_args(tensors, names):
-    """The operands as consecutive mlkb_heads, and their element type. Each is
-    [rows, heads, d], or None."""
-    global _HALF_DT
-    if _HALF_DT is None:
+    def __init__(self):
         import torch
 
-        _HALF_DT = {torch.float16: F16, torch.bfloat16: BF16}
-    flat = []
+        self.dtypes = {torch.float16: F16, torch.bfloat16: BF16}
+        self.int32, self.float32, self.uint8 = torch.int32, torch.float32, torch.uint8
+        self.empty, self.device = torch.empty, torch.cuda.device
+        self.external_stream = torch.cuda.ExternalStream
+        self.current_device = torch.cuda.current_device
+        self.current_stream = torch.cuda.current_stream
+        # the stream's handle without the object around it, where torch has it
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+_torch = None
+_HEADS = {n: C.c_int64 * (4 * n) for n in (4, 6)}  # mlkb_heads: data, rows, row and head stride
+
+
+def _bind():
+    global _torch
+    if _torch is None:
+        _torch = _Torch()
+    return _torch
+
+
+def _heads(tensors, names):
+    """The operands ([rows, heads, d] each, [a, b, heads, d] taken as [a * b,
+    heads, d], or None) as consecutive mlkb_heads, their element type and the
+    index of their device."""
     first = tensors[0]
-    dtype, device = first.dtype, first.device
-    if dtype not in _HALF_DT:
+    dtype, index = first.dtype, first.get_device()
+    code = _bind().dtypes.get(dtype)
+    if code is None:
         raise ValueError(f"{names[0]}: dtype must be float16 or bfloat16, got {dtype}")
-    for t, name in zip(tensors, names):
+    if index < 0:
+        raise ValueError(f"{names[0]}: must be on a CUDA device, not {first.device}")
+    flat = []
+    for i, t in enumerate(tensors):
         if t is None:
             flat += (0, 0, 0, 0)
             continue
-        if t.dtype is not dtype or t.device != device:
-            raise ValueError(f"{name}: {t.dtype} on {t.device}, but {names[0]} is {dtype} on {device}")
-        rows, heads, _ = t.shape
-        row, head, last = t.stride()
-        if last != 1 and t.shape[2] > 1:
-            raise ValueError(f"{name}: the last dimension must be contiguous")
-        flat += (t.data_ptr(), rows, row, head)
-    return _HEADS(*flat), _HALF_DT[dtype]
+        if t.dtype is not dtype or t.get_device() != index:
+            raise ValueError(f"{names[i]}: {t.dtype} on {t.device}, but {names[0]} is {dtype} on "
+                             f"{first.device}")
+        shape, strides = t.shape, t.stride()
+        if len(shape) == 4:
+            rows, row = shape[0] * shape[1], strides[1] if shape[1] > 1 else strides[0]
+            if shape[0] > 1 and strides[0] != shape[1] * row and shape[1] > 1:
+                raise ValueError(f"{names[i]}: its first two dimensions must have one common stride")
+        else:
+            rows, row = shape[0], strides[0]
+        if strides[-1] != 1 and shape[-1] > 1:
+            raise ValueError(f"{names[i]}: the last dimension must be contiguous")
+        flat += (t.data_ptr(), rows, row, strides[-2])
+    return _HEADS[len(tensors)](*flat), code, index
 
 
-def _int32_ptr(t, name, device, shape):
-    import torch
-
+def _int32(t, name, index, shape):
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous int32 on {device} needed")
-    if tuple(t.shape) != shape:
+    if t.dtype is not _torch.int32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous int32 on CUDA device {index} needed")
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
     return t.data_ptr()
 
 
-def _on_device(device, stream, call):
-    """call(stream handle) with `device` current (the default stream is the
-    device's current one)."""
-    import torch
-
-    if device.type != "cuda":
-        raise ValueError(f"tensors must be on a CUDA device, not {device}")
-    if device.index == torch.cuda.current_device():
-        check(call(_stream(stream)))
-    else:
-        with torch.cuda.device(device):
-            check(call(_stream(stream)))
+def _call(fn, args, index, stream):
+    """fn(*args, stream) with device `index` current, on its current stream by default."""
+    if index != _torch.current_device():
+        with _torch.device(index):
+            return _call(fn, args, index, stream)
+    status = fn(*args, _torch.raw_stream(index) if stream is None else int(stream))
+    if status != 0:
+        check(status)
 
 
 def norm_rope(q, k, q_out, k_out, table, positions, sections=None, q_weight=None, k_weight=None,
@@ -193,34 +218,37 @@ def norm_rope(q, k, q_out, k_out, table, positions, sections=None, q_weight=None
     positions: int32 [tokens], or [axes, tokens] with `sections`, the number
     of pairs each axis turns. A token whose position is outside the table is
     left as it is (take_device_error() then reports it)."""
-    import torch
-
-    tokens, heads, d = q.shape
-    kv = 0 if k is None else k.shape[1]
-    ops, dt = _heads_args((q, k, q_out, k_out), ("q", "k", "q_out", "k_out"))
-    device = q.device
-    if q_out.shape != q.shape or (k is None) != (k_out is None) or (
-            k is not None and (k_out.shape != k.shape or k.shape[0] != tokens or k.shape[2] != d)):
-        raise ValueError("q_out and k_out must have the shapes of q and k, of equal tokens and d")
-    if table.dtype is not torch.float32 or table.device != device or not table.is_contiguous() \
+    ops, dt, index = _heads((q, k, q_out, k_out), ("q", "k", "q_out", "k_out"))
+    shape = q.shape
+    tokens, heads, d = shape
+    kv = 0
+    if q_out.shape != shape or (k is None) != (k_out is None):
+        raise ValueError("q_out and k_out must have the shapes of q and k")
+    if k is not None:
+        kv = k.shape[1]
+        if k.shape != (tokens, kv, d) or k_out.shape != k.shape:
+            raise ValueError("k and k_out must have the tokens and d of q")
+    if table.dtype is not _torch.float32 or table.get_device() != index or not table.is_contiguous() \
             or table.dim() != 2:
         raise ValueError("table: contiguous float32 [positions, rot] on the device of q needed")
-    axes = 1 if positions.dim() == 1 else positions.shape[0]
-    pos = _int32_ptr(positions, "positions", device,
-                     (tokens,) if positions.dim() == 1 else (axes, tokens))
-    if sections is not None and len(sections) != axes:
-        raise ValueError(f"sections: {len(sections)} given for {axes} position axes")
-    sec = (C.c_int32 * axes)(*sections) if sections is not None else None
-    ptrs = []
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None and (w.dtype is not q.dtype or w.device != device or not w.is_contiguous()
-                              or tuple(w.shape) != (d,)):
-            raise ValueError(f"{name}: contiguous [{d}] of {q.dtype} on {device} needed")
-        ptrs.append(None if w is None else w.data_ptr())
     table_rows, rot = table.shape
-    _on_device(device, stream, lambda s: lib().mlkb_norm_rope(
-        ops, C.byref(ops, 32), C.byref(ops, 64), C.byref(ops, 96), heads, kv, d, rot, ptrs[0], ptrs[1],
-        eps, table.data_ptr(), table_rows, pos, tokens, sec, axes, int(interleaved), dt, s))
+    axes = 1 if positions.dim() == 1 else positions.shape[0]
+    pos = _int32(positions, "positions", index, (tokens,) if positions.dim() == 1 else (axes, tokens))
+    sec = None
+    if sections is not None:
+        if len(sections) != axes:
+            raise ValueError(f"sections: {len(sections)} given for {axes} position axes")
+        sec = (C.c_int32 * axes)(*sections)
+    weights = []
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None and (w.dtype is not q.dtype or w.get_device() != index or not w.is_contiguous()
+                              or w.shape != (d,)):
+            raise ValueError(f"{name}: contiguous [{d}] of {q.dtype} on the device of q needed")
+        weights.append(None if w is None else w.data_ptr())
+    at = C.addressof(ops)
+    _call(lib().mlkb_norm_rope,
+          (at, at + 32, at + 64, at + 96, heads, kv, d, rot, *weights, eps, table.data_ptr(),
+           table_rows, pos, tokens, sec, axes, int(interleaved), dt), index, stream)
 
 
 def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool = True, stream=None):
@@ -230,29 +258,27 @@ def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool 
     int32 [sequences + 1]: sequence s has the rows starts[s] .. starts[s+1]-1.
     causal: the last query of a sequence sees its last key. Rows of y outside
     the sequences are left as they were; a query that sees no key gets zeros."""
-    ops, dt = _heads_args((q, k, v, y), ("q", "k", "v", "y"))
-    rows, heads, d = q.shape
+    ops, dt, index = _heads((q, k, v, y), ("q", "k", "v", "y"))
+    _, heads, d = q.shape
     kv = k.shape[1]
     if y.shape != q.shape or v.shape != k.shape or k.shape[2] != d:
         raise ValueError("y must have the shape of q, v that of k, and all the same d")
-    device = q.device
     n = q_starts.shape[0]
     if n < 1:
         raise ValueError("q_starts: sequences + 1 entries needed")
-    qs = _int32_ptr(q_starts, "q_starts", device, (n,))
-    ks = _int32_ptr(k_starts, "k_starts", device, (n,))
-    _on_device(device, stream, lambda s: lib().mlkb_attention_packed(
-        ops, C.byref(ops, 32), C.byref(ops, 64), C.byref(ops, 96), heads, kv, d, qs, ks, n - 1,
-        int(causal), scale, dt, s))
+    qs = _int32(q_starts, "q_starts", index, (n,))
+    ks = _int32(k_starts, "k_starts", index, (n,))
+    at = C.addressof(ops)
+    _call(lib().mlkb_attention_packed,
+          (at, at + 32, at + 64, at + 96, heads, kv, d, qs, ks, n - 1, int(causal), scale, dt),
+          index, stream)
 
 
 def attention_prefix_workspace(q, prefix_k, k_pages, pages=None) -> int:
     """Bytes of workspace attention_prefix needs for these operands."""
-    import torch
-
     batch, steps, heads, d = q.shape
     wide = pages.shape[1] if pages is not None else min(1, k_pages.shape[0])
-    with torch.cuda.device(q.device):
+    with _bind().device(q.device):
         return lib().mlkb_attention_prefix_workspace(batch, steps, heads, prefix_k.shape[1], d,
                                                      prefix_k.shape[0], k_pages.shape[1], wide)
 
@@ -269,51 +295,40 @@ def attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale: fl
     b's. lens int32 [batch]. workspace: a CUDA tensor of at least
     attention_prefix_workspace bytes, allocated here (on the current stream)
     when None."""
-    import torch
-
     batch, steps, heads, d = q.shape
     kv = prefix_k.shape[1]
-    page = k_pages.shape[1]
+    count, page = k_pages.shape[:2]
     if y.shape != q.shape or prefix_v.shape != prefix_k.shape or v_pages.shape != k_pages.shape \
-            or prefix_k.shape[2] != d or tuple(k_pages.shape[2:]) != (kv, d):
+            or prefix_k.shape[2] != d or k_pages.shape[2:] != (kv, d):
         raise ValueError("y must have the shape of q, v that of k, and all the same d and kv heads")
-    flat = [_flat2(t, n) for t, n in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (y, "y"))]
-    ops, dt = _heads_args((flat[0], prefix_k, prefix_v, flat[1], flat[2], flat[3]),
-                          ("q", "prefix_k", "prefix_v", "k_pages", "v_pages", "y"))
-    device = q.device
-    wide = pages.shape[1] if pages is not None else min(1, k_pages.shape[0])
-    if pages is None and k_pages.shape[0] not in (0, batch):
-        raise ValueError("without a page table there must be one page for each request")
-    table = _int32_ptr(pages, "pages", device, (batch, wide))
-    own = _int32_ptr(lens, "lens", device, (batch,))
-
-    def call(s):
-        L = lib()
-        ws = workspace
-        if ws is None:
-            need = L.mlkb_attention_prefix_workspace(batch, steps, heads, kv, d, prefix_k.shape[0],
-                                                     page, wide)
-            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=device)
-            if stream is not None:
-                # the memory returns to the pool on the current stream: not before `stream` is done
-                ws.record_stream(torch.cuda.ExternalStream(int(stream), device=device))
-        elif ws.device != device or not ws.is_contiguous():
-            raise ValueError(f"workspace: contiguous on {device} needed")
-        return L.mlkb_attention_prefix(
-            ops, C.byref(ops, 32), C.byref(ops, 64), C.byref(ops, 96), C.byref(ops, 128),
-            C.byref(ops, 160), batch, steps, heads, kv, d, page, wide, table, own, scale, dt,
-            ws.data_ptr(), ws.numel() * ws.element_size(), s)
-
-    _on_device(device, stream, call)
-
-
-def _flat2(t, name):
-    """[a, b, heads, d] as [a * b, heads, d] without a copy."""
-    a, b, heads, d = t.shape
-    if a > 1 and b > 1 and t.stride(0) != b * t.stride(1):
-        raise ValueError(f"{name}: its first two dimensions must have one common stride")
-    row = t.stride(1) if b > 1 else t.stride(0)
-    return t.as_strided((a * b, heads, d), (row, t.stride(2), t.stride(3)))
+    if pages is None:
+        if count not in (0, batch):
+            raise ValueError("without a page table there must be one page for each request")
+        wide = min(1, count)
+    else:
+        wide = pages.shape[1]
+    ops, dt, index = _heads((q, prefix_k, prefix_v, k_pages, v_pages, y),
+                            ("q", "prefix_k", "prefix_v", "k_pages", "v_pages", "y"))
+    table = _int32(pages, "pages", index, (batch, wide))
+    own = _int32(lens, "lens", index, (batch,))
+    L = lib()
+    if workspace is None:
+        if index != _torch.current_device():
+            with _torch.device(index):
+                return attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale, pages,
+                                        None, stream)
+        need = L.mlkb_attention_prefix_workspace(batch, steps, heads, kv, d, prefix_k.shape[0], page, wide)
+        workspace = _torch.empty(max(need, 0), dtype=_torch.uint8, device=q.device)
+        if stream is not None:
+            # the memory returns to the pool on the current stream: not before `stream` is done
+            workspace.record_stream(_torch.external_stream(int(stream), device=q.device))
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError(f"workspace: contiguous on CUDA device {index} needed")
+    at = C.addressof(ops)
+    _call(L.mlkb_attention_prefix,
+          (at, at + 32, at + 64, at + 96, at + 128, at + 160, batch, steps, heads, kv, d, page, wide,
+           table, own, scale, dt, workspace.data_ptr(), workspace.numel() * workspace.element_size()),
+          index, stream)
 
 
 def fill(out, seed: int, stream_id: int, dist: str, lo: float, hi: float, stream=None):

@@ -6,72 +6,115 @@
 // table rows chosen by the token's position on the pair's axis.
 //
 // HBM-bound: 2 B read and 2 B written per element, about 7 flops. A head row
-// belongs to L lanes (a power of two, >= d/16), each holding two 8-element
-// vectors: the two halves of the same 8 pairs, so a rotation never leaves the
-// lane and only the norm's sum crosses lanes (log2 L shuffles). Elements past
-// `rot` pass through as further vector pairs. A lane's cosines and sines
-// depend on the token alone, so a warp loads them once and applies them to
-// several of the token's head rows.
+// belongs to d/16 lanes, each holding two 8-element vectors: the two halves of
+// the same 8 pairs, so a rotation never leaves the lane and only the norm's sum
+// crosses lanes. Elements past `rot` pass through as further vector pairs. A
+// lane's cosines and sines depend on the token alone, so a warp loads them once
+// and applies them to several of the token's head rows.
 #include "heads.cuh"
+#include "tc_common.cuh"
 
 namespace mlkb {
 namespace {
 
 constexpr int kMaxAxes = 4;
-constexpr int kThreads = 256;
-constexpr int kSteps = 2;   // head-row steps a warp has in flight
-constexpr int kBlocks = 4;  // blocks of an SM
+constexpr int kThreads = 128;
+constexpr int kSteps = 10; // most steps of a warp (each 32 / (d / 16) head rows)
+constexpr int kDepth = 3;  // steps in flight
+constexpr int kBlocks = 6; // blocks of an SM
+
+// One of q and k.
+struct RopeSide {
+    mlkb_heads in, out;
+    const void* weight;
+    int32_t rows, steps;  // head rows of a token, and the steps that do them
+};
 
 struct RopeParams {
-    mlkb_heads q, k, qo, ko;
-    const void* qw;
-    const void* kw;
+    RopeSide side[2];
     const float* table;
     const int32_t* positions;
     int64_t table_rows, pos_stride;
     int32_t ends[kMaxAxes];  // first pair past each axis' section
-    int32_t tokens, heads, rows, d, rot, axes;  // rows: head rows of a token, q's then k's
-    int32_t spw;                                // steps a warp does (each 32 / L head rows)
-    int32_t chunks;                             // warps per token
+    int32_t tokens, d, rot, axes;
+    int32_t steps, chunks;   // steps a warp does; warps that share a token
     float eps, inv_d;
     int* status;
 };
 
-template <typename T, int L, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads, kBlocks) norm_rope_kernel(const RopeParams p) {
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ void copy16(void* smem, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(smem)), "l"(global)
+                 : "memory");
+}
+
+// 8 elements as 4 pairs of f32.
+template <typename T>
+__device__ __forceinline__ void widen(const uint4& u, uint64_t (&x)[4]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2<T>(w[i]);
+        x[i] = tc::pair(f.x, f.y);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 narrow(const uint64_t (&x)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = tc::unpair(x[i]);
+        w[i] = pack2<T>(f.x, f.y);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads, kBlocks)
+norm_rope_kernel(const __grid_constant__ RopeParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const unsigned warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
     const int64_t tok = warp / static_cast<unsigned>(p.chunks);
     if (tok >= p.tokens) return;
-    const int step0 = static_cast<int>(warp - static_cast<unsigned>(tok) * p.chunks) * p.spw;
-    const int c = lane % L, sub = lane / L;
+    // The warp's steps of the token: q's come first, then k's.
+    const int first = static_cast<int>(warp - static_cast<unsigned>(tok) * p.chunks) * p.steps;
+    const int last = min(first + p.steps, p.side[0].steps + p.side[1].steps);
+    const int units = p.d >> 4, rows = 32 / units;  // lanes of a head row, head rows of a step
+    const int sub = lane / units, c = lane - sub * units;
     const int half = p.rot >> 1, nrot = p.rot >> 4;
-    const bool live = c < p.d / 16, turned = c < nrot;
+    const bool live = sub < rows, turned = c < nrot;
     // element offsets of the lane's two vectors
     const int e0 = turned ? 8 * c : p.rot + 16 * (c - nrot);
     const int e1 = turned ? half + 8 * c : e0 + 8;
-    constexpr int kRowsPerStep = 32 / L;
 
-    uint4 va[kSteps], vb[kSteps];
-    int row[kSteps];
-    auto load = [&](int st) {
-#pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            row[u] = (st + u < step0 + p.spw) ? (st + u) * kRowsPerStep + sub : p.rows;
-            va[u] = vb[u] = make_uint4(0, 0, 0, 0);
-            if (live && row[u] < p.rows) {
-                const bool isq = row[u] < p.heads;
-                const mlkb_heads& v = isq ? p.q : p.k;
-                const T* x = static_cast<const T*>(v.data) + tok * v.row_stride +
-                             (isq ? row[u] : row[u] - p.heads) * v.head_stride;
-                va[u] = *reinterpret_cast<const uint4*>(x + e0);
-                vb[u] = *reinterpret_cast<const uint4*>(x + e1);
-            }
+    // A lane's vectors arrive through shared memory, kDepth steps ahead: in
+    // registers so many would cost the warps that keep HBM busy. Each lane reads
+    // what it fetched itself.
+    __shared__ uint4 ring[kDepth][2][kThreads];
+    int ahead = first;
+    auto fetch = [&]() {
+        const RopeSide& side = p.side[ahead >= p.side[0].steps ? 1 : 0];
+        const int row = (ahead >= p.side[0].steps ? ahead - p.side[0].steps : ahead) * rows + sub;
+        if (ahead < last && live && row < side.rows) {
+            const T* x = static_cast<const T*>(side.in.data) + tok * side.in.row_stride +
+                         row * side.in.head_stride;
+            const int at = ahead % kDepth;
+            copy16(&ring[at][0][threadIdx.x], x + e0);
+            copy16(&ring[at][1][threadIdx.x], x + e1);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ++ahead;
     };
-    load(step0);  // in flight under the position and the table row below
+#pragma unroll 1
+    for (int u = 0; u < kDepth - 1; ++u) fetch();  // under the position and the table row below
 
     // The lane's cosines and sines: for split pairs (i, i + half), pairs 8c..8c+7
     // serve both vectors; for neighbours (2i, 2i + 1), vector 0 holds pairs
@@ -82,16 +125,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_rope_kernel(const Rope
         const int64_t pos = p.positions[tok];
         bad = pos < 0 || pos >= p.table_rows;
         if (turned && !bad) {
-            const float* row = p.table + pos * p.rot;
+            const float* t = p.table + pos * p.rot;
             const int i0 = kInterleaved ? 4 * c : 8 * c, i1 = kInterleaved ? half / 2 + 4 * c : i0 + 4;
-            const float4 a = *reinterpret_cast<const float4*>(row + i0);
-            const float4 b = *reinterpret_cast<const float4*>(row + i1);
-            const float4 s = *reinterpret_cast<const float4*>(row + half + i0);
-            const float4 t = *reinterpret_cast<const float4*>(row + half + i1);
-            cs[0] = a.x; cs[1] = a.y; cs[2] = a.z; cs[3] = a.w;
-            cs[4] = b.x; cs[5] = b.y; cs[6] = b.z; cs[7] = b.w;
-            sn[0] = s.x; sn[1] = s.y; sn[2] = s.z; sn[3] = s.w;
-            sn[4] = t.x; sn[5] = t.y; sn[6] = t.z; sn[7] = t.w;
+            *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(t + i0);
+            *reinterpret_cast<float4*>(cs + 4) = *reinterpret_cast<const float4*>(t + i1);
+            *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(t + half + i0);
+            *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(t + half + i1);
         }
     } else {
         int64_t pos[kMaxAxes];
@@ -118,89 +157,121 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_rope_kernel(const Rope
         if (lane == 0 && p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
         return;
     }
-
-    for (int st = step0; st < step0 + p.spw; st += kSteps) {
-        if (st > step0) load(st);
+    // As pairs: for split pairs those of two neighbours, else one value twice
+    // (the sine with the signs of the two sums).
+    constexpr int kPairs = kInterleaved ? 8 : 4;
+    uint64_t cs2[kPairs], sn2[kPairs];
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            const bool isq = row[u] < p.heads;
-            const T* w = static_cast<const T*>(isq ? p.qw : p.kw);
-            float a[8], b[8];
-            unpack8<T>(va[u], a);
-            unpack8<T>(vb[u], b);
-            if (p.qw != nullptr) {  // uniform
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-#pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
-                if (__any_sync(0xffffffffu, ss > 3.0e38f)) {
-                    // The squares left the f32 range (bf16 values past 2^63): once
-                    // more on values scaled by 2^-70, exact in f32. (eps has no
-                    // weight there.)
-                    float s2 = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float x = a[i] * 0x1p-70f, y = b[i] * 0x1p-70f;
-                        s2 = fmaf(x, x, fmaf(y, y, s2));
-                    }
-#pragma unroll
-                    for (int o = L / 2; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-                    if (ss > 3.0e38f) r = rsqrtf(s2 * p.inv_d) * 0x1p-70f;
-                }
-                if (live && row[u] < p.rows) {
-                    float wa[8], wb[8];
-                    unpack8<T>(*reinterpret_cast<const uint4*>(w + e0), wa);
-                    unpack8<T>(*reinterpret_cast<const uint4*>(w + e1), wb);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        a[i] = a[i] * r * wa[i];
-                        b[i] = b[i] * r * wb[i];
-                    }
-                }
-            }
-            if (!live || row[u] >= p.rows) continue;
-            if (turned) {
-                if constexpr (kInterleaved) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], t = b[2 * i + 1];
-                        a[2 * i] = x * cs[i] - y * sn[i];
-                        a[2 * i + 1] = y * cs[i] + x * sn[i];
-                        b[2 * i] = z * cs[4 + i] - t * sn[4 + i];
-                        b[2 * i + 1] = t * cs[4 + i] + z * sn[4 + i];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float x = a[i], y = b[i];
-                        a[i] = x * cs[i] - y * sn[i];
-                        b[i] = y * cs[i] + x * sn[i];
-                    }
-                }
-            }
-            const mlkb_heads& v = isq ? p.qo : p.ko;
-            T* y = static_cast<T*>(v.data) + tok * v.row_stride +
-                   (isq ? row[u] : row[u] - p.heads) * v.head_stride;
-            *reinterpret_cast<uint4*>(y + e0) = pack8<T>(a);
-            *reinterpret_cast<uint4*>(y + e1) = pack8<T>(b);
+    for (int i = 0; i < kPairs; ++i) {
+        cs2[i] = kInterleaved ? tc::pair(cs[i], cs[i]) : tc::pair(cs[2 * i], cs[2 * i + 1]);
+        sn2[i] = kInterleaved ? tc::pair(-sn[i], sn[i]) : tc::pair(sn[2 * i], sn[2 * i + 1]);
+    }
+    uint64_t wa[4] = {}, wb[4] = {};
+    const bool norm = p.side[0].weight != nullptr;
+    const bool butterfly = (units & (units - 1)) == 0;
+    auto sum = [&](float v) {  // over the lanes of a head row
+        if (butterfly) {
+            for (int o = units >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            return v;
         }
+        float t = v;
+        for (int o = 1, at = c + 1; o < units; ++o, ++at) {
+            if (at == units) at = 0;
+            t += __shfl_sync(0xffffffffu, v, sub * units + at);
+        }
+        return t;
+    };
+
+    for (int step = first; step < last; ++step) {
+        const bool second = step >= p.side[0].steps;
+        const RopeSide& side = p.side[second ? 1 : 0];
+        const int row = (second ? step - p.side[0].steps : step) * rows + sub;
+        const bool mine = live && row < side.rows;
+        if (norm && live && (step == first || step == p.side[0].steps)) {
+            const T* w = static_cast<const T*>(side.weight);
+            widen<T>(*reinterpret_cast<const uint4*>(w + e0), wa);
+            widen<T>(*reinterpret_cast<const uint4*>(w + e1), wb);
+        }
+        fetch();
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        uint64_t a[4], b[4];
+        widen<T>(ring[step % kDepth][0][threadIdx.x], a);
+        widen<T>(ring[step % kDepth][1][threadIdx.x], b);
+        if (norm) {  // uniform
+            uint64_t s2[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s2[0] = tc::fma2(a[i], a[i], s2[0]);
+                s2[1] = tc::fma2(b[i], b[i], s2[1]);
+            }
+            const float2 sa = tc::unpair(tc::add2(s2[0], s2[1]));
+            const float ss = sum(mine ? sa.x + sa.y : 0.0f);
+            float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
+            if (__any_sync(0xffffffffu, ss > 3.0e38f)) {
+                // The squares left the f32 range (bf16 values past 2^63): once more
+                // on values scaled by 2^-70, exact in f32. (eps has no weight there.)
+                float t = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = tc::unpair(a[i]), g = tc::unpair(b[i]);
+                    const float f0 = f.x * 0x1p-70f, f1 = f.y * 0x1p-70f;
+                    const float g0 = g.x * 0x1p-70f, g1 = g.y * 0x1p-70f;
+                    t += fmaf(f0, f0, f1 * f1) + fmaf(g0, g0, g1 * g1);
+                }
+                t = sum(mine ? t : 0.0f);
+                if (ss > 3.0e38f) r = rsqrtf(t * p.inv_d) * 0x1p-70f;
+            }
+            const uint64_t r2 = tc::pair(r, r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = mul2(mul2(a[i], r2), wa[i]);
+                b[i] = mul2(mul2(b[i], r2), wb[i]);
+            }
+        }
+        if (!mine) continue;
+        if (turned) {
+            if constexpr (kInterleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = tc::unpair(a[i]), g = tc::unpair(b[i]);
+                    a[i] = tc::fma2(a[i], cs2[i], mul2(tc::pair(f.y, f.x), sn2[i]));
+                    b[i] = tc::fma2(b[i], cs2[4 + i], mul2(tc::pair(g.y, g.x), sn2[4 + i]));
+                }
+            } else {
+                const uint64_t minus = tc::pair(-1.0f, -1.0f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint64_t f = a[i], g = b[i];
+                    a[i] = tc::fma2(mul2(g, minus), sn2[i], mul2(f, cs2[i]));
+                    b[i] = tc::fma2(f, sn2[i], mul2(g, cs2[i]));
+                }
+            }
+        }
+        T* y = static_cast<T*>(side.out.data) + tok * side.out.row_stride +
+               row * side.out.head_stride;
+        *reinterpret_cast<uint4*>(y + e0) = narrow<T>(a);
+        *reinterpret_cast<uint4*>(y + e1) = narrow<T>(b);
     }
 }
 
-template <typename T, int L>
+template <typename T>
 int launchNormRope(RopeParams& p, bool interleaved, cudaStream_t s) {
-    const int steps = (p.rows + 32 / L - 1) / (32 / L);
-    // Few tokens: a warp takes one step, so that they spread over the SMs. Many:
-    // kSteps, whose loads are in flight together and share the table row.
-    const int64_t all = static_cast<int64_t>(p.tokens) * steps;
-    p.chunks = all <= static_cast<int64_t>(smCount()) * 32 ? steps : (steps + kSteps - 1) / kSteps;
-    p.spw = (steps + p.chunks - 1) / p.chunks;
-    const int64_t blocks = (static_cast<int64_t>(p.tokens) * p.chunks + kThreads / 32 - 1) / (kThreads / 32);
-    if (blocks > 0x7fffffff / (kThreads / 32)) return setError(MLKB_ERR_INVALID, "norm_rope: too many head rows");
+    const int rows = 32 / (p.d / 16);
+    int total = 0;
+    for (RopeSide& side : p.side) {
+        side.steps = (side.rows + rows - 1) / rows;
+        total += side.steps;
+    }
+    // A warp's steps share the token's position, table row and weights: up to
+    // kSteps of them where that leaves 32 warps to an SM.
+    const int64_t most = static_cast<int64_t>(p.tokens) * total / (static_cast<int64_t>(smCount()) * 32);
+    const int steps = most < 1 ? 1 : most < kSteps ? static_cast<int>(most) : kSteps;
+    p.chunks = (total + steps - 1) / steps;
+    p.steps = (total + p.chunks - 1) / p.chunks;
+    const int64_t warps = static_cast<int64_t>(p.tokens) * p.chunks;
+    if (warps > 0x7fffff00) return setError(MLKB_ERR_INVALID, "norm_rope: too many head rows");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.gridDim = dim3(static_cast<unsigned>((warps + kThreads / 32 - 1) / (kThreads / 32)));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
     cudaLaunchAttribute pdl[1];
@@ -208,20 +279,9 @@ int launchNormRope(RopeParams& p, bool interleaved, cudaStream_t s) {
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
-    const cudaError_t e = interleaved ? cudaLaunchKernelEx(&cfg, norm_rope_kernel<T, L, true>, p)
-                                      : cudaLaunchKernelEx(&cfg, norm_rope_kernel<T, L, false>, p);
+    const cudaError_t e = interleaved ? cudaLaunchKernelEx(&cfg, norm_rope_kernel<T, true>, p)
+                                      : cudaLaunchKernelEx(&cfg, norm_rope_kernel<T, false>, p);
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "norm_rope launch");
-}
-
-template <typename T>
-int launchNormRope(RopeParams& p, bool interleaved, cudaStream_t s) {
-    const int units = p.d / 16;
-    return units <= 1    ? launchNormRope<T, 1>(p, interleaved, s)
-           : units <= 2  ? launchNormRope<T, 2>(p, interleaved, s)
-           : units <= 4  ? launchNormRope<T, 4>(p, interleaved, s)
-           : units <= 8  ? launchNormRope<T, 8>(p, interleaved, s)
-           : units <= 16 ? launchNormRope<T, 16>(p, interleaved, s)
-                         : launchNormRope<T, 32>(p, interleaved, s);
 }
 
 }  // namespace
@@ -252,14 +312,15 @@ extern "C" int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const ml
         return setError(MLKB_ERR_INVALID, "norm_rope: weights must be 16-byte aligned");
     }
     RopeParams p = {};
-    if (int st = checkHeads(q, heads, d, false, "norm_rope q", &p.q)) return st;
-    if (int st = checkHeads(q_out, heads, d, true, "norm_rope q_out", &p.qo)) return st;
+    RopeSide &qs = p.side[0], &ks = p.side[1];
+    if (int st = checkHeads(q, heads, d, false, "norm_rope q", &qs.in)) return st;
+    if (int st = checkHeads(q_out, heads, d, true, "norm_rope q_out", &qs.out)) return st;
     if (kv_heads > 0) {
-        if (int st = checkHeads(k, kv_heads, d, false, "norm_rope k", &p.k)) return st;
-        if (int st = checkHeads(k_out, kv_heads, d, true, "norm_rope k_out", &p.ko)) return st;
+        if (int st = checkHeads(k, kv_heads, d, false, "norm_rope k", &ks.in)) return st;
+        if (int st = checkHeads(k_out, kv_heads, d, true, "norm_rope k_out", &ks.out)) return st;
     }
-    const int64_t tokens = p.q.rows;
-    if (p.qo.rows != tokens || (kv_heads > 0 && (p.k.rows != tokens || p.ko.rows != tokens))) {
+    const int64_t tokens = qs.in.rows;
+    if (qs.out.rows != tokens || (kv_heads > 0 && (ks.in.rows != tokens || ks.out.rows != tokens))) {
         return setError(MLKB_ERR_INVALID, "norm_rope: q, k and their outputs must have equal rows");
     }
     if (n_axes < 1 || n_axes > kMaxAxes || (n_axes > 1 && sections == nullptr)) {
@@ -286,15 +347,15 @@ extern "C" int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const ml
         return setError(MLKB_ERR_INVALID, "norm_rope: negative position stride");
     }
     if (int st = needDevice()) return st;
-    p.qw = q_weight;
-    p.kw = k_weight;
+    qs.weight = q_weight;
+    ks.weight = k_weight;
+    qs.rows = static_cast<int32_t>(heads);
+    ks.rows = static_cast<int32_t>(kv_heads);
     p.table = table;
     p.positions = positions;
     p.table_rows = table_rows;
     p.pos_stride = position_stride;
     p.tokens = static_cast<int32_t>(tokens);
-    p.heads = static_cast<int32_t>(heads);
-    p.rows = static_cast<int32_t>(heads + kv_heads);
     p.d = static_cast<int32_t>(d);
     p.rot = static_cast<int32_t>(rot);
     p.axes = n_axes;
