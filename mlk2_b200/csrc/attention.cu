@@ -70,7 +70,7 @@ constexpr int kConsumers = 10;                  // warps that read an item
 constexpr uint64_t kLimitNs = 2000000000ull;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
 constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe
-constexpr int kMaxSlots = 32;     // partial results a row may have: 16 of the prefix, 16 of its own keys
+constexpr int kMaxSlots = 128;    // partial results a row may have: 16 x 4 of the prefix, as many of its own keys
 constexpr int kOwnItems = 4;      // items of own keys an SM should get, and their most key tiles
 constexpr int kOwnTiles = 32;
 
@@ -92,6 +92,7 @@ struct Item {
     int32_t n[2];      // its key tiles
     int32_t vis0[2];
     int32_t slot;      // partial-result slot (prefix)
+    int32_t spread;    // at most 32 rows, four times in the tile: each 32 lanes take 32 of a tile's keys
 };
 
 struct KeySource {
@@ -120,6 +121,8 @@ struct Params {
     int32_t page, page_shift, wide, n_pages;  // page size; pages of a request; pages in all
     int32_t pre_items, pre_tiles, pre_splits, pre_mt, pre_pairs;  // prefix items
     int32_t suf_slots, suf_mt, tickets, sms;                      // request items
+    int32_t pre_spread, suf_spread, spread_tt;  // which items are spread; tokens of a spread tile
+    int32_t pre_parts, suf_parts;               // slots of an item: 4 when spread, else 1
     int32_t* chunk;                                               // keys of a chunk, for the join
     float* part;
     float* lse;
@@ -146,6 +149,7 @@ struct Smem {
     int abort;
 };
 
+static_assert(Smem<128>::kStages > 4 && Smem<64>::kStages > 4, "ring places move by up to 4");
 static_assert(sizeof(Smem<128>) <= 227 * 1024 && sizeof(Smem<64>) <= 227 * 1024, "shared memory of a block");
 
 __device__ __forceinline__ int ceilDiv(int a, int b) { return (a + b - 1) / b; }
@@ -237,6 +241,7 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
                 it.page_row = 0;
                 it.key0 = 0;
                 it.slot = 0;
+                it.spread = 0;
                 for (int st = 0; st < 2; ++st) {
                     const int t0 = (2 * pair + st) * p.tt;
                     int n = s.nq - t0;
@@ -333,7 +338,8 @@ __device__ bool nextPrefix(const Params& p, OwnKeys& own, Walker& w, int64_t idx
             it.src = 0;
             it.k_row = first;
             it.nk = last - first;
-            it.slot = split;
+            it.slot = split * p.pre_parts;
+            it.spread = p.pre_spread;
             for (int st = 0; st < 2; ++st) {
                 const int t0 = (2 * mt + (it.paired ? st : 0)) * p.tt;
                 const int n = max(0, min(tokens - t0, p.tt));
@@ -387,7 +393,8 @@ __device__ bool nextPrefix(const Params& p, OwnKeys& own, Walker& w, int64_t idx
             it.page_row = b * p.wide;
             it.key0 = c0;
             it.vis0[0] = it.vis0[1] = len - p.steps + t0 + 1 - c0;
-            it.slot = p.pre_splits + chunk;
+            it.slot = p.pre_splits * p.pre_parts + chunk * p.suf_parts;
+            it.spread = p.suf_spread;
             for (int st = 0; st < 2; ++st) {
                 it.q_row[st] = b * p.steps + t0;
                 it.tok[st] = n;
@@ -407,9 +414,11 @@ __device__ __forceinline__ int pageRow(const Params& p, const Item& it, int key)
 }
 
 // Row `row` of the query tile from the definition, over the item's keys that
-// the row sees: o (normalised) and the log2 of its sum.
+// the row sees (of a spread item, those of `part`): o (normalised) and the log2
+// of its sum.
 template <int D, typename T>
-__device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, int row, float* o) {
+__device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, int row, int part,
+                                      float* o) {
     const int token = row / p.group, head = it.kvh * p.group + row % p.group;
     const T* q = static_cast<const T*>(p.q) + (it.q_row[st] + token) * p.q_row + head * p.q_head;
     const KeySource& src = p.src[it.src];
@@ -418,6 +427,7 @@ __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, i
     for (int pass = 0; pass < 2; ++pass) {
         for (int c = 0; c < D; ++c) o[c] = 0.0f;
         for (int key = 0; key < lim; ++key) {
+            if (it.spread && (key >> 5 & 3) != part) continue;
             int64_t krow = it.k_row + static_cast<int64_t>(key);
             if (it.src == 1 && p.pages != nullptr) krow = pageRow(p, it, key);
             const T* k = static_cast<const T*>(src.k) + krow * src.k_row + it.kvh * src.k_head;
@@ -479,6 +489,7 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
 template <int D, typename T, bool kPrefix>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
+                  const __grid_constant__ CUtensorMap map_qs,
                   const __grid_constant__ CUtensorMap map_k0,
                   const __grid_constant__ CUtensorMap map_v0,
                   const __grid_constant__ CUtensorMap map_k1,
@@ -593,7 +604,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
     } else if (warp == kTma) {
         // ---------------- TMA producer ----------------
         uint32_t ring = 0, qn[2] = {0, 0};
-        Item it;  // a copy
+        Item it = {};  // a copy
         bool ok = true;
         auto load_q = [&](int st) -> bool {
             if (qn[st] > 0 && !tc::mbar_wait(&sm.qempty[st], (qn[st] - 1) & 1u, abort, kLimitNs)) {
@@ -601,10 +612,18 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             }
             ++qn[st];
             if (lane == 0) {
+                if (kPrefix && it.spread) {  // the same rows for each 32 lanes
+                    tc::mbar_arrive_expect_tx(&sm.qfull[st], Sm::kHalves * 512u * p.group * p.spread_tt);
+                    for (int h = 0; h < 4 * Sm::kHalves; ++h) {
+                        tc::tma_load_3d(sm.q[st] + (h >> 2) * Sm::kBox + (h & 3) * 4096, &map_qs,
+                                        &sm.qfull[st], (h >> 2) * 64, it.kvh * p.group, it.q_row[0]);
+                    }
+                } else {
                 tc::mbar_arrive_expect_tx(&sm.qfull[st], Sm::kHalves * 128u * p.group * p.tt);
                 for (int h = 0; h < Sm::kHalves; ++h) {
                     tc::tma_load_3d(sm.q[st] + h * Sm::kBox, &map_q, &sm.qfull[st], h * 64,
                                     it.kvh * p.group, st == 0 ? it.q_row[0] : it.q_row[1]);
+                }
                 }
             }
             __syncwarp();
@@ -813,8 +832,6 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
     } else if (warp < kMma) {
         // ---------------- softmax and epilogue ----------------
         const int st = warp >> 2, quarter = warp & 3;
-        const int row = quarter * 32 + lane;
-        const int token = row / p.group, head_in = row - token * p.group;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_addr = tmem + lanes + st * kTile;
         const uint32_t o_addr = tmem + lanes + 2 * kTile;  // stream 1's is kTile further
@@ -830,14 +847,35 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             const Item* item = take(i);  // kept in the ring: a copy would not fit the registers
             if (item == nullptr) break;
             const Item& it = *item;
+            const bool spread = kPrefix && it.spread != 0;
+            const int row = (spread ? 0 : quarter * 32) + lane;
+            const int token = row / p.group, head_in = row - token * p.group;
             const int lim = rowLimit(it, st, token);
             const int n = st == 0 ? it.n[0] : it.n[1], theirs = st == 0 ? it.n[1] : it.n[0];
             // keys the row sees from the stream's current tile on
             int left = lim - (it.paired ? 0 : st * kTile);
             const int stride = it.paired ? kTile : 2 * kTile;
-            const bool mine = token < (st == 0 ? it.tok[0] : it.tok[1]) && token < p.tt;
+            const bool mine = token < (st == 0 ? it.tok[0] : it.tok[1]) &&
+                              token < (spread ? p.spread_tt : p.tt);
             const bool idle = !__any_sync(0xffffffffu, mine);  // no row of the warp is wanted
             float m = -INFINITY, l = 0.0f;
+            // Takes a tile's row maximum into m, the sum and the accumulator (`begun`).
+            auto raise = [&](float top, bool begun) {
+                const bool grow = top > m + p.grow;
+                if (!__any_sync(0xffffffffu, grow)) return;
+                const float f = grow ? tc::ex2((m - top) * p.c2) : 1.0f;
+                m = grow ? top : m;
+                l *= f;
+                if (!begun) return;
+                for (int x = 0; x < p.d; x += 16) {
+                    uint32_t o[16];
+                    tc::tmem_ld16(o_addr + st * kTile + x, o);
+                    tc::tmem_ld_wait(o);
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                    tc::tmem_st16(o_addr + st * kTile + x, o);
+                }
+            };
             for (int jj = 0; jj < n; ++jj, ++sn, left -= stride) {
                 if (!tc::mbar_wait(&sm.sfull[st], sn & 1u, abort, kLimitNs)) {
                     ok = false;
@@ -848,6 +886,50 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     continue;
                 }
                 tc::tc_fence_after();
+                if (spread) {
+                    // 32 of the tile's keys; the others' probabilities are zeros here
+                    uint32_t v[32], w[16], zero[16] = {};
+                    tc::tmem_ld32(s_addr + quarter * 32, v);
+                    tc::tmem_ld_wait(v);
+                    const int seen = left - quarter * 32;
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    if (__any_sync(0xffffffffu, seen < 32)) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) {
+                            if (x >= seen) v[x] = __float_as_uint(-INFINITY);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        mx[x / 2 % 2] = tc::max3(mx[x / 2 % 2], __uint_as_float(v[x]),
+                                                 __uint_as_float(v[x + 1]));
+                    }
+                    raise(fmaxf(mx[0], mx[1]), jj > 0);
+                    const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
+                    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const float a = tc::ex2(fmaf(__uint_as_float(v[2 * x]), p.c2, nm));
+                        const float b = tc::ex2(fmaf(__uint_as_float(v[2 * x + 1]), p.c2, nm));
+                        sum[0] += a;
+                        sum[1] += b;
+                        w[x] = pack2<T>(a, b);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (c == quarter) {
+                            tc::tmem_st16(s_addr + c * 16, w);
+                        } else {
+                            tc::tmem_st16(s_addr + c * 16, zero);
+                        }
+                    }
+                    tc::tmem_st_wait();
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&sm.pfull[st]);
+                    l += sum[0] + sum[1];
+                    continue;
+                }
                 // The tile's scores are read twice, 32 at a time, for the row maximum
                 // and for the probabilities: held whole they would spill.
                 const bool masked = __any_sync(0xffffffffu, left < kTile);
@@ -872,22 +954,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     }
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const bool grow = top > m + p.grow;
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? tc::ex2((m - top) * p.c2) : 1.0f;
-                    m = grow ? top : m;
-                    l *= f;
-                    if (jj > 0) {
-                        for (int x = 0; x < p.d; x += 16) {
-                            uint32_t o[16];
-                            tc::tmem_ld16(o_addr + st * kTile + x, o);
-                            tc::tmem_ld_wait(o);
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-                            tc::tmem_st16(o_addr + st * kTile + x, o);
-                        }
-                    }
-                }
+                raise(top, jj > 0);
                 const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
                 const uint64_t c2 = tc::pair(p.c2, p.c2), nm2 = tc::pair(nm, nm);
                 uint64_t sum[2] = {0, 0};
@@ -948,9 +1015,9 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             float f0 = 1.0f, f1 = 0.0f;  // shares of this stream's and the other's accumulator
             int from = 0, to = D;
             if (!it.paired) {
-                sm.xch[st][row] = make_float2(m, l);
+                sm.xch[st][quarter * 32 + lane] = make_float2(m, l);
                 if (!meet()) break;
-                const float2 o = sm.xch[st ^ 1][row];
+                const float2 o = sm.xch[st ^ 1][quarter * 32 + lane];
                 if (theirs > 0 && !tc::mbar_wait(&sm.ofull[st ^ 1], o_other & 1u, abort, kLimitNs)) break;
                 const float both = fmaxf(m, o.x);
                 f0 = l == 0.0f ? 0.0f : tc::ex2((m - both) * p.c2);
@@ -970,8 +1037,9 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             using Out = typename std::conditional<kPrefix, float, T>::type;
             constexpr int kVec = 16 / sizeof(Out);  // elements of a 16-byte store
             constexpr int kPass = 4 * kVec;         // columns at a time: 64 bytes of a row
+            const int64_t slot = it.slot + (spread ? quarter : 0);
             Out* out = kPrefix
-                ? reinterpret_cast<Out*>(p.part) + (it.slot * p.rows + tok_row * p.heads + head) * p.d
+                ? reinterpret_cast<Out*>(p.part) + (slot * p.rows + tok_row * p.heads + head) * p.d
                 : static_cast<Out*>(p.y) + tok_row * p.y_row + head * p.y_head;
             // Four lanes store four rows together, 64 bytes of one row at a time. A
             // row that sees nothing is left to the end.
@@ -1047,13 +1115,13 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             if (__any_sync(0xffffffffu, again || zeros)) {  // (ordered after the other lanes' stores)
                 float o[D];
                 if (again) {
-                    lse = slowRow<D, T>(p, it, st, row, o);
+                    lse = slowRow<D, T>(p, it, st, row, quarter, o);
                 } else {
                     for (int x = from; x < end; ++x) o[x] = 0.0f;
                 }
                 for (int x = from; x < end && (again || zeros); ++x) out[x] = static_cast<Out>(o[x]);
             }
-            if (kPrefix && mine && from == 0) p.lse[it.slot * p.rows + tok_row * p.heads + head] = lse;
+            if (kPrefix && mine && from == 0) p.lse[slot * p.rows + tok_row * p.heads + head] = lse;
             tc::tc_fence_before();  // the reads above come before the next item's products
             const bool together = !it.paired;
             drop(i);
@@ -1075,7 +1143,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 template <typename T>
 __global__ void __launch_bounds__(256) attention_join(const float* __restrict__ part,
                                                       const float* __restrict__ lse, int splits,
-                                                      int own, const int32_t* __restrict__ chunk,
+                                                      int own, int parts,
+                                                      const int32_t* __restrict__ chunk,
                                                       const int32_t* __restrict__ lens, int cap,
                                                       int64_t rows, int per_request, int heads,
                                                       int d, T* y, int64_t y_row, int64_t y_head) {
@@ -1090,7 +1159,7 @@ __global__ void __launch_bounds__(256) attention_join(const float* __restrict__ 
         const int keys = *chunk;
         int len = lens[row / per_request];
         len = len < 0 ? 0 : len < cap ? len : cap;
-        slots += (len + keys - 1) / keys;
+        slots += (len + keys - 1) / keys * parts;
     }
     float e[kMaxSlots / 32];
     float top = -INFINITY;
@@ -1136,7 +1205,7 @@ __global__ void __launch_bounds__(256) attention_join(const float* __restrict__ 
 
 // ---- host ---------------------------------------------------------------------------------
 struct Maps {
-    CUtensorMap q, k0, v0, k1, v1;
+    CUtensorMap q, qs, k0, v0, k1, v1;
 };
 
 // [rows, heads, d] view as a 3-D map, box [box_rows, box_heads, 64]. A view
@@ -1175,7 +1244,7 @@ int launchKernel(const Maps& m, const Params& p, int grid, cudaStream_t s) {
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, m.q, m.k0, m.v0, m.k1, m.v1, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, m.q, m.qs, m.k0, m.v0, m.k1, m.v1, p);
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention launch");
 }
 
@@ -1229,6 +1298,7 @@ KeySource keySource(const mlkb_heads& k, const mlkb_heads& v) {
 struct PrefixPlan {
     int64_t tt, rows, pairs, mt, tiles, splits, pre_items;
     int64_t suf_mt, suf_slots, tickets, slots;
+    int64_t spread_tt, pre_spread, suf_spread;
 
     // The partial results, their log-sums, and the chunk length.
     int64_t bytes(int64_t d) const { return slots * rows * (d + 1) * 4 + 16; }
@@ -1267,7 +1337,12 @@ PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_he
     // known on the device only, and a block that finds none costs its launch.
     const int64_t items = batch * kv_heads * r.suf_mt * r.suf_slots;
     r.tickets = items < 8 * sms ? items : 8 * sms;
-    r.slots = r.splits + r.suf_slots;
+    // Few rows: spread over the tile's lanes. That divides the softmax, the
+    // longest link between two products, by four.
+    r.spread_tt = 32 / (heads / kv_heads);
+    r.pre_spread = r.spread_tt >= batch * steps;
+    r.suf_spread = r.spread_tt >= steps;
+    r.slots = r.splits * (r.pre_spread ? 4 : 1) + r.suf_slots * (r.suf_spread ? 4 : 1);
     return r;
 }
 
@@ -1317,6 +1392,7 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
     if (int st = headsMap(&m.q, hq, heads, d, elem_dtype, p.group, p.tt, nullptr)) return st;
     if (int st = headsMap(&m.k0, hk, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
     if (int st = headsMap(&m.v0, hv, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
+    m.qs = m.q;
     m.k1 = m.k0;
     m.v1 = m.v0;
     // Most pairs of query tiles there can be: every sequence may end inside one.
@@ -1426,6 +1502,11 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     p.suf_slots = static_cast<int32_t>(r.suf_slots);
     p.suf_mt = static_cast<int32_t>(r.suf_mt);
     p.tickets = static_cast<int32_t>(r.tickets);
+    p.pre_spread = static_cast<int32_t>(r.pre_spread);
+    p.suf_spread = static_cast<int32_t>(r.suf_spread);
+    p.spread_tt = static_cast<int32_t>(r.spread_tt);
+    p.pre_parts = r.pre_spread ? 4 : 1;
+    p.suf_parts = r.suf_spread ? 4 : 1;
     p.sms = smCount();
     p.rows = r.rows;
     p.chunk = static_cast<int32_t*>(workspace);
@@ -1434,6 +1515,10 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     Maps m;
     const int box = pages != nullptr && page_size < kTile ? static_cast<int>(page_size) : kTile;
     if (int st = headsMap(&m.q, hq, heads, d, elem_dtype, p.group, p.tt, nullptr)) return st;
+    m.qs = m.q;
+    if (p.pre_spread || p.suf_spread) {
+        if (int st = headsMap(&m.qs, hq, heads, d, elem_dtype, p.group, p.spread_tt, nullptr)) return st;
+    }
     if (int st = headsMap(&m.k0, hpk, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
     if (int st = headsMap(&m.v0, hpv, kv_heads, d, elem_dtype, 1, kTile, hq.data)) return st;
     if (int st = headsMap(&m.k1, hk, kv_heads, d, elem_dtype, 1, box, hq.data)) return st;
@@ -1460,11 +1545,11 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     const int per_request = p.steps * p.heads, cap32 = static_cast<int>(cap);
     const cudaError_t e =
         elem_dtype == MLKB_F16
-            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, p.pre_splits, p.suf_slots,
+            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, p.pre_splits * p.pre_parts, p.suf_slots, p.suf_parts,
                                  chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
                                  static_cast<__half*>(hy.data), hy.row_stride, hy.head_stride)
-            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, p.pre_splits,
-                                 p.suf_slots, chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
+            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, p.pre_splits * p.pre_parts,
+                                 p.suf_slots, p.suf_parts, chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
                                  static_cast<__nv_bfloat16*>(hy.data), hy.row_stride, hy.head_stride);
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention join launch");
 }
