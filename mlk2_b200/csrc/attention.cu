@@ -1044,6 +1044,48 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             // Four lanes store four rows together, 64 bytes of one row at a time. A
             // row that sees nothing is left to the end.
             const bool store = mine && l != 0.0f;
+            const int end = to < p.d ? to : p.d;
+            const uint64_t f02 = tc::pair(f0, f0), f12 = tc::pair(f1, f1);
+            uint64_t bad2 = 0;  // 0 times every value: NaN when one is infinite or NaN
+            if (spread) {
+                // Few rows, each for itself: all of both accumulators at once.
+                if constexpr (kPrefix) {
+                    uint32_t o[D / 32][16], u[D / 32][16];
+#pragma unroll
+                    for (int g = 0; g < D / 32; ++g) {
+                        tc::tmem_ld16(o_addr + st * kTile + from + g * 16, o[g]);
+                        tc::tmem_ld16(o_addr + (st ^ 1) * kTile + from + g * 16, u[g]);
+                    }
+#pragma unroll
+                    for (int g = 0; g < D / 32; ++g) {
+                        tc::tmem_ld_wait(o[g]);
+                        tc::tmem_ld_wait(u[g]);
+                        const bool done = from + g * 16 < p.d;  // columns that were computed
+#pragma unroll
+                        for (int y = 0; y < 16; y += 4) {
+                            uint64_t f[2] = {0, 0};
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) {
+                                const int c = y + 2 * z;
+                                if (n > 0 && done) {
+                                    f[z] = tc::fma2(tc::pair(__uint_as_float(o[g][c]), __uint_as_float(o[g][c + 1])),
+                                                    f02, 0);
+                                }
+                                if (theirs > 0 && done) {
+                                    f[z] = tc::fma2(tc::pair(__uint_as_float(u[g][c]), __uint_as_float(u[g][c + 1])),
+                                                    f12, f[z]);
+                                }
+                                bad2 = tc::fma2(f[z], 0, bad2);
+                            }
+                            if (store && from + g * 16 + y < end) {
+                                const float2 a = tc::unpair(f[0]), b = tc::unpair(f[1]);
+                                *reinterpret_cast<float4*>(out + from + g * 16 + y) =
+                                    make_float4(a.x, a.y, b.x, b.y);
+                            }
+                        }
+                    }
+                }
+            } else {
             Out* rows[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -1053,9 +1095,6 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     ? reinterpret_cast<Out*>(addr) + (lane & 3) * kVec
                     : nullptr;
             }
-            const int end = to < p.d ? to : p.d;
-            const uint64_t f02 = tc::pair(f0, f0), f12 = tc::pair(f1, f1);
-            uint64_t bad2 = 0;  // 0 times every value: NaN when one is infinite or NaN
 #pragma unroll 1
             for (int x = from; x < end; x += kPass) {
                 uint4 v[4] = {};
@@ -1106,6 +1145,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                         *reinterpret_cast<uint4*>(rows[r] + x) = v[r];
                     }
                 }
+            }
             }
             float lse = l > 0.0f ? fmaf(m, p.c2, log2f(l)) : -INFINITY;
             // A NaN somewhere, also seen as a sum no row can have (ex2_poly), or an infinity.
