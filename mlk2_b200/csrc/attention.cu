@@ -71,7 +71,7 @@ constexpr uint64_t kLimitNs = 2000000000ull;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
 constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe
 constexpr int kMaxSlots = 128;    // partial results a row may have: 16 x 4 of the prefix, as many of its own keys
-constexpr int kOwnItems = 4;      // items of own keys an SM should get, and their most key tiles
+constexpr int kOwnItems = 2;      // items of own keys an SM should get, and their most key tiles
 constexpr int kOwnTiles = 32;
 
 // What one pass through the pipeline computes. Keys are counted from the
@@ -126,7 +126,7 @@ struct Params {
     int32_t* chunk;                                               // keys of a chunk, for the join
     float* part;
     float* lse;
-    int64_t rows;  // result rows: batch * steps * heads
+    int32_t slots;  // partial results of a row, side by side
 };
 
 template <int D>
@@ -530,6 +530,16 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         tc::fence_proxy_async();
     }
     if (warp == kMma) tc::tmem_alloc(&sm.tmem_base, 512);
+    if (warp == kTma && lane == 0) {
+        tc::prefetch_tmap(&map_q);
+        tc::prefetch_tmap(&map_k0);
+        tc::prefetch_tmap(&map_v0);
+        if (kPrefix) {
+            tc::prefetch_tmap(&map_qs);
+            tc::prefetch_tmap(&map_k1);
+            tc::prefetch_tmap(&map_v1);
+        }
+    }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -1039,7 +1049,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             constexpr int kPass = 4 * kVec;         // columns at a time: 64 bytes of a row
             const int64_t slot = it.slot + (spread ? quarter : 0);
             Out* out = kPrefix
-                ? reinterpret_cast<Out*>(p.part) + (slot * p.rows + tok_row * p.heads + head) * p.d
+                ? reinterpret_cast<Out*>(p.part) + ((tok_row * p.heads + head) * p.slots + slot) * p.d
                 : static_cast<Out*>(p.y) + tok_row * p.y_row + head * p.y_head;
             // Four lanes store four rows together, 64 bytes of one row at a time. A
             // row that sees nothing is left to the end.
@@ -1161,7 +1171,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
                 for (int x = from; x < end && (again || zeros); ++x) out[x] = static_cast<Out>(o[x]);
             }
-            if (kPrefix && mine && from == 0) p.lse[slot * p.rows + tok_row * p.heads + head] = lse;
+            if (kPrefix && mine && from == 0) p.lse[(tok_row * p.heads + head) * p.slots + slot] = lse;
             tc::tc_fence_before();  // the reads above come before the next item's products
             const bool together = !it.paired;
             drop(i);
@@ -1181,31 +1191,34 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 // One warp per result row: y = sum_i 2^(lse_i - top) o_i / sum_i 2^(lse_i - top)
 // over the row's slots; those that saw no key have lse = -inf and are not read.
 template <typename T>
-__global__ void __launch_bounds__(256) attention_join(const float* __restrict__ part,
-                                                      const float* __restrict__ lse, int splits,
-                                                      int own, int parts,
-                                                      const int32_t* __restrict__ chunk,
-                                                      const int32_t* __restrict__ lens, int cap,
-                                                      int64_t rows, int per_request, int heads,
-                                                      int d, T* y, int64_t y_row, int64_t y_head) {
+__global__ void __launch_bounds__(256)
+attention_join(const float* __restrict__ part, const float* __restrict__ lse, int slots,
+               int prefix_slots, int parts, const int32_t* __restrict__ chunk,
+               const int32_t* __restrict__ lens, int cap, int64_t rows, int per_request, int heads,
+               int d, T* y, int64_t y_row, int64_t y_head) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (row >= rows) return;
     // The prefix' slots are all written; of its own keys those of chunks that exist.
-    int slots = splits;
-    if (own > 0) {
+    const float* mine = lse + row * slots;
+    part += row * slots * d;
+    float e[kMaxSlots / 32];
+#pragma unroll
+    for (int i = 0; i < kMaxSlots / 32; ++i) {
+        e[i] = lane + 32 * i < slots ? mine[lane + 32 * i] : -INFINITY;
+    }
+    if (slots > prefix_slots) {
         const int keys = *chunk;
         int len = lens[row / per_request];
         len = len < 0 ? 0 : len < cap ? len : cap;
-        slots += (len + keys - 1) / keys * parts;
+        slots = prefix_slots + (len + keys - 1) / keys * parts;
     }
-    float e[kMaxSlots / 32];
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kMaxSlots / 32; ++i) {
-        e[i] = lane + 32 * i < slots ? lse[(lane + 32 * i) * rows + row] : -INFINITY;
+        if (lane + 32 * i >= slots) e[i] = -INFINITY;
         top = fmaxf(top, e[i]);
     }
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -1221,18 +1234,24 @@ __global__ void __launch_bounds__(256) attention_join(const float* __restrict__ 
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < kMaxSlots / 32; ++i) {
-#pragma unroll 8
-        for (int s = 0; s < 32; ++s) {
-            if (32 * i + s >= slots) break;
-            const float w = __shfl_sync(0xffffffffu, e[i], s);
-            if (w == 0.0f) continue;  // no key seen there, or nothing beside the others
-            if (live) {
-                const float4 v = *reinterpret_cast<const float4*>(
-                    part + ((32 * i + s) * rows + row) * d + 4 * lane);
-                acc.x = fmaf(w, v.x, acc.x);
-                acc.y = fmaf(w, v.y, acc.y);
-                acc.z = fmaf(w, v.z, acc.z);
-                acc.w = fmaf(w, v.w, acc.w);
+        for (int s = 0; s < 32 && 32 * i + s < slots; s += 8) {  // eight loads at a time
+            float4 v[8];
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = __shfl_sync(0xffffffffu, e[i], s + j);
+                v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                // a weight of 0: no key seen there, or nothing beside the others
+                if (live && w[j] != 0.0f) {
+                    v[j] = *reinterpret_cast<const float4*>(part + (32 * i + s + j) * d + 4 * lane);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                acc.x = fmaf(w[j], v[j].x, acc.x);
+                acc.y = fmaf(w[j], v[j].y, acc.y);
+                acc.z = fmaf(w[j], v[j].z, acc.z);
+                acc.w = fmaf(w[j], v[j].w, acc.w);
             }
         }
     }
@@ -1548,7 +1567,7 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     p.pre_parts = r.pre_spread ? 4 : 1;
     p.suf_parts = r.suf_spread ? 4 : 1;
     p.sms = smCount();
-    p.rows = r.rows;
+    p.slots = static_cast<int32_t>(r.slots);
     p.chunk = static_cast<int32_t*>(workspace);
     p.part = static_cast<float*>(workspace) + 4;
     p.lse = p.part + r.slots * r.rows * d;
@@ -1583,13 +1602,15 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     const float* lse = p.lse;
     const int32_t* chunk = p.chunk;
     const int per_request = p.steps * p.heads, cap32 = static_cast<int>(cap);
+    const int prefix_slots = p.pre_splits * p.pre_parts;
     const cudaError_t e =
         elem_dtype == MLKB_F16
-            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, p.pre_splits * p.pre_parts, p.suf_slots, p.suf_parts,
-                                 chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
+            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, p.slots, prefix_slots,
+                                 p.suf_parts, chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
                                  static_cast<__half*>(hy.data), hy.row_stride, hy.head_stride)
-            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, p.pre_splits * p.pre_parts,
-                                 p.suf_slots, p.suf_parts, chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
-                                 static_cast<__nv_bfloat16*>(hy.data), hy.row_stride, hy.head_stride);
+            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, p.slots,
+                                 prefix_slots, p.suf_parts, chunk, lens, cap32, r.rows, per_request,
+                                 p.heads, p.d, static_cast<__nv_bfloat16*>(hy.data), hy.row_stride,
+                                 hy.head_stride);
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention join launch");
 }
