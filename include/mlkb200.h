@@ -442,11 +442,23 @@ int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* q
  * whatever they or their values hold. A sequence whose starts fall or leave
  * the operands is skipped and raises MLKB_ERR_INVALID in the status word that
  * mlkb_take_device_error returns. y may not overlap the inputs.
+ *   workspace  few queries over many keys are cut along the keys and joined,
+ *              with at least mlkb_attention_packed_workspace bytes of device
+ *              memory (16-byte aligned); NULL or less: they are not cut. In use
+ *              until the call's work on `stream` is done: calls (and captured
+ *              graphs) that may run at the same time need workspaces of their
+ *              own. Its contents do not matter
  */
 int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* v,
                           const mlkb_heads* y, int64_t heads, int64_t kv_heads, int64_t d,
                           const int32_t* q_starts, const int32_t* k_starts, int64_t n_seqs,
-                          int32_t causal, double scale, int32_t elem_dtype, void* stream);
+                          int32_t causal, double scale, int32_t elem_dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace mlkb_attention_packed uses for these shapes on the
+ * current device, 0 where it needs none; negative for shapes it refuses. */
+int64_t mlkb_attention_packed_workspace(int64_t rows, int64_t key_rows, int64_t n_seqs,
+                                        int64_t heads, int64_t kv_heads, int64_t d);
 
 /*
  * Attention of a batch whose requests share a prefix: each request's `steps`

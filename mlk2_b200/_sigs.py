@@ -40,7 +40,8 @@ SIGNATURES = {
     "mlkb_qk_softmax_f16": (i32, [vp, vp, vp, i64, i64, i64, f64, vp]),
     "mlkb_qk_softmax_kt_f16": (i32, [vp, vp, vp, i64, i64, i64, i64, f64, vp]),
     "mlkb_norm_rope": (i32, [vp] * 4 + [i64] * 4 + [vp, vp, f64, vp, i64, vp, i64, vp, i32, i32, i32, vp]),
-    "mlkb_attention_packed": (i32, [vp] * 4 + [i64] * 3 + [vp, vp, i64, i32, f64, i32, vp]),
+    "mlkb_attention_packed": (i32, [vp] * 4 + [i64] * 3 + [vp, vp, i64, i32, f64, i32, vp, i64, vp]),
+    "mlkb_attention_packed_workspace": (i64, [i64] * 6),
     "mlkb_attention_prefix": (i32, [vp] * 6 + [i64] * 7 + [vp, vp, f64, i32, vp, i64, vp]),
     "mlkb_attention_prefix_workspace": (i64, [i64] * 8),
     "mlkb_fill_f32": (i32, [vp, i64, u64, u32, i32, f64, f64, vp]),

@@ -251,16 +251,20 @@ def norm_rope(q, k, q_out, k_out, table, positions, sections=None, q_weight=None
            table_rows, pos, tokens, sec, axes, int(interleaved), dt), index, stream)
 
 
-def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool = True, stream=None):
+def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool = True,
+                     workspace=None, stream=None):
     """y = softmax(scale q k^T) v for each head, over packed sequences.
 
     q, y [rows, heads, d]; k, v [key rows, kv_heads, d]; q_starts, k_starts
     int32 [sequences + 1]: sequence s has the rows starts[s] .. starts[s+1]-1.
     causal: the last query of a sequence sees its last key. Rows of y outside
-    the sequences are left as they were; a query that sees no key gets zeros."""
+    the sequences are left as they were; a query that sees no key gets zeros.
+    workspace: a CUDA tensor of at least attention_packed_workspace bytes (few
+    queries over many keys need one), allocated here (on the current stream)
+    when None."""
     ops, dt, index = _heads((q, k, v, y), ("q", "k", "v", "y"))
-    _, heads, d = q.shape
-    kv = k.shape[1]
+    rows, heads, d = q.shape
+    keys, kv, _ = k.shape
     if y.shape != q.shape or v.shape != k.shape or k.shape[2] != d:
         raise ValueError("y must have the shape of q, v that of k, and all the same d")
     n = q_starts.shape[0]
@@ -268,10 +272,40 @@ def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool 
         raise ValueError("q_starts: sequences + 1 entries needed")
     qs = _int32(q_starts, "q_starts", index, (n,))
     ks = _int32(k_starts, "k_starts", index, (n,))
+    L = lib()
+    ws, size = _workspace(workspace, L.mlkb_attention_packed_workspace,
+                          (rows, keys, n - 1, heads, kv, d), q, index, stream)
     at = C.addressof(ops)
-    _call(lib().mlkb_attention_packed,
-          (at, at + 32, at + 64, at + 96, heads, kv, d, qs, ks, n - 1, int(causal), scale, dt),
-          index, stream)
+    _call(L.mlkb_attention_packed,
+          (at, at + 32, at + 64, at + 96, heads, kv, d, qs, ks, n - 1, int(causal), scale, dt,
+           None if ws is None else ws.data_ptr(), size), index, stream)
+
+
+def attention_packed_workspace(q, k, q_starts) -> int:
+    """Bytes of workspace attention_packed uses for these operands (0: none)."""
+    rows, heads, d = q.shape
+    with _bind().device(q.device):
+        return lib().mlkb_attention_packed_workspace(rows, k.shape[0], q_starts.shape[0] - 1, heads,
+                                                     k.shape[1], d)
+
+
+def _workspace(given, size_of, shape, q, index, stream):
+    """The caller's workspace, or one of size_of(*shape) bytes; and its size."""
+    if given is not None:
+        if given.get_device() != index or not given.is_contiguous():
+            raise ValueError(f"workspace: contiguous on CUDA device {index} needed")
+        return given, given.numel() * given.element_size()
+    if index != _torch.current_device():
+        with _torch.device(index):
+            return _workspace(given, size_of, shape, q, index, stream)
+    need = size_of(*shape)
+    if need <= 0:
+        return None, 0
+    ws = _torch.empty(need, dtype=_torch.uint8, device=q.device)
+    if stream is not None:
+        # the memory returns to the pool on the current stream: not before `stream` is done
+        ws.record_stream(_torch.external_stream(int(stream), device=q.device))
+    return ws, need
 
 
 def attention_prefix_workspace(q, prefix_k, k_pages, pages=None) -> int:
@@ -312,23 +346,12 @@ def attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale: fl
     table = _int32(pages, "pages", index, (batch, wide))
     own = _int32(lens, "lens", index, (batch,))
     L = lib()
-    if workspace is None:
-        if index != _torch.current_device():
-            with _torch.device(index):
-                return attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale, pages,
-                                        None, stream)
-        need = L.mlkb_attention_prefix_workspace(batch, steps, heads, kv, d, prefix_k.shape[0], page, wide)
-        workspace = _torch.empty(max(need, 0), dtype=_torch.uint8, device=q.device)
-        if stream is not None:
-            # the memory returns to the pool on the current stream: not before `stream` is done
-            workspace.record_stream(_torch.external_stream(int(stream), device=q.device))
-    elif workspace.get_device() != index or not workspace.is_contiguous():
-        raise ValueError(f"workspace: contiguous on CUDA device {index} needed")
+    ws, size = _workspace(workspace, L.mlkb_attention_prefix_workspace,
+                          (batch, steps, heads, kv, d, prefix_k.shape[0], page, wide), q, index, stream)
     at = C.addressof(ops)
     _call(L.mlkb_attention_prefix,
           (at, at + 32, at + 64, at + 96, at + 128, at + 160, batch, steps, heads, kv, d, page, wide,
-           table, own, scale, dt, workspace.data_ptr(), workspace.numel() * workspace.element_size()),
-          index, stream)
+           table, own, scale, dt, None if ws is None else ws.data_ptr(), size), index, stream)
 
 
 def fill(out, seed: int, stream_id: int, dist: str, lo: float, hi: float, stream=None):

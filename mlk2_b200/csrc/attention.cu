@@ -91,7 +91,8 @@ struct Item {
     int32_t tok[2];    // its tokens
     int32_t n[2];      // its key tiles
     int32_t vis0[2];
-    int32_t slot;      // partial-result slot (prefix)
+    int32_t slot;      // partial-result slot
+    int32_t parts;     // packed: chunks the keys are cut into
     int32_t spread;    // at most 32 rows, four times in the tile: each 32 lanes take 32 of a tile's keys
 };
 
@@ -113,7 +114,7 @@ struct Params {
     // packed
     const int32_t* q_starts;
     const int32_t* k_starts;
-    int32_t seqs, q_rows, k_rows, causal;
+    int32_t seqs, q_rows, k_rows, causal;  // slots > 0: keys may be cut into as many chunks
     // prefix
     const int32_t* lens;
     const int32_t* pages;
@@ -176,9 +177,11 @@ __device__ __forceinline__ void splitTiles(Item& it, int keys) {
 // Items are (sequence, pair of query tiles, kv head), numbered in order of
 // falling cost (key tiles of the pair), so that the long ones start first. No
 // list is stored: the warp walks cost levels x groups of 32 sequences, each
-// lane counting its sequence's pairs of exactly that cost.
+// lane counting its sequence's pairs of exactly that cost. Where there are few
+// items the keys of the long ones are cut into chunks, items of their own.
 struct Walker {
     int level, base;     // cost level; first sequence of the current group
+    int chunk;           // packed: most key tiles of an item, 0: any
     int64_t before;      // items before (level, group)
 };
 
@@ -217,7 +220,9 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
     for (;;) {
         const Seq s = loadSeq(p, w.base + lane);
         const int ge = pairsFrom(p, s, w.level), gt = pairsFrom(p, s, w.level + 1);
-        const int64_t mine = static_cast<int64_t>(ge - gt) * p.kv_heads;
+        const int parts = w.chunk > 0 && w.level > w.chunk ? ceilDiv(w.level, w.chunk) : 1;
+        const int unit = p.kv_heads * parts;
+        const int64_t mine = static_cast<int64_t>(ge - gt) * unit;
         int64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -231,16 +236,19 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
             const int src = __ffs(hit) - 1;
             const int rem = static_cast<int>(at - (upto - mine));
             if (lane == src) {
-                const int pair = ceilDiv(s.nq, 2 * p.tt) - ge + rem / p.kv_heads;
+                const int pair = ceilDiv(s.nq, 2 * p.tt) - ge + rem / unit;
+                const int part = rem % unit / p.kv_heads;
+                const int c0 = parts > 1 ? part * w.chunk * kTile : 0;
                 it.live = 1;
                 it.causal = p.causal;
                 it.src = 0;
                 it.kvh = rem % p.kv_heads;
-                it.nk = s.nk;
-                it.k_row = s.k0;
+                it.nk = parts > 1 ? min(s.nk - c0, w.chunk * kTile) : s.nk;
+                it.k_row = s.k0 + c0;
                 it.page_row = 0;
                 it.key0 = 0;
-                it.slot = 0;
+                it.slot = part;
+                it.parts = parts;
                 it.spread = 0;
                 for (int st = 0; st < 2; ++st) {
                     const int t0 = (2 * pair + st) * p.tt;
@@ -248,7 +256,7 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
                     n = n < 0 ? 0 : n < p.tt ? n : p.tt;
                     it.q_row[st] = s.q0 + t0;
                     it.tok[st] = n;
-                    it.vis0[st] = s.nk - s.nq + t0 + 1;
+                    it.vis0[st] = s.nk - s.nq + t0 + 1 - c0;
                     it.n[st] = n > 0 ? ceilDiv(rowLimit(it, st, n - 1), kTile) : 0;
                 }
                 it.paired = it.tok[1] > 0;
@@ -486,7 +494,9 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
 }
 
 // ---- the kernel ---------------------------------------------------------------------------
-template <int D, typename T, bool kPrefix>
+// kPrefix: attention_prefix, else attention_packed. kPartial: results go to the
+// slots of the workspace, for the join.
+template <int D, typename T, bool kPrefix, bool kPartial>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_qs,
@@ -567,12 +577,23 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         OwnKeys own = {};
         if constexpr (!kPrefix) {
             int most = 0;
+            int64_t tiles = 0;  // of all pairs, about: a pair in the middle for each
             for (int s = lane; s - lane < p.seqs; s += 32) {
                 const Seq q = loadSeq(p, s);
                 if (q.nq > 0 && q.nk > most) most = q.nk;
+                const int middle = p.causal ? max(q.nk - q.nq / 2, 0) : q.nk;
+                tiles += static_cast<int64_t>(ceilDiv(q.nq, 2 * p.tt)) * ceilDiv(middle, kTile);
             }
             most = __reduce_max_sync(0xffffffffu, most);
             w.level = ceilDiv(most, kTile);
+            if (kPartial) {
+                // About kOwnItems items for each SM, of 4 tiles at least, in the slots there are.
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+                const int64_t want = (tiles * p.kv_heads + kOwnItems * p.sms - 1) / (kOwnItems * p.sms);
+                w.chunk = max(static_cast<int>(min(want, static_cast<int64_t>(w.level) + 1)), 4);
+                w.chunk = max(w.chunk, ceilDiv(w.level, p.slots));
+            }
         }
         int64_t at = blockIdx.x;  // the block's own item first, then those of blocks not yet launched
         for (uint32_t n = 0, asked = 0;;) {
@@ -1044,11 +1065,11 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             const float inv = l > 0.0f ? 1.0f / l : l;
             f0 *= inv;
             f1 *= inv;
-            using Out = typename std::conditional<kPrefix, float, T>::type;
+            using Out = typename std::conditional<kPartial, float, T>::type;
             constexpr int kVec = 16 / sizeof(Out);  // elements of a 16-byte store
             constexpr int kPass = 4 * kVec;         // columns at a time: 64 bytes of a row
             const int64_t slot = it.slot + (spread ? quarter : 0);
-            Out* out = kPrefix
+            Out* out = kPartial
                 ? reinterpret_cast<Out*>(p.part) + ((tok_row * p.heads + head) * p.slots + slot) * p.d
                 : static_cast<Out*>(p.y) + tok_row * p.y_row + head * p.y_head;
             // Four lanes store four rows together, 64 bytes of one row at a time. A
@@ -1059,7 +1080,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             uint64_t bad2 = 0;  // 0 times every value: NaN when one is infinite or NaN
             if (spread) {
                 // Few rows, each for itself: all of both accumulators at once.
-                if constexpr (kPrefix) {
+                if constexpr (kPartial) {
                     uint32_t o[D / 32][16], u[D / 32][16];
 #pragma unroll
                     for (int g = 0; g < D / 32; ++g) {
@@ -1136,7 +1157,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     for (int y = 0; y < 8; ++y) {
                         bad2 = tc::fma2(f[y], 0, bad2);
                         const float2 z = tc::unpair(f[y]);
-                        if constexpr (kPrefix) {
+                        if constexpr (kPartial) {
                             w[2 * y] = __float_as_uint(z.x);
                             w[2 * y + 1] = __float_as_uint(z.y);
                         } else {
@@ -1144,8 +1165,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                         }
                     }
 #pragma unroll
-                    for (int y = 0; y < (kPrefix ? 4 : 2); ++y) {
-                        v[(kPrefix ? 0 : 2 * g) + y] = make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
+                    for (int y = 0; y < (kPartial ? 4 : 2); ++y) {
+                        v[(kPartial ? 0 : 2 * g) + y] = make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
                     }
                 }
                 transpose4(v, lane);
@@ -1161,7 +1182,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             // A NaN somewhere, also seen as a sum no row can have (ex2_poly), or an infinity.
             const float2 bad = tc::unpair(bad2);
             const bool again = mine && l != 0.0f && (!(l < 0x1p60f) || bad.x != 0.0f || bad.y != 0.0f);
-            const bool zeros = !kPrefix && mine && l == 0.0f;
+            const bool zeros = !kPartial && mine && l == 0.0f;
             if (__any_sync(0xffffffffu, again || zeros)) {  // (ordered after the other lanes' stores)
                 float o[D];
                 if (again) {
@@ -1171,7 +1192,13 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
                 for (int x = from; x < end && (again || zeros); ++x) out[x] = static_cast<Out>(o[x]);
             }
-            if (kPrefix && mine && from == 0) p.lse[(tok_row * p.heads + head) * p.slots + slot] = lse;
+            if (kPartial && mine && from == 0) {
+                float* out_lse = p.lse + (tok_row * p.heads + head) * p.slots;
+                out_lse[slot] = lse;
+                if (!kPrefix && it.slot == 0) {  // slots without a chunk
+                    for (int x = it.parts; x < p.slots; ++x) out_lse[x] = -INFINITY;
+                }
+            }
             tc::tc_fence_before();  // the reads above come before the next item's products
             const bool together = !it.paired;
             drop(i);
@@ -1190,30 +1217,49 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 // ---- joining the partial results of attention_prefix ----------------------------------------
 // One warp per result row: y = sum_i 2^(lse_i - top) o_i / sum_i 2^(lse_i - top)
 // over the row's slots; those that saw no key have lse = -inf and are not read.
-template <typename T>
+struct JoinParams {
+    const float* part;
+    const float* lse;
+    int64_t rows, y_row, y_head;
+    int32_t slots, heads, d;
+    // prefix: slots of the prefix, of a chunk of own keys, and the chunk
+    int32_t prefix_slots, parts, cap, per_request;
+    const int32_t* chunk;
+    const int32_t* lens;
+};
+
+template <typename T, bool kPrefix>
 __global__ void __launch_bounds__(256)
-attention_join(const float* __restrict__ part, const float* __restrict__ lse, int slots,
-               int prefix_slots, int parts, const int32_t* __restrict__ chunk,
-               const int32_t* __restrict__ lens, int cap, int64_t rows, int per_request, int heads,
-               int d, T* y, int64_t y_row, int64_t y_head) {
+attention_join(const __grid_constant__ JoinParams p, const __grid_constant__ Params seqs, T* y) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (row >= rows) return;
+    if (row >= p.rows) return;
+    int slots = p.slots;
+    const int d = p.d;
+    if constexpr (!kPrefix) {  // a row of no sequence was not computed
+        const int token = static_cast<int>(row / p.heads);
+        bool mine = false;
+        for (int s = lane; s < seqs.seqs; s += 32) {
+            const Seq q = loadSeq(seqs, s);
+            mine = mine || (token >= q.q0 && token < q.q0 + q.nq);
+        }
+        if (!__any_sync(0xffffffffu, mine)) return;
+    }
     // The prefix' slots are all written; of its own keys those of chunks that exist.
-    const float* mine = lse + row * slots;
-    part += row * slots * d;
+    const float* mine = p.lse + row * slots;
+    const float* part = p.part + row * slots * d;
     float e[kMaxSlots / 32];
 #pragma unroll
     for (int i = 0; i < kMaxSlots / 32; ++i) {
         e[i] = lane + 32 * i < slots ? mine[lane + 32 * i] : -INFINITY;
     }
-    if (slots > prefix_slots) {
-        const int keys = *chunk;
-        int len = lens[row / per_request];
-        len = len < 0 ? 0 : len < cap ? len : cap;
-        slots = prefix_slots + (len + keys - 1) / keys * parts;
+    if (kPrefix && slots > p.prefix_slots) {
+        const int keys = *p.chunk;
+        int len = p.lens[row / p.per_request];
+        len = len < 0 ? 0 : len < p.cap ? len : p.cap;
+        slots = p.prefix_slots + (len + keys - 1) / keys * p.parts;
     }
     float top = -INFINITY;
 #pragma unroll
@@ -1256,7 +1302,7 @@ attention_join(const float* __restrict__ part, const float* __restrict__ lse, in
         }
     }
     if (live) {
-        T* out = y + (row / heads) * y_row + (row % heads) * y_head + 4 * lane;
+        T* out = y + (row / p.heads) * p.y_row + (row % p.heads) * p.y_head + 4 * lane;
         *reinterpret_cast<uint2*>(out) =
             make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
     }
@@ -1281,12 +1327,12 @@ int headsMap(CUtensorMap* map, const mlkb_heads& t, int64_t heads, int64_t d, in
                       CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int D, typename T, bool kPrefix>
+template <int D, typename T, bool kPrefix, bool kPartial>
 int launchKernel(const Maps& m, const Params& p, int grid, cudaStream_t s) {
     static std::atomic<bool> attr[64];
     int dev = 0;
     cudaGetDevice(&dev);
-    auto kernel = attention_tcgen05<D, T, kPrefix>;
+    auto kernel = attention_tcgen05<D, T, kPrefix, kPartial>;
     if (dev >= 0 && dev < 64 && !attr[dev]) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    static_cast<int>(sizeof(Smem<D>)));
@@ -1307,14 +1353,35 @@ int launchKernel(const Maps& m, const Params& p, int grid, cudaStream_t s) {
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention launch");
 }
 
-template <bool kPrefix>
+template <bool kPrefix, bool kPartial>
 int launchAttention(const Maps& m, const Params& p, int dtype, int grid, cudaStream_t s) {
     if (dtype == MLKB_F16) {
-        return p.d <= 64 ? launchKernel<64, __half, kPrefix>(m, p, grid, s)
-                         : launchKernel<128, __half, kPrefix>(m, p, grid, s);
+        return p.d <= 64 ? launchKernel<64, __half, kPrefix, kPartial>(m, p, grid, s)
+                         : launchKernel<128, __half, kPrefix, kPartial>(m, p, grid, s);
     }
-    return p.d <= 64 ? launchKernel<64, __nv_bfloat16, kPrefix>(m, p, grid, s)
-                     : launchKernel<128, __nv_bfloat16, kPrefix>(m, p, grid, s);
+    return p.d <= 64 ? launchKernel<64, __nv_bfloat16, kPrefix, kPartial>(m, p, grid, s)
+                     : launchKernel<128, __nv_bfloat16, kPrefix, kPartial>(m, p, grid, s);
+}
+
+template <bool kPrefix>
+int launchJoin(const JoinParams& j, const Params& p, void* y, int dtype, cudaStream_t s) {
+    const int64_t blocks = (j.rows + 7) / 8;
+    if (blocks > INT_MAX) return setError(MLKB_ERR_INVALID, "attention: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    const cudaError_t e =
+        dtype == MLKB_F16
+            ? cudaLaunchKernelEx(&cfg, attention_join<__half, kPrefix>, j, p, static_cast<__half*>(y))
+            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16, kPrefix>, j, p,
+                                 static_cast<__nv_bfloat16*>(y));
+    return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention join launch");
 }
 
 // Checks what both entries share.
@@ -1350,6 +1417,32 @@ void setShape(Params& p, int64_t heads, int64_t kv_heads, int64_t d, double scal
 
 KeySource keySource(const mlkb_heads& k, const mlkb_heads& v) {
     return {k.data, v.data, k.row_stride, k.head_stride, v.row_stride, v.head_stride};
+}
+
+// How attention_packed cuts its work.
+struct PackedPlan {
+    int64_t items, slots, rows;
+    int64_t bytes(int64_t d) const { return slots * rows * (d + 1) * 4; }
+};
+
+PackedPlan planPacked(int64_t rows, int64_t key_rows, int64_t seqs, int64_t heads, int64_t kv_heads,
+                      int64_t d) {
+    PackedPlan r = {};
+    const int64_t sms = smCount(), pair = 2 * (kTile / (heads / kv_heads));
+    // Most pairs of query tiles there can be: every sequence may end inside one.
+    r.items = (rows / pair + (seqs < rows ? seqs : rows)) * kv_heads;
+    r.rows = rows * heads;
+    // Items for at most half the SMs, and sequences that may be long: keys are cut
+    // into up to 8 chunks. With about an item to an SM joining costs more than it
+    // gives (1030 queries of 5 sequences, 32 heads: 84 us cut, 66 us whole); one
+    // query over 16384 keys, 8 heads to a kv head, KCUT.
+    const int64_t tiles = (key_rows + kTile - 1) / kTile;
+    if (r.items > 0 && 2 * r.items <= sms && tiles > 8) {
+        r.slots = (sms + r.items - 1) / r.items;
+        if (r.slots > tiles / 4) r.slots = tiles / 4;
+        if (r.slots > 8) r.slots = 8;
+    }
+    return r;
 }
 
 // How attention_prefix cuts its work, from shapes alone (the lengths are on
@@ -1412,7 +1505,8 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
                                      const mlkb_heads* y, int64_t heads, int64_t kv_heads,
                                      int64_t d, const int32_t* q_starts, const int32_t* k_starts,
                                      int64_t n_seqs, int32_t causal, double scale,
-                                     int32_t elem_dtype, void* stream) {
+                                     int32_t elem_dtype, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
     using namespace mlkb;
     if (int st = checkShape(heads, kv_heads, d, scale, elem_dtype)) return st;
     mlkb_heads hq = {}, hk = {}, hv = {}, hy = {};
@@ -1423,7 +1517,7 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
     if (hk.rows != hv.rows || hq.rows != hy.rows) {
         return setError(MLKB_ERR_INVALID, "attention: k and v, and q and y, must have equal rows");
     }
-    if (n_seqs < 0 || n_seqs > kMaxHeadRows) {
+    if (n_seqs < 0 || n_seqs > kMaxHeadRows || workspace_bytes < 0) {
         return setError(MLKB_ERR_INVALID, "attention: bad number of sequences");
     }
     if (n_seqs == 0 || hq.rows == 0) return okStatus();
@@ -1454,11 +1548,41 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
     m.qs = m.q;
     m.k1 = m.k0;
     m.v1 = m.v0;
-    // Most pairs of query tiles there can be: every sequence may end inside one.
-    const int64_t pairs = hq.rows / (2 * p.tt) + (n_seqs < hq.rows ? n_seqs : hq.rows);
-    const int64_t items = pairs * kv_heads;
+    const PackedPlan r = planPacked(hq.rows, hk.rows, n_seqs, heads, kv_heads, d);
+    const bool cut = r.slots > 0 && workspace != nullptr && workspace_bytes >= r.bytes(d);
+    const int64_t items = r.items * (cut ? r.slots : 1);
     if (items > INT_MAX) return setError(MLKB_ERR_INVALID, "attention: too much work for one call");
-    return launchAttention<false>(m, p, elem_dtype, static_cast<int>(items), asStream(stream));
+    const int grid = static_cast<int>(items);
+    if (!cut) return launchAttention<false, false>(m, p, elem_dtype, grid, asStream(stream));
+    if (!aligned16(workspace)) {
+        return setError(MLKB_ERR_INVALID, "attention: workspace must be 16-byte aligned");
+    }
+    p.sms = smCount();
+    p.slots = static_cast<int32_t>(r.slots);
+    p.part = static_cast<float*>(workspace);
+    p.lse = p.part + r.slots * r.rows * d;
+    if (int st = launchAttention<false, true>(m, p, elem_dtype, grid, asStream(stream))) return st;
+    JoinParams j = {};
+    j.part = p.part;
+    j.lse = p.lse;
+    j.rows = r.rows;
+    j.y_row = hy.row_stride;
+    j.y_head = hy.head_stride;
+    j.slots = p.slots;
+    j.heads = p.heads;
+    j.d = p.d;
+    return launchJoin<false>(j, p, hy.data, elem_dtype, asStream(stream));
+}
+
+extern "C" int64_t mlkb_attention_packed_workspace(int64_t rows, int64_t key_rows, int64_t n_seqs,
+                                                   int64_t heads, int64_t kv_heads, int64_t d) {
+    using namespace mlkb;
+    if (rows < 0 || key_rows < 0 || n_seqs < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
+        heads / kv_heads > kTile || d < 8 || d > 128 || rows > kMaxHeadRows ||
+        key_rows > kMaxHeadRows || n_seqs > kMaxHeadRows || heads > (1 << 23)) {
+        return -1;
+    }
+    return planPacked(rows, key_rows, n_seqs, heads, kv_heads, d).bytes(d);
 }
 
 extern "C" int64_t mlkb_attention_prefix_workspace(int64_t batch, int64_t steps, int64_t heads,
@@ -1585,32 +1709,22 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     const int64_t items = r.pre_items + r.tickets;
     cudaStream_t s = asStream(stream);
     if (items > 0) {
-        if (int st = launchAttention<true>(m, p, elem_dtype, static_cast<int>(items), s)) return st;
+        if (int st = launchAttention<true, true>(m, p, elem_dtype, static_cast<int>(items), s)) return st;
     }
-    const int64_t blocks = (r.rows + 7) / 8;
-    if (blocks > INT_MAX) return setError(MLKB_ERR_INVALID, "attention: too many rows");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute pdl[1];
-    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    pdl[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = pdl;
-    cfg.numAttrs = 1;
-    const float* part = p.part;
-    const float* lse = p.lse;
-    const int32_t* chunk = p.chunk;
-    const int per_request = p.steps * p.heads, cap32 = static_cast<int>(cap);
-    const int prefix_slots = p.pre_splits * p.pre_parts;
-    const cudaError_t e =
-        elem_dtype == MLKB_F16
-            ? cudaLaunchKernelEx(&cfg, attention_join<__half>, part, lse, p.slots, prefix_slots,
-                                 p.suf_parts, chunk, lens, cap32, r.rows, per_request, p.heads, p.d,
-                                 static_cast<__half*>(hy.data), hy.row_stride, hy.head_stride)
-            : cudaLaunchKernelEx(&cfg, attention_join<__nv_bfloat16>, part, lse, p.slots,
-                                 prefix_slots, p.suf_parts, chunk, lens, cap32, r.rows, per_request,
-                                 p.heads, p.d, static_cast<__nv_bfloat16*>(hy.data), hy.row_stride,
-                                 hy.head_stride);
-    return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention join launch");
+    JoinParams j = {};
+    j.part = p.part;
+    j.lse = p.lse;
+    j.rows = r.rows;
+    j.y_row = hy.row_stride;
+    j.y_head = hy.head_stride;
+    j.slots = p.slots;
+    j.heads = p.heads;
+    j.d = p.d;
+    j.prefix_slots = p.pre_splits * p.pre_parts;
+    j.parts = p.suf_parts;
+    j.cap = static_cast<int32_t>(cap);
+    j.per_request = p.steps * p.heads;
+    j.chunk = p.chunk;
+    j.lens = lens;
+    return launchJoin<true>(j, p, hy.data, elem_dtype, s);
 }

@@ -179,6 +179,49 @@ def test_packed_long(cuda):
     run_packed([2500, 1], [2500, 4100], 4, 2, 128, seed=11)
 
 
+@pytest.mark.parametrize("nq,nk,heads,kv,d,causal", [
+    ([1], [5000], 8, 1, 128, True), ([1, 1, 0, 3], [2000, 130, 700, 3], 4, 4, 64, True),
+    ([40, 7], [1500, 2200], 16, 2, 80, True), ([40, 7], [1500, 2200], 16, 2, 80, False),
+    ([100, 2], [60, 1700], 2, 1, 128, True), ([300], [1400], 4, 1, 96, True),
+    ([2, 2], [9000, 3], 3, 1, 72, True)])
+def test_packed_few_queries_over_many_keys(cuda, nq, nk, heads, kv, d, causal):
+    """Cut along the keys and joined; without a workspace the same values uncut."""
+    g = gen(18)
+    q = normal(g, sum(nq) + 5, heads, d)
+    k, v = normal(g, sum(nk), kv, d), normal(g, sum(nk), kv, d)
+    qs, ks = starts(nq, "cuda"), starts(nk, "cuda")
+    assert api.attention_packed_workspace(q, k, qs) > 0
+    n = sum(nq)
+    want, bound = packed(q[:n], k, v, nq, nk, d ** -0.5, causal)
+    for workspace in (None, torch.empty(0, device="cuda")):
+        y = torch.full_like(q, 5)
+        api.attention_packed(q, k, v, y, qs, ks, d ** -0.5, causal=causal, workspace=workspace)
+        check(y[:n], want, bound)
+        assert (y[n:] == 5).all()
+    need = api.attention_packed_workspace(q, k, qs)
+    y = torch.full_like(q, 5)
+    api.attention_packed(q, k, v, y, qs, ks, d ** -0.5, causal=causal,
+                         workspace=torch.full((need // 4,), torch.nan, device="cuda"))
+    check(y[:n], want, bound)
+    assert (y[n:] == 5).all()
+
+
+def test_packed_cut_keys_with_nan(cuda):
+    """A NaN value among cut keys reaches the queries that see it, and a bad sequence stays out."""
+    g = gen(19)
+    q, k, v = normal(g, 8, 4, 64), normal(g, 3000, 2, 64), normal(g, 3000, 2, 64)
+    v[2997] = torch.nan  # seen by the last three queries of sequence 1
+    y = torch.full_like(q, 5)
+    qs, ks = ints([0, 3, 7, 20]), ints([0, 1400, 3000, 3000])
+    api.attention_packed(q, k, v, y, qs, ks, 0.125)
+    assert api.take_device_error() == mb.ERR_INVALID
+    clean = v.clone()
+    clean[2997] = 0
+    want, bound = packed(q[:7], k, clean, [3, 4], [1400, 1600], 0.125)
+    check(y[:4], want[:4], bound[:4])
+    assert y[4:7].isnan().all() and (y[7] == 5).all()
+
+
 def test_packed_growing_scores(cuda):
     """Row maxima that rise by far more than 2^8 from tile to tile, and fall again."""
     g = gen(12)
