@@ -797,7 +797,46 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
                 __syncwarp();
             }
-            for (int t = 0; ok && (t < n[0] || t < n[1]); ++t) {
+            int t = 0;
+            // The steady state of a pair, without the cases of the loop below: both
+            // streams have a tile t + 1, stream 1 reads each tile last, and what
+            // stream 0 has waited for is there for stream 1.
+            for (; ok && paired && t + 1 < n[0] && t + 1 < n[1]; ++t) {
+                const Place vp = v[0];
+                k[0].move(2);
+                v[0].move(2);
+                const Place kp = k[0];
+                const uint64_t v0 = vdesc + vp.stage * kStep;
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    if (st == 0 && !known[0]) ok = wait(vp) && wait(kp);
+                    ok = ok && tc::mbar_wait(&sm.pfull[st], pphase[st], abort, kLimitNs);
+                    pphase[st] ^= 1u;
+                    if (!ok) break;
+                    if (st == 1) {  // look ahead: the answer comes while the products are issued
+                        Place kn = kp;
+                        kn.move(2);
+                        known[0] = loaded(v[0]) && loaded(kn);
+                    }
+                    tc::tc_fence_after();
+                    if (tc::elect_one()) {
+                        const uint32_t o0 = tmem + 2 * kTile + st * kTile, p0 = tmem + st * kTile;
+#pragma unroll
+                        for (int q = 0; q < kTile / 16; ++q) {
+                            tc::mma_f16_ts(o0, p0 + q * 8, v0 + q * 128, idesc_o, q > 0 || t > 0);
+                        }
+                        if (st == 1) tc::mma_commit(&sm.empty[vp.stage]);
+                        scores(st, st, kp, st == 1, t + 2 == n[st]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (paired && t > 0) {
+                k[1] = k[0];
+                v[1] = v[0];
+                known[0] = known[1] = false;
+            }
+            for (; ok && (t < n[0] || t < n[1]); ++t) {
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     // O (+)= P V of the stream's tile t, then S of its tile t + 1.
