@@ -137,9 +137,9 @@ class _Torch:
         self.dtypes = {torch.float16: F16, torch.bfloat16: BF16}
         self.int32, self.float32, self.uint8 = torch.int32, torch.float32, torch.uint8
         self.empty, self.device = torch.empty, torch.cuda.device
-        self.external_stream = torch.cuda.ExternalStream
+        self.external_stream, self.default_stream = torch.cuda.ExternalStream, torch.cuda.default_stream
+        self.stream = torch.cuda.stream
         self.current_device = torch.cuda.current_device
-        self.current_stream = torch.cuda.current_stream
         # the stream's handle without the object around it, where torch has it
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -260,8 +260,7 @@ def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool 
     causal: the last query of a sequence sees its last key. Rows of y outside
     the sequences are left as they were; a query that sees no key gets zeros.
     workspace: a CUDA tensor of at least attention_packed_workspace bytes (few
-    queries over many keys need one), allocated here (on the current stream)
-    when None."""
+    queries over many keys need one), allocated here (on `stream`) when None."""
     ops, dt, index = _heads((q, k, v, y), ("q", "k", "v", "y"))
     rows, heads, d = q.shape
     keys, kv, _ = k.shape
@@ -301,11 +300,13 @@ def _workspace(given, size_of, shape, q, index, stream):
     need = size_of(*shape)
     if need <= 0:
         return None, 0
-    ws = _torch.empty(need, dtype=_torch.uint8, device=q.device)
-    if stream is not None:
-        # the memory returns to the pool on the current stream: not before `stream` is done
-        ws.record_stream(_torch.external_stream(int(stream), device=q.device))
-    return ws, need
+    if stream is None or int(stream) == _torch.raw_stream(index):
+        return _torch.empty(need, dtype=_torch.uint8, device=q.device), need
+    # from the stream's own pool: what the memory held before, and holds next, is in its order
+    s = _torch.external_stream(int(stream), device=q.device) if int(stream) else \
+        _torch.default_stream(q.device)
+    with _torch.stream(s):
+        return _torch.empty(need, dtype=_torch.uint8, device=q.device), need
 
 
 def attention_prefix_workspace(q, prefix_k, k_pages, pages=None) -> int:
@@ -327,8 +328,7 @@ def attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale: fl
     k_pages, v_pages [pages, page size, kv_heads, d]; pages int32 [batch,
     pages a request may have] names them in order, or None: page b is request
     b's. lens int32 [batch]. workspace: a CUDA tensor of at least
-    attention_prefix_workspace bytes, allocated here (on the current stream)
-    when None."""
+    attention_prefix_workspace bytes, allocated here (on `stream`) when None."""
     batch, steps, heads, d = q.shape
     kv = prefix_k.shape[1]
     count, page = k_pages.shape[:2]

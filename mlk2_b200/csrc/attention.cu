@@ -44,7 +44,7 @@
 // tile may see (the causal edge) cannot be zeroed: a row whose result has a
 // NaN is computed again key by key from its own keys (slowRow).
 //
-// Every mbarrier wait is bounded (2 s); on a timeout the CTA raises the device
+// Every mbarrier wait is bounded; on a timeout the CTA raises the device
 // status word, drains its copies, frees TMEM and returns.
 #include <cudaTypedefs.h>
 
@@ -67,12 +67,14 @@ constexpr int kItems = 2;    // item ring: the one in work and the next
 constexpr int kThreads = 12 * 32;
 constexpr int kMma = 8, kTma = 9, kSched = 10;  // warps; 0 to 7 are softmax warps, 11 is idle
 constexpr int kConsumers = 10;                  // warps that read an item
-constexpr uint64_t kLimitNs = 2000000000ull;
+constexpr uint64_t kLimitNs = 2000000000ull;  // of a wait, and its share for each key an item may have:
+constexpr uint64_t kKeyNs = 16000, kMostNs = 60000000000ull;  // 32 rows done again take up to 7 us a key
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
 constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe
 constexpr int kMaxSlots = 128;    // partial results a row may have: 16 x 4 of the prefix, as many of its own keys
 constexpr int kOwnItems = 2;      // items of own keys an SM should get, and their most key tiles
 constexpr int kOwnTiles = 32;
+constexpr int64_t kMaxHeadTotal = int64_t(1) << 40;  // rows x heads of a call, so that workspace bytes fit 64 bits
 
 // What one pass through the pipeline computes. Keys are counted from the
 // item's first; row limits (how many keys token i of a stream sees) are
@@ -105,6 +107,7 @@ struct KeySource {
 struct Params {
     int32_t heads, kv_heads, group, d, tt;  // tt: tokens of a query tile
     float c2, grow;                         // scale * log2 e; kRescale / c2
+    uint64_t limit;                         // of a wait, ns
     int* status;
     const void* q;
     int64_t q_row, q_head;
@@ -182,6 +185,7 @@ __device__ __forceinline__ void splitTiles(Item& it, int keys) {
 struct Walker {
     int level, base;     // cost level; first sequence of the current group
     int chunk;           // packed: most key tiles of an item, 0: any
+    int top;             // packed: the first level
     int64_t before;      // items before (level, group)
 };
 
@@ -217,6 +221,11 @@ __device__ __forceinline__ int pairsFrom(const Params& p, const Seq& s, int c) {
 }
 
 __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, int lane) {
+    if (idx < w.before) {  // numbers usually rise
+        w.level = w.top;
+        w.base = 0;
+        w.before = 0;
+    }
     for (;;) {
         const Seq s = loadSeq(p, w.base + lane);
         const int ge = pairsFrom(p, s, w.level), gt = pairsFrom(p, s, w.level + 1);
@@ -413,35 +422,43 @@ __device__ bool nextPrefix(const Params& p, OwnKeys& own, Walker& w, int64_t idx
     }
 }
 
-// ---- one row, key by key ----------------------------------------------------------------
+// ---- one row from its definition ----------------------------------------------------------
 __device__ __forceinline__ int pageRow(const Params& p, const Item& it, int key) {
     const int at = it.key0 + key;
     const int pg = p.pages[it.page_row + (at >> p.page_shift)];
-    // an index outside the pages reads rows past the map's end, which load as zeros
+    // -1 for an index outside the pages: its keys and values are zeros
     return (pg < 0 || pg >= p.n_pages) ? -1 : (pg << p.page_shift) + (at & (p.page - 1));
 }
 
 // Row `row` of the query tile from the definition, over the item's keys that
-// the row sees (of a spread item, those of `part`): o (normalised) and the log2
-// of its sum.
-template <int D, typename T>
+// the row sees (of a spread item, those of `part`), by a warp: a lane scores
+// one of 32 keys and then owns four columns of the result. o: those columns
+// (normalised); returns the log2 of the row's sum. All lanes have one row.
+template <typename T>
 __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, int row, int part,
-                                      float* o) {
+                                      float (&o)[4]) {
+    const int lane = threadIdx.x & 31;
     const int token = row / p.group, head = it.kvh * p.group + row % p.group;
     const T* q = static_cast<const T*>(p.q) + (it.q_row[st] + token) * p.q_row + head * p.q_head;
     const KeySource& src = p.src[it.src];
+    const T* kbase = static_cast<const T*>(src.k) + it.kvh * src.k_head;
+    const T* vbase = static_cast<const T*>(src.v) + it.kvh * src.v_head + 4 * lane;
+    const bool column = 4 * lane < p.d;
     const int lim = rowLimit(it, st, token);
     float m = -INFINITY, l = 0.0f;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int c = 0; c < D; ++c) o[c] = 0.0f;
-        for (int key = 0; key < lim; ++key) {
-            if (it.spread && (key >> 5 & 3) != part) continue;
-            int64_t krow = it.k_row + static_cast<int64_t>(key);
-            if (it.src == 1 && p.pages != nullptr) krow = pageRow(p, it, key);
-            const T* k = static_cast<const T*>(src.k) + krow * src.k_row + it.kvh * src.k_head;
-            const T* v = static_cast<const T*>(src.v) + krow * src.v_row + it.kvh * src.v_head;
-            float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = 0.0f;
+    for (int first = 0; first < lim; first += 32) {
+        if (it.spread && (first >> 5 & 3) != part) continue;
+        const int key = first + lane;
+        int64_t krow = -1;
+        float s = -INFINITY;
+        if (key < lim) {
+            krow = it.src == 1 && p.pages != nullptr ? pageRow(p, it, key)
+                                                     : it.k_row + static_cast<int64_t>(key);
+            s = 0.0f;
             if (krow >= 0) {
+                const T* k = kbase + krow * src.k_row;
                 for (int c = 0; c < p.d; c += 8) {
                     float a[8], b[8];
                     unpack8<T>(*reinterpret_cast<const uint4*>(q + c), a);
@@ -450,26 +467,44 @@ __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, i
                     for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
                 }
             }
-            if (pass == 0) {
-                m = (s > m || s != s) ? s : m;  // a NaN score stays
-                if (m != m) break;
-                continue;
-            }
-            const float e = tc::ex2((s - m) * p.c2);
-            l += e;
-            if (krow >= 0) {
-                for (int c = 0; c < p.d; c += 8) {
-                    float b[8];
-                    unpack8<T>(*reinterpret_cast<const uint4*>(v + c), b);
+        }
+        float top = s;
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        if (__any_sync(0xffffffffu, s != s)) top = NAN;
+        if (top == -INFINITY) continue;
+        top = m > top ? m : top;  // a NaN score stays
+        const float f = m == -INFINITY ? 0.0f : tc::ex2((m - top) * p.c2);
+        m = top;
+        const float e = key < lim ? tc::ex2((s - m) * p.c2) : 0.0f;
+        float sum = e;
+        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        l = fmaf(l, f, sum);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) o[c + i] = fmaf(e, b[i], o[c + i]);
-                }
+        for (int i = 0; i < 4; ++i) o[i] *= f;
+        for (int j = 0; j < 32; j += 8) {  // eight loads at a time
+            uint2 u[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const int64_t r = __shfl_sync(0xffffffffu, krow, j + x);
+                u[x] = make_uint2(0, 0);
+                if (r >= 0 && column) u[x] = *reinterpret_cast<const uint2*>(vbase + r * src.v_row);
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const float w = __shfl_sync(0xffffffffu, e, j + x);
+                const float2 a = unpack2<T>(u[x].x), b = unpack2<T>(u[x].y);
+                o[0] = fmaf(w, a.x, o[0]);
+                o[1] = fmaf(w, a.y, o[1]);
+                o[2] = fmaf(w, b.x, o[2]);
+                o[3] = fmaf(w, b.y, o[3]);
             }
         }
-        if (m == -INFINITY) return -INFINITY;  // nothing to see: zeros
+        if (m != m) break;
     }
+    if (m == -INFINITY) return -INFINITY;  // nothing to see: zeros
     const float inv = 1.0f / l;
-    for (int c = 0; c < D; ++c) o[c] *= inv;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= inv;
     return fmaf(m, p.c2, log2f(l));
 }
 
@@ -563,7 +598,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
     // aborted. It stays in the ring until drop(i).
     auto take = [&](uint32_t i) -> const Item* {
         const Item& it = sm.item[i % kItems];
-        if (!tc::mbar_wait(&sm.ifull[i % kItems], (i / kItems) & 1u, abort, kLimitNs)) return nullptr;
+        if (!tc::mbar_wait(&sm.ifull[i % kItems], (i / kItems) & 1u, abort, p.limit)) return nullptr;
         return it.live != 0 ? &it : nullptr;
     };
     auto drop = [&](uint32_t i) {
@@ -585,7 +620,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 tiles += static_cast<int64_t>(ceilDiv(q.nq, 2 * p.tt)) * ceilDiv(middle, kTile);
             }
             most = __reduce_max_sync(0xffffffffu, most);
-            w.level = ceilDiv(most, kTile);
+            w.level = w.top = ceilDiv(most, kTile);
             if (kPartial) {
                 // About kOwnItems items for each SM, of 4 tiles at least, in the slots there are.
 #pragma unroll
@@ -599,7 +634,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         for (uint32_t n = 0, asked = 0;;) {
             Item& slot = sm.item[n % kItems];
             if (n >= kItems &&
-                !tc::mbar_wait(&sm.iempty[n % kItems], ((n / kItems) - 1) & 1u, abort, kLimitNs)) {
+                !tc::mbar_wait(&sm.iempty[n % kItems], ((n / kItems) - 1) & 1u, abort, p.limit)) {
                 break;
             }
             bool live = false;
@@ -617,7 +652,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 if (!live) break;
                 // The next number is asked for towards the end of this item's loads:
                 // earlier would take work that another block is free for.
-                if (!tc::mbar_wait(&sm.cnext, n++ & 1u, abort, kLimitNs)) break;
+                if (!tc::mbar_wait(&sm.cnext, n++ & 1u, abort, p.limit)) break;
                 if (kPrefix && at >= p.pre_items) {  // every `tickets`-th item of the requests
                     at += p.tickets;
                     continue;
@@ -638,7 +673,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         Item it = {};  // a copy
         bool ok = true;
         auto load_q = [&](int st) -> bool {
-            if (qn[st] > 0 && !tc::mbar_wait(&sm.qempty[st], (qn[st] - 1) & 1u, abort, kLimitNs)) {
+            if (qn[st] > 0 && !tc::mbar_wait(&sm.qempty[st], (qn[st] - 1) & 1u, abort, p.limit)) {
                 return false;
             }
             ++qn[st];
@@ -650,11 +685,11 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                                         &sm.qfull[st], (h >> 2) * 64, it.kvh * p.group, it.q_row[0]);
                     }
                 } else {
-                tc::mbar_arrive_expect_tx(&sm.qfull[st], Sm::kHalves * 128u * p.group * p.tt);
-                for (int h = 0; h < Sm::kHalves; ++h) {
-                    tc::tma_load_3d(sm.q[st] + h * Sm::kBox, &map_q, &sm.qfull[st], h * 64,
-                                    it.kvh * p.group, st == 0 ? it.q_row[0] : it.q_row[1]);
-                }
+                    tc::mbar_arrive_expect_tx(&sm.qfull[st], Sm::kHalves * 128u * p.group * p.tt);
+                    for (int h = 0; h < Sm::kHalves; ++h) {
+                        tc::tma_load_3d(sm.q[st] + h * Sm::kBox, &map_q, &sm.qfull[st], h * 64,
+                                        it.kvh * p.group, st == 0 ? it.q_row[0] : it.q_row[1]);
+                    }
                 }
             }
             __syncwarp();
@@ -662,7 +697,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         };
         auto load_kv = [&](const CUtensorMap* map, int tile) -> bool {
             const uint32_t st = ring % kStages;
-            if (!tc::mbar_wait(&sm.empty[st], ((ring / kStages) & 1u) ^ 1u, abort, kLimitNs)) {
+            if (!tc::mbar_wait(&sm.empty[st], ((ring / kStages) & 1u) ^ 1u, abort, p.limit)) {
                 return false;
             }
             ++ring;
@@ -679,7 +714,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 if (lane < boxes) {
                     int row = pageRow(p, it, tile * kTile + lane * box);
                     if (row < 0) {
-                        row = p.n_pages << p.page_shift;
+                        row = kMaxHeadRows;
                         if (p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
                     }
                     for (int h = 0; h < Sm::kHalves; ++h) {
@@ -750,7 +785,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             }
         };
         auto wait = [&](const Place& x) {
-            return tc::mbar_wait(&sm.full[x.stage], x.parity, abort, kLimitNs);
+            return tc::mbar_wait(&sm.full[x.stage], x.parity, abort, p.limit);
         };
         auto loaded = [&](const Place& x) { return tc::mbar_test(&sm.full[x.stage], x.parity); };
         // S[st] = Q[slot] K^T, by one thread.
@@ -785,7 +820,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 v[st].move(1);
                 if (!ok || n[st] == 0) continue;
                 const uint32_t slot = paired ? st : 0;
-                if (paired || st == 0) ok = tc::mbar_wait(&sm.qfull[slot], qphase[slot], abort, kLimitNs);
+                if (paired || st == 0) ok = tc::mbar_wait(&sm.qfull[slot], qphase[slot], abort, p.limit);
                 ok = ok && wait(k[st]);
                 tc::tc_fence_after();
                 // In a pair the second stream, where it reads a tile, is the tile's
@@ -810,7 +845,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     if (st == 0 && !known[0]) ok = wait(vp) && wait(kp);
-                    ok = ok && tc::mbar_wait(&sm.pfull[st], pphase[st], abort, kLimitNs);
+                    ok = ok && tc::mbar_wait(&sm.pfull[st], pphase[st], abort, p.limit);
                     pphase[st] ^= 1u;
                     if (!ok) break;
                     if (st == 1) {  // look ahead: the answer comes while the products are issued
@@ -857,7 +892,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                         tc::fence_proxy_async();
                         __syncwarp();
                     }
-                    ok = ok && tc::mbar_wait(&sm.pfull[st], pphase[st], abort, kLimitNs);
+                    ok = ok && tc::mbar_wait(&sm.pfull[st], pphase[st], abort, p.limit);
                     pphase[st] ^= 1u;
                     if (!ok) continue;
                     const bool k_known = known[st];
@@ -910,7 +945,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         auto meet = [&]() -> bool {
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&sm.xbar[quarter]);
-            return tc::mbar_wait(&sm.xbar[quarter], xn++ & 1u, abort, kLimitNs);
+            return tc::mbar_wait(&sm.xbar[quarter], xn++ & 1u, abort, p.limit);
         };
         bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
@@ -947,7 +982,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
             };
             for (int jj = 0; jj < n; ++jj, ++sn, left -= stride) {
-                if (!tc::mbar_wait(&sm.sfull[st], sn & 1u, abort, kLimitNs)) {
+                if (!tc::mbar_wait(&sm.sfull[st], sn & 1u, abort, p.limit)) {
                     ok = false;
                     break;
                 }
@@ -1081,14 +1116,14 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             // A pair's streams have rows of their own. Otherwise both have seen
             // half of the same rows' keys: each joins the two results for half
             // of the columns.
-            if (n > 0 && !tc::mbar_wait(&sm.ofull[st], o_own & 1u, abort, kLimitNs)) break;
+            if (n > 0 && !tc::mbar_wait(&sm.ofull[st], o_own & 1u, abort, p.limit)) break;
             float f0 = 1.0f, f1 = 0.0f;  // shares of this stream's and the other's accumulator
             int from = 0, to = D;
             if (!it.paired) {
                 sm.xch[st][quarter * 32 + lane] = make_float2(m, l);
                 if (!meet()) break;
                 const float2 o = sm.xch[st ^ 1][quarter * 32 + lane];
-                if (theirs > 0 && !tc::mbar_wait(&sm.ofull[st ^ 1], o_other & 1u, abort, kLimitNs)) break;
+                if (theirs > 0 && !tc::mbar_wait(&sm.ofull[st ^ 1], o_other & 1u, abort, p.limit)) break;
                 const float both = fmaxf(m, o.x);
                 f0 = l == 0.0f ? 0.0f : tc::ex2((m - both) * p.c2);
                 f1 = o.y == 0.0f ? 0.0f : tc::ex2((o.x - both) * p.c2);
@@ -1156,80 +1191,94 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     }
                 }
             } else {
-            Out* rows[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int src = (lane & ~3) + r;
-                const int64_t addr = __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(out), src);
-                rows[r] = __shfl_sync(0xffffffffu, static_cast<int>(store), src) != 0
-                    ? reinterpret_cast<Out*>(addr) + (lane & 3) * kVec
-                    : nullptr;
-            }
-#pragma unroll 1
-            for (int x = from; x < end; x += kPass) {
-                uint4 v[4] = {};
-#pragma unroll
-                for (int g = 0; g < kPass / 16; ++g) {
-                    if (x + g * 16 >= end) break;  // columns there are not computed
-                    uint32_t o[16];
-                    uint64_t f[8] = {};
-                    if (n > 0) {
-                        tc::tmem_ld16(o_addr + st * kTile + x + g * 16, o);
-                        tc::tmem_ld_wait(o);
-#pragma unroll
-                        for (int y = 0; y < 8; ++y) {
-                            f[y] = tc::fma2(tc::pair(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])),
-                                            f02, 0);
-                        }
-                    }
-                    if (!it.paired && theirs > 0) {
-                        tc::tmem_ld16(o_addr + (st ^ 1) * kTile + x + g * 16, o);
-                        tc::tmem_ld_wait(o);
-#pragma unroll
-                        for (int y = 0; y < 8; ++y) {
-                            f[y] = tc::fma2(tc::pair(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])),
-                                            f12, f[y]);
-                        }
-                    }
-                    uint32_t w[16];
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        bad2 = tc::fma2(f[y], 0, bad2);
-                        const float2 z = tc::unpair(f[y]);
-                        if constexpr (kPartial) {
-                            w[2 * y] = __float_as_uint(z.x);
-                            w[2 * y + 1] = __float_as_uint(z.y);
-                        } else {
-                            w[y] = pack2<T>(z.x, z.y);
-                        }
-                    }
-#pragma unroll
-                    for (int y = 0; y < (kPartial ? 4 : 2); ++y) {
-                        v[(kPartial ? 0 : 2 * g) + y] = make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
-                    }
-                }
-                transpose4(v, lane);
+                Out* rows[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (rows[r] != nullptr && x + (lane & 3) * kVec < end) {
-                        *reinterpret_cast<uint4*>(rows[r] + x) = v[r];
+                    const int src = (lane & ~3) + r;
+                    const int64_t addr = __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(out), src);
+                    rows[r] = __shfl_sync(0xffffffffu, static_cast<int>(store), src) != 0
+                        ? reinterpret_cast<Out*>(addr) + (lane & 3) * kVec
+                        : nullptr;
+                }
+#pragma unroll 1
+                for (int x = from; x < end; x += kPass) {
+                    uint4 v[4] = {};
+#pragma unroll
+                    for (int g = 0; g < kPass / 16; ++g) {
+                        if (x + g * 16 >= end) break;  // columns there are not computed
+                        uint32_t o[16];
+                        uint64_t f[8] = {};
+                        if (n > 0) {
+                            tc::tmem_ld16(o_addr + st * kTile + x + g * 16, o);
+                            tc::tmem_ld_wait(o);
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) {
+                                f[y] = tc::fma2(tc::pair(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])),
+                                                f02, 0);
+                            }
+                        }
+                        if (!it.paired && theirs > 0) {
+                            tc::tmem_ld16(o_addr + (st ^ 1) * kTile + x + g * 16, o);
+                            tc::tmem_ld_wait(o);
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) {
+                                f[y] = tc::fma2(tc::pair(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])),
+                                                f12, f[y]);
+                            }
+                        }
+                        uint32_t w[16];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            bad2 = tc::fma2(f[y], 0, bad2);
+                            const float2 z = tc::unpair(f[y]);
+                            if constexpr (kPartial) {
+                                w[2 * y] = __float_as_uint(z.x);
+                                w[2 * y + 1] = __float_as_uint(z.y);
+                            } else {
+                                w[y] = pack2<T>(z.x, z.y);
+                            }
+                        }
+#pragma unroll
+                        for (int y = 0; y < (kPartial ? 4 : 2); ++y) {
+                            v[(kPartial ? 0 : 2 * g) + y] = make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
+                        }
+                    }
+                    transpose4(v, lane);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (rows[r] != nullptr && x + (lane & 3) * kVec < end) {
+                            *reinterpret_cast<uint4*>(rows[r] + x) = v[r];
+                        }
                     }
                 }
-            }
             }
             float lse = l > 0.0f ? fmaf(m, p.c2, log2f(l)) : -INFINITY;
             // A NaN somewhere, also seen as a sum no row can have (ex2_poly), or an infinity.
             const float2 bad = tc::unpair(bad2);
             const bool again = mine && l != 0.0f && (!(l < 0x1p60f) || bad.x != 0.0f || bad.y != 0.0f);
             const bool zeros = !kPartial && mine && l == 0.0f;
-            if (__any_sync(0xffffffffu, again || zeros)) {  // (ordered after the other lanes' stores)
-                float o[D];
-                if (again) {
-                    lse = slowRow<D, T>(p, it, st, row, quarter, o);
-                } else {
-                    for (int x = from; x < end; ++x) o[x] = 0.0f;
+            const unsigned todo = __ballot_sync(0xffffffffu, again || zeros);
+            if (todo != 0) {
+                __syncwarp();  // after the other lanes' stores
+                const unsigned slow = __ballot_sync(0xffffffffu, again);
+                for (unsigned left_rows = todo; left_rows != 0; left_rows &= left_rows - 1) {
+                    const int src = __ffs(left_rows) - 1;
+                    Out* to_row = reinterpret_cast<Out*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(out), src));
+                    float o[4] = {};
+                    if (slow >> src & 1u) {
+                        const float z = slowRow<T>(p, it, st, __shfl_sync(0xffffffffu, row, src), quarter, o);
+                        if (lane == src) lse = z;
+                    }
+                    if (4 * lane >= from && 4 * lane < end) {
+                        if constexpr (kPartial) {
+                            *reinterpret_cast<float4*>(to_row + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
+                        } else {
+                            *reinterpret_cast<uint2*>(to_row + 4 * lane) =
+                                make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
+                        }
+                    }
                 }
-                for (int x = from; x < end && (again || zeros); ++x) out[x] = static_cast<Out>(o[x]);
             }
             if (kPartial && mine && from == 0) {
                 float* out_lse = p.lse + (tok_row * p.heads + head) * p.slots;
@@ -1443,7 +1492,7 @@ int checkShape(int64_t heads, int64_t kv_heads, int64_t d, double scale, int32_t
     return MLKB_OK;
 }
 
-void setShape(Params& p, int64_t heads, int64_t kv_heads, int64_t d, double scale) {
+void setShape(Params& p, int64_t heads, int64_t kv_heads, int64_t d, double scale, int64_t keys) {
     p.heads = static_cast<int32_t>(heads);
     p.kv_heads = static_cast<int32_t>(kv_heads);
     p.group = static_cast<int32_t>(heads / kv_heads);
@@ -1451,6 +1500,8 @@ void setShape(Params& p, int64_t heads, int64_t kv_heads, int64_t d, double scal
     p.tt = kTile / p.group;
     p.c2 = static_cast<float>(scale * 1.4426950408889634);
     p.grow = kRescale / p.c2;
+    p.limit = kLimitNs + kKeyNs * static_cast<uint64_t>(keys);
+    if (p.limit > kMostNs) p.limit = kMostNs;
     p.status = deviceStatusPtr();
 }
 
@@ -1553,6 +1604,7 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
     if (int st = checkHeads(k, kv_heads, d, false, "attention k", &hk)) return st;
     if (int st = checkHeads(v, kv_heads, d, false, "attention v", &hv)) return st;
     if (int st = checkHeads(y, heads, d, true, "attention y", &hy)) return st;
+    if (hq.rows * heads > kMaxHeadTotal) return setError(MLKB_ERR_INVALID, "attention: too many rows");
     if (hk.rows != hv.rows || hq.rows != hy.rows) {
         return setError(MLKB_ERR_INVALID, "attention: k and v, and q and y, must have equal rows");
     }
@@ -1564,9 +1616,12 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
         ((reinterpret_cast<uintptr_t>(q_starts) | reinterpret_cast<uintptr_t>(k_starts)) & 3u) != 0) {
         return setError(MLKB_ERR_INVALID, "attention: q_starts and k_starts needed");
     }
+    if (hy.data == hq.data || (hk.rows > 0 && (hy.data == hk.data || hy.data == hv.data))) {
+        return setError(MLKB_ERR_INVALID, "attention: y may not overlap the inputs");
+    }
     if (int st = needDevice()) return st;
     Params p = {};
-    setShape(p, heads, kv_heads, d, scale);
+    setShape(p, heads, kv_heads, d, scale, hk.rows);
     p.q = hq.data;
     p.q_row = hq.row_stride;
     p.q_head = hq.head_stride;
@@ -1618,7 +1673,7 @@ extern "C" int64_t mlkb_attention_packed_workspace(int64_t rows, int64_t key_row
     using namespace mlkb;
     if (rows < 0 || key_rows < 0 || n_seqs < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
         heads / kv_heads > kTile || d < 8 || d > 128 || rows > kMaxHeadRows ||
-        key_rows > kMaxHeadRows || n_seqs > kMaxHeadRows || heads > (1 << 23)) {
+        key_rows > kMaxHeadRows || n_seqs > kMaxHeadRows || heads > (1 << 23) || rows * heads > kMaxHeadTotal) {
         return -1;
     }
     return planPacked(rows, key_rows, n_seqs, heads, kv_heads, d).bytes(d);
@@ -1631,7 +1686,8 @@ extern "C" int64_t mlkb_attention_prefix_workspace(int64_t batch, int64_t steps,
     if (batch < 0 || steps < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
         heads / kv_heads > kTile || d < 8 || d > 128 || prefix_rows < 0 || page_size < 0 ||
         pages_per_request < 0 || batch > kMaxHeadRows || steps > kMaxHeadRows || heads > (1 << 23) ||
-        prefix_rows > kMaxHeadRows || page_size > kMaxHeadRows || pages_per_request > kMaxHeadRows) {
+        prefix_rows > kMaxHeadRows || page_size > kMaxHeadRows || pages_per_request > kMaxHeadRows ||
+        batch * steps > kMaxHeadRows || batch * steps * heads > kMaxHeadTotal) {
         return -1;
     }
     const PrefixPlan r =
@@ -1660,6 +1716,7 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
         hq.rows != batch * steps || hy.rows != hq.rows) {
         return setError(MLKB_ERR_INVALID, "attention: q and y must have batch * steps rows");
     }
+    if (hq.rows * heads > kMaxHeadTotal) return setError(MLKB_ERR_INVALID, "attention: too many rows");
     if (hpk.rows != hpv.rows || hk.rows != hv.rows) {
         return setError(MLKB_ERR_INVALID, "attention: k and v must have equal rows");
     }
@@ -1697,9 +1754,10 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
                         "attention: workspace (16-byte aligned) smaller than "
                         "mlkb_attention_prefix_workspace says");
     }
+    if (hy.data == hq.data) return setError(MLKB_ERR_INVALID, "attention: y may not overlap the inputs");
     if (int st = needDevice()) return st;
     Params p = {};
-    setShape(p, heads, kv_heads, d, scale);
+    setShape(p, heads, kv_heads, d, scale, hpk.rows > cap ? hpk.rows : cap);
     p.q = hq.data;
     p.q_row = hq.row_stride;
     p.q_head = hq.head_stride;

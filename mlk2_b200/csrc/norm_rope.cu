@@ -207,19 +207,28 @@ norm_rope_kernel(const __grid_constant__ RopeParams p) {
             const float2 sa = tc::unpair(tc::add2(s2[0], s2[1]));
             const float ss = sum(mine ? sa.x + sa.y : 0.0f);
             float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
-            if (__any_sync(0xffffffffu, ss > 3.0e38f)) {
-                // The squares left the f32 range (bf16 values past 2^63): once more
-                // on values scaled by 2^-70, exact in f32. (eps has no weight there.)
+            const bool large = ss > 3.0e38f, small = ss < 0x1p-80f && p.eps < 0x1p-60f;
+            if (__any_sync(0xffffffffu, large || small)) {
+                // The squares left the f32 range (bf16 values past 2^63, or below 2^-63
+                // with an eps that does not hide them): once more on values scaled by
+                // 2^-70 or 2^70, exact in f32. (eps has no weight beside large ones.)
+                const float f = large ? 0x1p-70f : 0x1p70f;
                 float t = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 f = tc::unpair(a[i]), g = tc::unpair(b[i]);
-                    const float f0 = f.x * 0x1p-70f, f1 = f.y * 0x1p-70f;
-                    const float g0 = g.x * 0x1p-70f, g1 = g.y * 0x1p-70f;
-                    t += fmaf(f0, f0, f1 * f1) + fmaf(g0, g0, g1 * g1);
+                    const float2 u = tc::unpair(a[i]), v = tc::unpair(b[i]);
+                    const float u0 = u.x * f, u1 = u.y * f, v0 = v.x * f, v1 = v.y * f;
+                    t += fmaf(u0, u0, u1 * u1) + fmaf(v0, v0, v1 * v1);
                 }
                 t = sum(mine ? t : 0.0f);
-                if (ss > 3.0e38f) r = rsqrtf(t * p.inv_d) * 0x1p-70f;
+                if (large) r = rsqrtf(t * p.inv_d) * 0x1p-70f;
+                if (small) r = rsqrtf(fmaf(t, p.inv_d, p.eps * 0x1p70f * 0x1p70f));
+                const uint64_t keep = small ? tc::pair(f, f) : tc::pair(1.0f, 1.0f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    a[i] = mul2(a[i], keep);
+                    b[i] = mul2(b[i], keep);
+                }
             }
             const uint64_t r2 = tc::pair(r, r);
 #pragma unroll

@@ -76,8 +76,20 @@ int* deviceStatusPtr() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(mu);
     if (words[dev] == nullptr) {
+        // The first call may come while a stream of this thread is captured, where
+        // allocating is allowed in relaxed mode only, and a stream of its own
+        // keeps the clear out of the capture.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
         int* p = nullptr;
-        if (cudaMalloc(&p, 16) != cudaSuccess || cudaMemset(p, 0, 16) != cudaSuccess) {
+        cudaStream_t own = nullptr;
+        const bool ok = cudaMalloc(&p, 16) == cudaSuccess &&
+                        cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess &&
+                        cudaMemsetAsync(p, 0, 16, own) == cudaSuccess &&
+                        cudaStreamSynchronize(own) == cudaSuccess;
+        if (own != nullptr) cudaStreamDestroy(own);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!ok) {
             cudaGetLastError();
             return nullptr;
         }

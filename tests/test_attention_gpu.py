@@ -604,3 +604,188 @@ def test_captured_prompt(cuda):
         t = sum(n)
         check(y[:t], *packed(q[:t], k[:t], v[:t], n, n, 0.1))
         assert (y[t:] == 5).all()
+
+
+FIRST_CALLS = """
+import sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+from attention_util import check, norm_rope, packed, prefix, starts, table
+from mlk2_b200 import api
+g = torch.Generator(device="cuda").manual_seed(1)
+q, k, v = (torch.randn(40, h, 64, generator=g, device="cuda").half() for h in (4, 2, 2))
+t, pos = table(64, 64, "cuda"), torch.arange(40, device="cuda", dtype=torch.int32)
+s, lens = starts([30, 10], "cuda"), torch.full((5,), 8, device="cuda", dtype=torch.int32)
+qo, ko, y, z = (torch.zeros_like(x) for x in (q, k, q, q))
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    api.norm_rope(q, k, qo, ko, t, pos)
+    api.attention_packed(qo, ko, v, y, s, s, 0.125)
+    api.attention_prefix(qo.view(5, 8, 4, 64), ko, v, ko.view(5, 8, 2, 64), v.view(5, 8, 2, 64),
+                         z.view(5, 8, 4, 64), lens, 0.125)
+graph.replay()
+torch.cuda.synchronize()
+check(qo, *norm_rope(q, None, 0, t, pos, None, False))
+check(y, *packed(qo, ko, v, [30, 10], [30, 10], 0.125))
+want, bound = prefix(qo.view(5, 8, 4, 64), ko, v, ko.view(5, 8, 2, 64), v.view(5, 8, 2, 64), [8] * 5, 0.125)
+check(z.view(5, 8, 4, 64), want, bound)
+assert api.take_device_error() == 0
+print("captured first calls ok")
+"""
+
+
+def test_first_calls_of_a_process_captured(cuda):
+    """Nothing that a first call sets up gets in the way of a capture."""
+    import os
+    import subprocess
+    import sys
+
+    tests = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=os.path.dirname(tests), tests=tests)],
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "captured first calls ok" in r.stdout, r.stdout + r.stderr
+
+
+def test_empty_operands(cuda):
+    q, k = torch.empty(0, 4, 64, device="cuda", dtype=F16), torch.empty(0, 2, 64, device="cuda", dtype=F16)
+    api.norm_rope(q, k, q, k, table(4, 64, "cuda"), torch.empty(0, device="cuda", dtype=torch.int32))
+    api.attention_packed(q, k, k, q, ints([0]), ints([0]), 0.1)
+    api.attention_packed(q, k, k, q, ints([0, 0]), ints([0, 0]), 0.1)
+    api.attention_prefix(q[:, None], k, k, k[:, None], k[:, None], q[:, None], ints([]), 0.1)
+    x = torch.full((3, 4, 64), 7, device="cuda", dtype=F16)
+    y = torch.full_like(x, 5)
+    api.attention_packed(x, k, k, y, ints([0, 2]), ints([0, 0]), 0.1)  # no keys at all
+    assert (y[:2] == 0).all() and (y[2] == 5).all()
+    api.attention_prefix(x[:, None], k, k, k[:, None], k[:, None], y[:, None], ints([0, 0, 0]), 0.1)
+    assert (y == 0).all() and api.take_device_error() == 0
+
+
+def test_prefix_pages_shared_between_requests(cuda):
+    """Requests may name the same page, and one request a page twice."""
+    q, pk, pv, kp, vp, lens, pages = make_prefix(3, 1, 40, [60, 64, 33], 4, 2, 64, 16, seed=7)
+    pages[1] = pages[0]
+    pages[2, 1] = pages[2, 0]
+    y = torch.empty_like(q)
+    api.attention_prefix(q, pk, pv, kp, vp, y, lens, 0.125, pages=pages)
+    check(y, *prefix(q, pk, pv, kp, vp, lens.tolist(), 0.125, pages))
+
+
+def test_prefix_batch_stride(cuda):
+    """q, y and the caches as views with a common stride over their first two dimensions."""
+    q, pk, pv, kp, vp, lens, _ = make_prefix(4, 3, 100, [50, 3, 200, 70], 8, 2, 64, 0, seed=8)
+    wide = normal(gen(9), 4, 3, 16, 64)
+    wide[:, :, 4:12] = q
+    out = torch.full((4, 3, 8, 128), 5, device="cuda", dtype=BF16)
+    y = out[..., :64]
+    api.attention_prefix(wide[:, :, 4:12], pk, pv, kp, vp, y, lens, 0.125)
+    check(y, *prefix(q, pk, pv, kp, vp, lens.tolist(), 0.125))
+    assert (out[..., 64:] == 5).all()
+    with pytest.raises(ValueError, match="common stride"):
+        api.attention_prefix(normal(gen(9), 4, 4, 8, 64)[:, :3], pk, pv, kp, vp, q, lens, 0.125)
+
+
+def test_wrappers_refuse(cuda):
+    q, k = torch.zeros(4, 8, 64, device="cuda", dtype=F16), torch.zeros(4, 2, 64, device="cuda", dtype=F16)
+    pos, t, s = ints([0, 1, 2, 3]), table(9, 64, "cuda"), ints([0, 4])
+    for call in (lambda: api.norm_rope(q, k, q[:3], k, t, pos), lambda: api.norm_rope(q, k, q, None, t, pos),
+                 lambda: api.norm_rope(q, k[:3], q, k[:3], t, pos), lambda: api.norm_rope(q, k, q, k, t, pos[:3]),
+                 lambda: api.norm_rope(q, k, q, k, t, pos.long()), lambda: api.norm_rope(q, k, q, k, t.half(), pos),
+                 lambda: api.norm_rope(q, k.bfloat16(), q, k, t, pos),
+                 lambda: api.norm_rope(q, k, q, k, t, pos, sections=[16, 16]),
+                 lambda: api.norm_rope(q, k, q, k, t, pos, q_weight=t[0], k_weight=t[0]),
+                 lambda: api.attention_packed(q, k, k[:3], q.clone(), s, s, 0.1),
+                 lambda: api.attention_packed(q, k, k, q[:, :4], s, s, 0.1),
+                 lambda: api.attention_packed(q, k, k, q.clone(), s, ints([0, 4, 4]), 0.1),
+                 lambda: api.attention_packed(q, k, k, q.clone(), ints([]), ints([]), 0.1),
+                 lambda: api.attention_packed(q.transpose(1, 2), k, k, q, s, s, 0.1),
+                 lambda: api.attention_prefix(q[:, None], k, k, k[:2, None], k[:2, None], q[:, None].clone(), pos, 0.1),
+                 lambda: api.attention_prefix(q[:, None], k, k, k[:, None], k[:, None], q[:, None].clone(), pos[:2], 0.1)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(mb.MLKBError):
+        api.attention_packed(q, k, k, q.clone(), s, s, -0.1)
+    with pytest.raises(mb.MLKBError):
+        api.norm_rope(q, k, q, k, t, pos, q_weight=t[0].half(), k_weight=None)
+    with pytest.raises(mb.MLKBError, match="overlap"):
+        api.attention_packed(q, k, k, q, s, s, 0.1)
+    with pytest.raises(mb.MLKBError, match="overlap"):
+        api.attention_prefix(q[:, None], k, k, k[:, None], k[:, None], q[:, None], pos, 0.1)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_norm_rope_without_eps(cuda, interleaved):
+    """eps 0: rows whose squares leave the f32 range downwards, to the smallest bf16 values."""
+    g = gen(21)
+    q = normal(g, 6, 3, 96)
+    for r, size in enumerate((1.0, 1e-18, 1e-25, 1e-37, 3e-39, 1e19)):
+        q[r] = (q[r].double() * size).to(BF16)
+    w, t = normal(g, 96), table(8, 64, "cuda")
+    pos = torch.arange(6, device="cuda", dtype=torch.int32)
+    y = torch.empty_like(q)
+    api.norm_rope(q, None, y, None, t, pos, q_weight=w, eps=0.0, interleaved=interleaved)
+    check(y, *norm_rope(q, w, 0.0, t, pos, None, interleaved))
+
+
+@pytest.mark.parametrize("d,dtype", [(64, BF16), (40, F16), (128, F16)])
+def test_packed_every_value_infinite_or_nan(cuda, d, dtype):
+    """Every row is computed again, and the columns stay apart."""
+    g = gen(22)
+    n = [300, 77]
+    q, k, v = normal(g, 377, 6, d, dtype=dtype), normal(g, 377, 2, d, dtype=dtype), normal(g, 377, 2, d, dtype=dtype)
+    v[:, 0, 3] = torch.inf
+    v[:, 1, d - 1] = torch.nan
+    y = torch.empty_like(q)
+    s = starts(n, "cuda")
+    api.attention_packed(q, k, v, y, s, s, 0.1)
+    assert y[:, :3, 3].isinf().all() and (y[:, :3, 3] > 0).all() and y[:, 3:, d - 1].isnan().all()
+    clean = v.clone()
+    clean[:, 0, 3] = clean[:, 1, d - 1] = 0
+    want, bound = packed(q, k, clean, n, n, 0.1)
+    y[:, :3, 3] = y[:, 3:, d - 1] = 0
+    check(y, want, bound)
+
+
+@pytest.mark.parametrize("heads,steps", [(4, 1), (16, 5)])
+def test_prefix_infinite_value(cuda, heads, steps):
+    """An infinity in the prefix and one of a request's own, in few (spread) rows and in many."""
+    q, pk, pv, kp, vp, lens, pages = make_prefix(5, steps, 500, [40, 300, 9, 170, 33], heads, 2, 64, 32, seed=9)
+    want, bound = prefix(q, pk, pv, kp, vp, lens.tolist(), 0.125, pages)
+    pv[77, 0, 9] = torch.inf
+    vp[pages[1, 2], 5, 1, 11] = -torch.inf
+    y = torch.empty_like(q)
+    api.attention_prefix(q, pk, pv, kp, vp, y, lens, 0.125, pages=pages)
+    group = heads // 2
+    assert (y[:, :, :group, 9] == torch.inf).all() and (y[1, :, group:, 11] == -torch.inf).all()
+    for z in (y, want):
+        z[:, :, :group, 9] = 0
+        z[1, :, group:, 11] = 0
+    check(y, want, bound)
+
+
+def test_prefix_table_without_pages(cuda):
+    """Page indices into an empty cache read as zeros."""
+    q, pk, pv, _, _, lens, pages = make_prefix(3, 1, 64, [40, 20, 48], 4, 2, 64, 16, seed=10)
+    none = torch.empty(0, 16, 2, 64, device="cuda", dtype=BF16)
+    zeros = torch.zeros(1, 16, 2, 64, device="cuda", dtype=BF16)
+    y = torch.empty_like(q)
+    for index in (0, 1, -1, 2 ** 31 - 1):
+        api.attention_prefix(q, pk, pv, none, none, y, lens, 0.125, pages=torch.full_like(pages, index))
+        assert api.take_device_error() == mb.ERR_INVALID
+        check(y, *prefix(q, pk, pv, zeros, zeros, lens.tolist(), 0.125, torch.zeros_like(pages)))
+
+
+def test_calls_at_once_given_streams(cuda):
+    """Streams by handle, the workspaces allocated by the calls."""
+    ins = [make_prefix(20, 1, 2000, [100] * 20, 8, 2, 64, 0, seed=s) for s in (1, 2, 3)]
+    streams = [torch.cuda.Stream() for _ in ins]
+    outs = [[torch.empty_like(i[0]) for _ in range(6)] for i in ins]
+    torch.cuda.synchronize()
+    for r in range(6):
+        for (q, pk, pv, kp, vp, lens, _), st, y in zip(ins, streams, outs):
+            api.attention_prefix(q, pk, pv, kp, vp, y[r], lens, 0.125,
+                                 stream=st.cuda_stream if r % 3 else torch.cuda.default_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for (q, pk, pv, kp, vp, lens, _), y in zip(ins, outs):
+        want, bound = prefix(q, pk, pv, kp, vp, lens.tolist(), 0.125)
+        for z in y:
+            check(z, want, bound)
