@@ -9,31 +9,40 @@
 // One CTA per SM at a time, one item per CTA of the grid; a running CTA takes
 // the items of CTAs that are not launched yet (cluster launch control), so
 // uneven items spread by themselves and a CTA's set-up is paid once. Two
-// streams of work per CTA, each with its own
-// 128-row query tile, score accumulator and softmax warps:
-//   warps 0-7    stream 0: softmax and epilogue. Two threads share a row, one
-//                for each half of a tile's 64 + 64 keys; they exchange the
-//                half maxima through shared memory (a row in one thread made
-//                the softmax twice as long a chain between two products)
-//   warps 8-15   stream 1: the same
-//   warp 16      MMA issuer
-//   warp 17      TMA producer (Q tiles; K and V tiles of 128 keys in a ring)
-//   warp 18      scheduler: writes the items into a ring for the other warps
-//   warp 19      idle (register shares move by groups of four warps)
+// streams of work per CTA, each with a 128-row query tile, score accumulator
+// and softmax warps of its own:
+//   warps 0-3    stream 0: softmax and epilogue, a row to a thread
+//   warps 4-7    stream 1: the same
+//   warp 8       MMA issuer
+//   warp 9       TMA producer (Q tiles; K and V tiles of 128 keys in a ring)
+//   warp 10      scheduler: writes the items into a ring for the other warps
+//   warp 11      idle (12 warps leave 168 registers to a thread)
 // TMEM: two score tiles (128 f32 columns each; the tile's probabilities
 // overwrite its first half as 16-bit pairs and are the A operand of P V) and
 // two output accumulators (128 columns each). For one stream the issuer
 // alternates P V of key tile j and Q K^T of tile j + 1; the streams interleave,
 // so one's softmax runs under the other's products. An item's streams are
 // either two query tiles over the same keys (`paired`) or one query tile over
-// alternate key tiles.
+// alternate key tiles, joined in the block.
+//
+// What bounds it (d 128, f16, a causal prompt of 8192 with 32 heads: 0.49 ms,
+// 1.12 PFLOP/s at the 1.6-1.75 GHz that the chip holds then; 65 % of the
+// measured matrix peak): a pair's step over 128 keys takes about 3800 cycles,
+// 2048 of them matrix work. A stream's own chain is longer than half of the
+// step: 1700-1900 cycles of softmax (768 of them the exponentials that stay on
+// the special-function unit), then its two products, 1024 cycles alone and
+// 1300 behind the other stream's, then the way through two barriers. TMEM is
+// full, so a third tile in flight would have to be smaller, which was slower:
+// 64-key score tiles, two of them to a stream (the products then read Q twice
+// as often); two threads to a row (more exchange than it saved); P handed on
+// in parts; a second issuing warp.
 //
 // Softmax: running row maximum m (of the raw scores) and sum in f32;
 // p = 2^(c s - c m), c = scale log2 e. The accumulator is rescaled only when a
 // row's maximum has grown by more than 2^8 since the last rescale: until then
 // p stays within 2^8 of 1, far inside the 16-bit formats' range, and the
 // factor cancels in the final division. The commit that makes Q K^T of tile
-// j + 1 visible also covers P V of tile j (same issuing thread), so a rescale
+// j + 1 visible also covers P V of tile j (one thread issues both), so a rescale
 // finds the accumulator at rest without another barrier.
 //
 // p is rounded to the inputs' 16-bit type for the product with V (the tensor
@@ -42,7 +51,9 @@
 // Keys past an item's end are masked in the scores and zeroed in V's tile (a
 // zero probability times a NaN would be NaN). Values that only some rows of a
 // tile may see (the causal edge) cannot be zeroed: a row whose result has a
-// NaN is computed again key by key from its own keys (slowRow).
+// NaN or an infinity is computed again from its own keys (slowRow), which costs
+// about 7 us a key and warp where all rows of a tile need it (a prompt of 8192
+// whose values are all NaN: 182 ms; one such value: 52 ms).
 //
 // Every mbarrier wait is bounded; on a timeout the CTA raises the device
 // status word, drains its copies, frees TMEM and returns.
@@ -70,10 +81,10 @@ constexpr int kConsumers = 10;                  // warps that read an item
 constexpr uint64_t kLimitNs = 2000000000ull;  // of a wait, and its share for each key an item may have:
 constexpr uint64_t kKeyNs = 16000, kMostNs = 60000000000ull;  // 32 rows done again take up to 7 us a key
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
-constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe
+constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe (0, 1, 3, 4: slower)
 constexpr int kMaxSlots = 128;    // partial results a row may have: 16 x 4 of the prefix, as many of its own keys
-constexpr int kOwnItems = 2;      // items of own keys an SM should get, and their most key tiles
-constexpr int kOwnTiles = 32;
+constexpr int kOwnItems = 2;      // items of own keys an SM should get (4: more epilogues than the even end gives)
+constexpr int kOwnTiles = 32;     // and their most key tiles (16 to 64: within 3 %)
 constexpr int64_t kMaxHeadTotal = int64_t(1) << 40;  // rows x heads of a call, so that workspace bytes fit 64 bits
 
 // What one pass through the pipeline computes. Keys are counted from the
@@ -288,9 +299,12 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
 }
 
 // ---- scheduling: a shared prefix ------------------------------------------------------
-// Items 0 .. pre_items-1: (key split, kv head, query tile or pair) over the
+// Items 0 .. pre_items-1: (query tile or pair, key split, kv head) over the
 // prefix, all tokens of the batch as rows; then the requests' own keys, cut
-// into chunks: (request and chunk, kv head, query tile).
+// into chunks: (request and chunk, kv head, query tile). Pairs come first and a
+// single tile last: side by side over the same keys, pairs took 4.2 us for a
+// key tile and singles 1.9, apart 2.3 and 1.5 (80 requests over 32768 keys: 165
+// us with the query tile counted fastest, 139 us so).
 struct OwnKeys {
     int keys;       // of a chunk; 0: not planned yet
     int64_t items;  // chunks of all requests x kv heads x query tiles
@@ -340,8 +354,9 @@ __device__ bool nextPrefix(const Params& p, OwnKeys& own, Walker& w, int64_t idx
                            int lane) {
     if (idx < p.pre_items) {
         if (lane == 0) {
-            const int mt = static_cast<int>(idx) % p.pre_mt;
-            const int r = static_cast<int>(idx) / p.pre_mt;
+            const int per_mt = p.pre_items / p.pre_mt;
+            const int mt = static_cast<int>(idx) / per_mt;
+            const int r = static_cast<int>(idx) % per_mt;
             const int split = r / p.kv_heads;
             const int first = split * p.pre_tiles * kTile;
             const int last = min(first + p.pre_tiles * kTile, p.prefix);
@@ -1303,7 +1318,10 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 }
 
 // ---- joining the partial results of attention_prefix ----------------------------------------
-// One warp per result row: y = sum_i 2^(lse_i - top) o_i / sum_i 2^(lse_i - top)
+// Bound by latency at the sizes there are (13 slots of 2560 rows: 17 MB out of
+// L2), so slots lie side by side and eight are loaded at a time (a slot's rows
+// side by side, one load at a time: 171 us instead of 153 for a whole call over
+// a prefix of 32768). One warp per result row: y = sum_i 2^(lse_i - top) o_i / sum_i 2^(lse_i - top)
 // over the row's slots; those that saw no key have lse = -inf and are not read.
 struct JoinParams {
     const float* part;
@@ -1525,7 +1543,7 @@ PackedPlan planPacked(int64_t rows, int64_t key_rows, int64_t seqs, int64_t head
     // Items for at most half the SMs, and sequences that may be long: keys are cut
     // into up to 8 chunks. With about an item to an SM joining costs more than it
     // gives (1030 queries of 5 sequences, 32 heads: 84 us cut, 66 us whole); one
-    // query over 16384 keys, 8 heads to a kv head, KCUT.
+    // query over 16384 keys, 8 heads to a kv head: 33 us cut, 131 us whole.
     const int64_t tiles = (key_rows + kTile - 1) / kTile;
     if (r.items > 0 && 2 * r.items <= sms && tiles > 8) {
         r.slots = (sms + r.items - 1) / r.items;
@@ -1580,7 +1598,8 @@ PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_he
     const int64_t items = batch * kv_heads * r.suf_mt * r.suf_slots;
     r.tickets = items < 8 * sms ? items : 8 * sms;
     // Few rows: spread over the tile's lanes. That divides the softmax, the
-    // longest link between two products, by four.
+    // longest link between two products, by four (128 requests of up to 4096
+    // own keys: 203 us, 5.4 TB/s, 83 % of the measured copy rate).
     r.spread_tt = 32 / (heads / kv_heads);
     r.pre_spread = r.spread_tt >= batch * steps;
     r.suf_spread = r.spread_tt >= steps;
