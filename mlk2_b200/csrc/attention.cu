@@ -1559,14 +1559,16 @@ PackedPlan planPacked(int64_t rows, int64_t key_rows, int64_t seqs, int64_t head
     r.items = (rows / pair + (seqs < rows ? seqs : rows)) * kv_heads;
     r.rows = rows * heads;
     // Items for at most half the SMs, and sequences that may be long: keys are cut
-    // into up to 8 chunks. With about an item to an SM joining costs more than it
-    // gives (1030 queries of 5 sequences, 32 heads: 84 us cut, 66 us whole); one
-    // query over 16384 keys, 8 heads to a kv head: 33 us cut, 131 us whole.
+    // into up to 64 chunks of 4 tiles at least, no more than one to an SM. With
+    // about an item to an SM joining costs more than it gives (1030 queries of 5
+    // sequences, 32 heads: 84 us cut, 63 us whole); one query over 16384 keys, 8
+    // heads to a kv head: 131 us whole, 30 us in 8 chunks, 25 us in 32; twice as
+    // many chunks, or chunks of 2 tiles, are no faster or slower there (28 us).
     const int64_t tiles = (key_rows + kTile - 1) / kTile;
     if (r.items > 0 && 2 * r.items <= sms && tiles > 8) {
-        r.slots = (sms + r.items - 1) / r.items;
+        r.slots = sms / r.items;
         if (r.slots > tiles / 4) r.slots = tiles / 4;
-        if (r.slots > 8) r.slots = 8;
+        if (r.slots > 64) r.slots = 64;
     }
     return r;
 }

@@ -183,7 +183,7 @@ def test_packed_long(cuda):
     ([1], [5000], 8, 1, 128, True), ([1, 1, 0, 3], [2000, 130, 700, 3], 4, 4, 64, True),
     ([40, 7], [1500, 2200], 16, 2, 80, True), ([40, 7], [1500, 2200], 16, 2, 80, False),
     ([100, 2], [60, 1700], 2, 1, 128, True), ([300], [1400], 4, 1, 96, True),
-    ([2, 2], [9000, 3], 3, 1, 72, True)])
+    ([2, 2], [9000, 3], 3, 1, 72, True), ([1], [33000], 4, 1, 64, True)])
 def test_packed_few_queries_over_many_keys(cuda, nq, nk, heads, kv, d, causal):
     """Cut along the keys and joined; without a workspace the same values uncut."""
     g = gen(18)
