@@ -434,14 +434,15 @@ int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* q
  *   q, y     [rows, heads, d]; k, v [key rows, kv_heads, d]; heads a multiple
  *            of kv_heads, at most 128 times it; d a multiple of 8, 8 to 128;
  *            f16 or bf16 (elem_dtype), y in the same type
- *   scale    positive
+ *   scale    positive; scores times scale stay within the f32 range
  * Scores, row maxima, sums and outputs are held in f32; the probabilities are
  * rounded to the element type before the product with v. A query that sees no
  * key (or only scores of -inf) gets zeros. Rows of y outside every sequence
  * are left as they were. Keys a query does not see have no effect on it,
  * whatever they or their values hold. A sequence whose starts fall or leave
  * the operands is skipped and raises MLKB_ERR_INVALID in the status word that
- * mlkb_take_device_error returns. y may not overlap the inputs.
+ * mlkb_take_device_error returns (rows that two others claim around it hold
+ * either's results). y may not overlap the inputs.
  *   workspace  few queries over many keys are cut along the keys and joined,
  *              with at least mlkb_attention_packed_workspace bytes of device
  *              memory (16-byte aligned); NULL or less: they are not cut. In use
