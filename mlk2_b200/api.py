@@ -7,6 +7,7 @@ are numpy arrays or CPU tensors.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Sequence
 
 import numpy as np
@@ -139,14 +140,15 @@ class _Torch:
         self.empty, self.device = torch.empty, torch.cuda.device
         self.external_stream, self.default_stream = torch.cuda.ExternalStream, torch.cuda.default_stream
         self.stream = torch.cuda.stream
-        self.current_device = torch.cuda.current_device
-        # the stream's handle without the object around it, where torch has it
+        self.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        # the device's index and the stream's handle without what is around them, where torch has that
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 _torch = None
-_HEADS = {n: C.c_int64 * (4 * n) for n in (4, 6)}  # mlkb_heads: data, rows, row and head stride
+_pack_heads = struct.Struct("4q").pack  # mlkb_heads: data, rows, row and head stride
+_NO_HEADS = _pack_heads(0, 0, 0, 0)
 
 
 def _bind():
@@ -158,8 +160,8 @@ def _bind():
 
 def _heads(tensors, names):
     """The operands ([rows, heads, d] each, [a, b, heads, d] taken as [a * b,
-    heads, d], or None) as consecutive mlkb_heads, their element type and the
-    index of their device."""
+    heads, d], or None) as mlkb_heads and their shapes, then their element type
+    and the index of their device."""
     first = tensors[0]
     dtype, index = first.dtype, first.get_device()
     code = _bind().dtypes.get(dtype)
@@ -167,25 +169,31 @@ def _heads(tensors, names):
         raise ValueError(f"{names[0]}: dtype must be float16 or bfloat16, got {dtype}")
     if index < 0:
         raise ValueError(f"{names[0]}: must be on a CUDA device, not {first.device}")
-    flat = []
-    for i, t in enumerate(tensors):
+    heads, shapes, pack = [], [], _pack_heads
+    for t in tensors:
         if t is None:
-            flat += (0, 0, 0, 0)
+            heads.append(_NO_HEADS)
+            shapes.append(None)
             continue
         if t.dtype is not dtype or t.get_device() != index:
-            raise ValueError(f"{names[i]}: {t.dtype} on {t.device}, but {names[0]} is {dtype} on "
+            raise ValueError(f"{names[len(heads)]}: {t.dtype} on {t.device}, but {names[0]} is {dtype} on "
                              f"{first.device}")
         shape, strides = t.shape, t.stride()
+        rows, row = shape[0], strides[0]
         if len(shape) == 4:
-            rows, row = shape[0] * shape[1], strides[1] if shape[1] > 1 else strides[0]
-            if shape[0] > 1 and strides[0] != shape[1] * row and shape[1] > 1:
-                raise ValueError(f"{names[i]}: its first two dimensions must have one common stride")
-        else:
-            rows, row = shape[0], strides[0]
+            if shape[1] > 1:
+                row = strides[1]
+                if rows > 1 and strides[0] != shape[1] * row:
+                    raise ValueError(f"{names[len(heads)]}: its first two dimensions must have one common "
+                                     "stride")
+            rows *= shape[1]
+        elif len(shape) != 3:
+            raise ValueError(f"{names[len(heads)]}: {len(shape)} dimensions, expected [rows, heads, d]")
         if strides[-1] != 1 and shape[-1] > 1:
-            raise ValueError(f"{names[i]}: the last dimension must be contiguous")
-        flat += (t.data_ptr(), rows, row, strides[-2])
-    return _HEADS[len(tensors)](*flat), code, index
+            raise ValueError(f"{names[len(heads)]}: the last dimension must be contiguous")
+        heads.append(pack(t.data_ptr(), rows, row, strides[-2]))
+        shapes.append(shape)
+    return heads, shapes, code, index
 
 
 def _int32(t, name, index, shape):
@@ -218,15 +226,15 @@ def norm_rope(q, k, q_out, k_out, table, positions, sections=None, q_weight=None
     positions: int32 [tokens], or [axes, tokens] with `sections`, the number
     of pairs each axis turns. A token whose position is outside the table is
     left as it is (take_device_error() then reports it)."""
-    ops, dt, index = _heads((q, k, q_out, k_out), ("q", "k", "q_out", "k_out"))
-    shape = q.shape
+    ops, shapes, dt, index = _heads((q, k, q_out, k_out), ("q", "k", "q_out", "k_out"))
+    shape, keys, shape_out, keys_out = shapes
     tokens, heads, d = shape
     kv = 0
-    if q_out.shape != shape or (k is None) != (k_out is None):
+    if shape_out != shape or (k is None) != (k_out is None):
         raise ValueError("q_out and k_out must have the shapes of q and k")
     if k is not None:
-        kv = k.shape[1]
-        if k.shape != (tokens, kv, d) or k_out.shape != k.shape:
+        kv = keys[1]
+        if keys != (tokens, kv, d) or keys_out != keys:
             raise ValueError("k and k_out must have the tokens and d of q")
     if table.dtype is not _torch.float32 or table.get_device() != index or not table.is_contiguous() \
             or table.dim() != 2:
@@ -245,10 +253,9 @@ def norm_rope(q, k, q_out, k_out, table, positions, sections=None, q_weight=None
                               or w.shape != (d,)):
             raise ValueError(f"{name}: contiguous [{d}] of {q.dtype} on the device of q needed")
         weights.append(None if w is None else w.data_ptr())
-    at = C.addressof(ops)
     _call(lib().mlkb_norm_rope,
-          (at, at + 32, at + 64, at + 96, heads, kv, d, rot, *weights, eps, table.data_ptr(),
-           table_rows, pos, tokens, sec, axes, int(interleaved), dt), index, stream)
+          (*ops, heads, kv, d, rot, *weights, eps, table.data_ptr(), table_rows, pos, tokens, sec, axes,
+           int(interleaved), dt), index, stream)
 
 
 def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool = True,
@@ -261,10 +268,10 @@ def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool 
     the sequences are left as they were; a query that sees no key gets zeros.
     workspace: a CUDA tensor of at least attention_packed_workspace bytes (few
     queries over many keys need one), allocated here (on `stream`) when None."""
-    ops, dt, index = _heads((q, k, v, y), ("q", "k", "v", "y"))
-    rows, heads, d = q.shape
-    keys, kv, _ = k.shape
-    if y.shape != q.shape or v.shape != k.shape or k.shape[2] != d:
+    ops, shapes, dt, index = _heads((q, k, v, y), ("q", "k", "v", "y"))
+    rows, heads, d = shapes[0]
+    keys, kv, d_keys = shapes[1]
+    if shapes[3] != shapes[0] or shapes[2] != shapes[1] or d_keys != d:
         raise ValueError("y must have the shape of q, v that of k, and all the same d")
     n = q_starts.shape[0]
     if n < 1:
@@ -274,9 +281,8 @@ def attention_packed(q, k, v, y, q_starts, k_starts, scale: float, causal: bool 
     L = lib()
     ws, size = _workspace(workspace, L.mlkb_attention_packed_workspace,
                           (rows, keys, n - 1, heads, kv, d), q, index, stream)
-    at = C.addressof(ops)
     _call(L.mlkb_attention_packed,
-          (at, at + 32, at + 64, at + 96, heads, kv, d, qs, ks, n - 1, int(causal), scale, dt,
+          (*ops, heads, kv, d, qs, ks, n - 1, int(causal), scale, dt,
            None if ws is None else ws.data_ptr(), size), index, stream)
 
 
@@ -329,11 +335,13 @@ def attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale: fl
     pages a request may have] names them in order, or None: page b is request
     b's. lens int32 [batch]. workspace: a CUDA tensor of at least
     attention_prefix_workspace bytes, allocated here (on `stream`) when None."""
-    batch, steps, heads, d = q.shape
-    kv = prefix_k.shape[1]
-    count, page = k_pages.shape[:2]
-    if y.shape != q.shape or prefix_v.shape != prefix_k.shape or v_pages.shape != k_pages.shape \
-            or prefix_k.shape[2] != d or k_pages.shape[2:] != (kv, d):
+    ops, shapes, dt, index = _heads((q, prefix_k, prefix_v, k_pages, v_pages, y),
+                                    ("q", "prefix_k", "prefix_v", "k_pages", "v_pages", "y"))
+    batch, steps, heads, d = shapes[0]
+    prefix, kv, d_keys = shapes[1]
+    count, page, kv_pages, d_pages = shapes[3]
+    if shapes[5] != shapes[0] or shapes[2] != shapes[1] or shapes[4] != shapes[3] or d_keys != d \
+            or kv_pages != kv or d_pages != d:
         raise ValueError("y must have the shape of q, v that of k, and all the same d and kv heads")
     if pages is None:
         if count not in (0, batch):
@@ -341,17 +349,14 @@ def attention_prefix(q, prefix_k, prefix_v, k_pages, v_pages, y, lens, scale: fl
         wide = min(1, count)
     else:
         wide = pages.shape[1]
-    ops, dt, index = _heads((q, prefix_k, prefix_v, k_pages, v_pages, y),
-                            ("q", "prefix_k", "prefix_v", "k_pages", "v_pages", "y"))
     table = _int32(pages, "pages", index, (batch, wide))
     own = _int32(lens, "lens", index, (batch,))
     L = lib()
     ws, size = _workspace(workspace, L.mlkb_attention_prefix_workspace,
-                          (batch, steps, heads, kv, d, prefix_k.shape[0], page, wide), q, index, stream)
-    at = C.addressof(ops)
+                          (batch, steps, heads, kv, d, prefix, page, wide), q, index, stream)
     _call(L.mlkb_attention_prefix,
-          (at, at + 32, at + 64, at + 96, at + 128, at + 160, batch, steps, heads, kv, d, page, wide,
-           table, own, scale, dt, None if ws is None else ws.data_ptr(), size), index, stream)
+          (*ops, batch, steps, heads, kv, d, page, wide, table, own, scale, dt,
+           None if ws is None else ws.data_ptr(), size), index, stream)
 
 
 def fill(out, seed: int, stream_id: int, dist: str, lo: float, hi: float, stream=None):

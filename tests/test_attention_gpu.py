@@ -789,3 +789,14 @@ def test_calls_at_once_given_streams(cuda):
         want, bound = prefix(q, pk, pv, kp, vp, lens.tolist(), 0.125)
         for z in y:
             check(z, want, bound)
+
+
+def test_wrappers_refuse_other_ranks(cuda):
+    q, s = torch.zeros(8, 64, device="cuda", dtype=F16), ints([0, 8])
+    for x in (q, q[0], q[None, None, None]):
+        with pytest.raises(ValueError):
+            api.attention_packed(x, x, x, x.clone(), s, s, 0.1)
+        with pytest.raises(ValueError):
+            api.norm_rope(x, None, x, None, table(9, 64, "cuda"), s)
+    with pytest.raises(ValueError):
+        api.attention_packed(q[None, None], q[None, None], q[None, None], q[None, None].clone(), s, s, 0.1)
