@@ -141,7 +141,8 @@ struct Params {
     int32_t* chunk;                                               // keys of a chunk, for the join
     float* part;
     float* lse;
-    int32_t slots;  // partial results of a row, side by side
+    int32_t slots;       // partial results of a row, side by side
+    int32_t wide_store;  // they start at multiples of 32 bytes
 };
 
 template <int D>
@@ -537,6 +538,18 @@ __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, i
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= inv;
     return fmaf(m, p.c2, log2f(l));
+}
+
+// 8 floats, in one store where `wide` says that the address is a multiple of 32.
+__device__ __forceinline__ void store32(float* to, const uint64_t (&f)[4], int wide) {
+    if (wide) {
+        asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(to), "l"(f[0]), "l"(f[1]), "l"(f[2]),
+                     "l"(f[3])
+                     : "memory");
+    } else {
+        reinterpret_cast<ulonglong2*>(to)[0] = make_ulonglong2(f[0], f[1]);
+        reinterpret_cast<ulonglong2*>(to)[1] = make_ulonglong2(f[2], f[3]);
+    }
 }
 
 // Among each four lanes, lane q's v[i] becomes lane i's v[q].
@@ -1186,7 +1199,9 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
             const uint64_t f02 = tc::pair(f0, f0), f12 = tc::pair(f1, f1);
             uint64_t bad2 = 0;  // 0 times every value: NaN when one is infinite or NaN
             if (spread) {
-                // Few rows, each for itself: all of both accumulators at once.
+                // Few rows, each for itself: all of both accumulators at once, stored 32
+                // bytes at a time (16: 29.9 us instead of 27.4 for 24 requests of 5
+                // tokens; whole tiles' rows are faster four lanes together, below).
                 if constexpr (kPartial) {
                     uint32_t o[D / 32][16], u[D / 32][16];
 #pragma unroll
@@ -1200,10 +1215,10 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                         tc::tmem_ld_wait(u[g]);
                         const bool done = from + g * 16 < p.d;  // columns that were computed
 #pragma unroll
-                        for (int y = 0; y < 16; y += 4) {
-                            uint64_t f[2] = {0, 0};
+                        for (int y = 0; y < 16; y += 8) {
+                            uint64_t f[4] = {0, 0, 0, 0};
 #pragma unroll
-                            for (int z = 0; z < 2; ++z) {
+                            for (int z = 0; z < 4; ++z) {
                                 const int c = y + 2 * z;
                                 if (n > 0 && done) {
                                     f[z] = tc::fma2(tc::pair(__uint_as_float(o[g][c]), __uint_as_float(o[g][c + 1])),
@@ -1215,11 +1230,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                                 }
                                 bad2 = tc::fma2(f[z], 0, bad2);
                             }
-                            if (store && from + g * 16 + y < end) {
-                                const float2 a = tc::unpair(f[0]), b = tc::unpair(f[1]);
-                                *reinterpret_cast<float4*>(out + from + g * 16 + y) =
-                                    make_float4(a.x, a.y, b.x, b.y);
-                            }
+                            if (store && from + g * 16 + y < end) store32(out + from + g * 16 + y, f, p.wide_store);
                         }
                     }
                 }
@@ -1581,7 +1592,7 @@ struct PrefixPlan {
     int64_t spread_tt, pre_spread, suf_spread;
 
     // The partial results, their log-sums, and the chunk length.
-    int64_t bytes(int64_t d) const { return slots * rows * (d + 1) * 4 + 16; }
+    int64_t bytes(int64_t d) const { return slots * rows * (d + 1) * 4 + 32; }
 };
 
 PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_heads,
@@ -1829,7 +1840,8 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     p.sms = smCount();
     p.slots = static_cast<int32_t>(r.slots);
     p.chunk = static_cast<int32_t*>(workspace);
-    p.part = static_cast<float*>(workspace) + 4;
+    p.part = static_cast<float*>(workspace) + 8;
+    p.wide_store = (reinterpret_cast<uintptr_t>(p.part) & 31u) == 0;
     p.lse = p.part + r.slots * r.rows * d;
     Maps m;
     const int box = pages != nullptr && page_size < kTile ? static_cast<int>(page_size) : kTile;

@@ -800,3 +800,15 @@ def test_wrappers_refuse_other_ranks(cuda):
             api.norm_rope(x, None, x, None, table(9, 64, "cuda"), s)
     with pytest.raises(ValueError):
         api.attention_packed(q[None, None], q[None, None], q[None, None], q[None, None].clone(), s, s, 0.1)
+
+
+@pytest.mark.parametrize("offset", [16, 32])
+def test_prefix_workspace_alignment(cuda, offset):
+    """A workspace that is a multiple of 16 bytes only."""
+    q, pk, pv, kp, vp, lens, pages = make_prefix(6, 2, 300, [30, 2, 100, 64, 65, 7], 8, 2, 72, 32, seed=11)
+    need = api.attention_prefix_workspace(q, pk, kp, pages)
+    ws = torch.full((need + 64,), 255, device="cuda", dtype=torch.uint8)
+    y = torch.empty_like(q)
+    api.attention_prefix(q, pk, pv, kp, vp, y, lens, 0.125, pages=pages, workspace=ws[offset:offset + need])
+    check(y, *prefix(q, pk, pv, kp, vp, lens.tolist(), 0.125, pages))
+    assert (ws[:offset] == 255).all() and (ws[offset + need:] == 255).all()
