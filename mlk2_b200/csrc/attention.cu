@@ -74,6 +74,8 @@ int makeTmap3d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const
 namespace {
 
 constexpr int kTile = 128;   // rows of a query tile, keys of a key tile
+constexpr int kWalk = 256;   // about how many groups a block may look at to find its items (512 single tokens
+                             // over 10^6 keys: 0.80-0.87 ms; with levels of one key tile always, 1.05 ms)
 constexpr int kItems = 2;    // item ring: the one in work and the next
 constexpr int kThreads = 12 * 32;
 constexpr int kMma = 8, kTma = 9, kSched = 10;  // warps; 0 to 7 are softmax warps, 11 is idle
@@ -117,6 +119,7 @@ struct KeySource {
 
 struct Params {
     int32_t heads, kv_heads, group, d, tt;  // tt: tokens of a query tile
+    uint64_t pair_inv;                      // 2^64 / (2 tt), upwards: exact quotients below 2^31
     float c2, grow;                         // scale * log2 e; kRescale / c2
     uint64_t limit;                         // of a wait, ns
     int* status;
@@ -192,7 +195,7 @@ __device__ __forceinline__ void splitTiles(Item& it, int keys) {
 // Items are (sequence, pair of query tiles, kv head), numbered in order of
 // falling cost (key tiles of the pair), so that the long ones start first. No
 // list is stored: the warp walks cost levels x groups of 32 sequences, each
-// lane counting its sequence's pairs of exactly that cost, and goes on to the
+// lane counting its sequence's pairs of that cost, and goes on to the
 // next cost that any sequence has (level by level: 63 us instead of 32 for 4
 // queries over 16380 uneven keys, most of it spent by blocks that find no item).
 // Where there are few items the keys of the long ones are cut into chunks, items
@@ -205,9 +208,14 @@ struct Walker {
     int level, base;     // cost level; first sequence of the current group
     int next;            // highest level below that any group seen at this one has
     int chunk;           // packed: most key tiles of an item, 0: any
-    int top;             // packed: the first level
+    int top, step;       // packed: the first level; key tiles of a level
     int64_t before;      // items before (level, group)
-    Seq seq;             // packed: the lane's sequence where all fit one group
+    // packed, what is known of (level, group): its items, those up to the lane's
+    // sequence, and of that its items, pairs, pairs from the level on and chunks
+    bool known;
+    int64_t total, upto, mine;
+    Seq seq;
+    int np, ge, parts;
 };
 
 __device__ __forceinline__ Seq loadSeq(const Params& p, int s) {
@@ -224,23 +232,26 @@ __device__ __forceinline__ Seq loadSeq(const Params& p, int s) {
     return r;
 }
 
-// Pairs of a sequence whose cost is at least `c` key tiles (they are its last).
-__device__ __forceinline__ int pairsFrom(const Params& p, const Seq& s, int c) {
-    const int w = 2 * p.tt;
-    const int np = ceilDiv(s.nq, w);
-    if (c <= 0) return np;
-    const int need = kTile * (c - 1) + 1;  // keys
-    if (s.nk < need) return 0;
-    if (!p.causal) return np;
-    const int tokens = need - (s.nk - s.nq);  // the pair's last token is at least this one
-    const int first = tokens <= 0 ? 0 : (tokens - 1) / w;
-    return np - first;
+// Pair of query tiles that has token `t`.
+__device__ __forceinline__ int pairOf(const Params& p, int t) {
+    return static_cast<int>(__umul64hi(static_cast<uint64_t>(t), p.pair_inv));
 }
 
-// Cost of the pair that ends with the sequence's token `end` (from 1).
-__device__ __forceinline__ int pairCost(const Params& p, const Seq& s, int end) {
+// Of a sequence's `np` pairs, how many have at least level `c` (they are its last).
+__device__ __forceinline__ int pairsFrom(const Params& p, const Seq& s, int np, int c, int step) {
+    if (c <= 0) return np;
+    const int64_t need = static_cast<int64_t>(c - 1) * step * kTile + 1;  // keys
+    if (s.nk < need) return 0;
+    if (!p.causal) return np;
+    const int tokens = static_cast<int>(need) - (s.nk - s.nq);  // the pair's last token is at least this one
+    return np - (tokens <= 0 ? 0 : pairOf(p, tokens - 1));
+}
+
+// Level of the pair that ends with the sequence's token `end` (from 1).
+__device__ __forceinline__ int pairLevel(const Params& p, const Seq& s, int end, int step) {
     const int keys = p.causal ? s.nk - s.nq + min(end, s.nq) : s.nk;
-    return keys <= 0 ? 0 : ceilDiv(keys, kTile);
+    const int tiles = keys <= 0 ? 0 : ceilDiv(keys, kTile);
+    return step == 1 ? tiles : ceilDiv(tiles, step);
 }
 
 __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, int lane) {
@@ -249,40 +260,58 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
         w.base = 0;
         w.next = -1;
         w.before = 0;
+        w.known = false;
     }
     for (;;) {
         if (w.level < 0) return false;
-        const Seq s = p.seqs <= 32 ? w.seq : loadSeq(p, w.base + lane);
-        const int ge = pairsFrom(p, s, w.level), gt = pairsFrom(p, s, w.level + 1);
-        const int parts = w.chunk > 0 && w.level > w.chunk ? ceilDiv(w.level, w.chunk) : 1;
-        const int unit = p.kv_heads * parts;
-        const int64_t mine = static_cast<int64_t>(ge - gt) * unit;
-        int64_t upto = mine;
+        if (!w.known) {
+            w.known = true;
+            if (p.seqs > 32) w.seq = loadSeq(p, w.base + lane);
+            const Seq& s = w.seq;
+            w.np = s.nq > 0 ? pairOf(p, s.nq - 1) + 1 : 0;
+            w.ge = pairsFrom(p, s, w.np, w.level, w.step);
+            w.parts = w.chunk > 0 && w.level > w.chunk ? ceilDiv(w.level, w.chunk) : 1;
+            w.mine = static_cast<int64_t>(w.ge - pairsFrom(p, s, w.np, w.level + 1, w.step)) * p.kv_heads * w.parts;
+            if (__any_sync(0xffffffffu, w.mine > 1 << 25)) {
+                w.upto = w.mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += t;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t t = __shfl_up_sync(0xffffffffu, w.upto, o);
+                    if (lane >= o) w.upto += t;
+                }
+            } else {  // the sums fit 32 bits
+                int upto = static_cast<int>(w.mine);
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int t = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += t;
+                }
+                w.upto = upto;
+            }
+            w.total = __shfl_sync(0xffffffffu, w.upto, 31);
+            const int below = w.np - w.ge;  // pairs of a lower level; the last one's:
+            w.next = max(w.next, below > 0 ? pairLevel(p, s, below * 2 * p.tt, w.step) : -1);
         }
-        const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
-        if (idx < w.before + total) {
+        if (idx < w.before + w.total) {
             const int64_t at = idx - w.before;
-            const unsigned hit = __ballot_sync(0xffffffffu, at < upto);
-            const int src = __ffs(hit) - 1;
-            const int rem = static_cast<int>(at - (upto - mine));
-            if (lane == src) {
-                const int pair = ceilDiv(s.nq, 2 * p.tt) - ge + rem / unit;
+            const unsigned hit = __ballot_sync(0xffffffffu, at < w.upto);
+            if (lane == __ffs(hit) - 1) {
+                const Seq& s = w.seq;
+                const int unit = p.kv_heads * w.parts;
+                const int rem = static_cast<int>(at - (w.upto - w.mine));
+                const int pair = w.np - w.ge + rem / unit;
                 const int part = rem % unit / p.kv_heads;
-                const int c0 = parts > 1 ? part * w.chunk * kTile : 0;
+                const int c0 = w.parts > 1 ? part * w.chunk * kTile : 0;
                 it.live = 1;
                 it.causal = p.causal;
                 it.src = 0;
                 it.kvh = rem % p.kv_heads;
-                it.nk = parts > 1 ? min(s.nk - c0, w.chunk * kTile) : s.nk;
+                it.nk = w.parts > 1 ? min(s.nk - c0, w.chunk * kTile) : s.nk;
                 it.k_row = s.k0 + c0;
                 it.page_row = 0;
                 it.key0 = 0;
                 it.slot = part;
-                it.parts = parts;
+                it.parts = w.parts;
                 it.spread = 0;
                 for (int st = 0; st < 2; ++st) {
                     const int t0 = (2 * pair + st) * p.tt;
@@ -303,10 +332,9 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
             }
             return true;
         }
-        w.before += total;
+        w.known = false;
+        w.before += w.total;
         w.base += 32;
-        const int below = ceilDiv(s.nq, 2 * p.tt) - ge;  // pairs of lower cost; the last one's:
-        w.next = max(w.next, below > 0 ? pairCost(p, s, below * 2 * p.tt) : -1);
         if (w.base >= p.seqs) {
             w.base = 0;
             w.level = __reduce_max_sync(0xffffffffu, w.next);
@@ -665,16 +693,23 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 tiles += static_cast<int64_t>(ceilDiv(q.nq, 2 * p.tt)) * ceilDiv(middle, kTile);
             }
             most = __reduce_max_sync(0xffffffffu, most);
-            w.level = w.top = ceilDiv(most, kTile);
-            w.next = -1;
+            w.top = ceilDiv(most, kTile);
+            w.step = 1;
             if (kPartial) {
                 // About kOwnItems items for each SM, of 4 tiles at least, in the slots there are.
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
                 const int64_t want = (tiles * p.kv_heads + kOwnItems * p.sms - 1) / (kOwnItems * p.sms);
-                w.chunk = max(static_cast<int>(min(want, static_cast<int64_t>(w.level) + 1)), 4);
-                w.chunk = max(w.chunk, ceilDiv(w.level, p.slots));
+                w.chunk = max(static_cast<int>(min(want, static_cast<int64_t>(w.top) + 1)), 4);
+                w.chunk = max(w.chunk, ceilDiv(w.top, p.slots));
+            } else {
+                // With many sequences a level is several key tiles: the walk has kWalk steps at most.
+                const int64_t steps = static_cast<int64_t>(w.top) * ceilDiv(p.seqs, 32);
+                w.step = steps <= kWalk ? 1 : static_cast<int>(min(steps / kWalk, static_cast<int64_t>(max(w.top, 1))));
+                w.top = ceilDiv(w.top, w.step);
             }
+            w.level = w.top;
+            w.next = -1;
         }
         int64_t at = blockIdx.x;  // the block's own item first, then those of blocks not yet launched
         for (uint32_t n = 0, asked = 0;;) {
@@ -1545,6 +1580,7 @@ void setShape(Params& p, int64_t heads, int64_t kv_heads, int64_t d, double scal
     p.group = static_cast<int32_t>(heads / kv_heads);
     p.d = static_cast<int32_t>(d);
     p.tt = kTile / p.group;
+    p.pair_inv = ~uint64_t(0) / static_cast<uint64_t>(2 * p.tt) + 1;
     p.c2 = static_cast<float>(scale * 1.4426950408889634);
     p.grow = kRescale / p.c2;
     p.limit = kLimitNs + kKeyNs * static_cast<uint64_t>(keys);
@@ -1671,7 +1707,7 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
     }
     if (int st = needDevice()) return st;
     Params p = {};
-    setShape(p, heads, kv_heads, d, scale, hk.rows);
+    setShape(p, heads, kv_heads, d, scale, hk.rows + n_seqs);
     p.q = hq.data;
     p.q_row = hq.row_stride;
     p.q_head = hq.head_stride;
@@ -1807,7 +1843,7 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     if (hy.data == hq.data) return setError(MLKB_ERR_INVALID, "attention: y may not overlap the inputs");
     if (int st = needDevice()) return st;
     Params p = {};
-    setShape(p, heads, kv_heads, d, scale, hpk.rows > cap ? hpk.rows : cap);
+    setShape(p, heads, kv_heads, d, scale, (hpk.rows > cap ? hpk.rows : cap) + batch);
     p.q = hq.data;
     p.q_row = hq.row_stride;
     p.q_head = hq.head_stride;

@@ -812,3 +812,13 @@ def test_prefix_workspace_alignment(cuda, offset):
     api.attention_prefix(q, pk, pv, kp, vp, y, lens, 0.125, pages=pages, workspace=ws[offset:offset + need])
     check(y, *prefix(q, pk, pv, kp, vp, lens.tolist(), 0.125, pages))
     assert (ws[:offset] == 255).all() and (ws[offset + need:] == 255).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_very_many_sequences(cuda, causal):
+    """Enough sequences that costs are compared in units of several key tiles."""
+    r = random.Random(5)
+    nq = [r.choice([0, 1, 1, 1, 2, 140]) for _ in range(1500)]
+    nk = [n + r.choice([0, 0, 1, 40, 300, 700]) for n in nq]
+    nk[700] += 6000
+    run_packed(nq, nk, 2, 1, 64, seed=12, causal=causal)
