@@ -1135,11 +1135,11 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     if (masked) hide(s[c & 1], c);
 #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        mx[x / 2 % 4] = tc::max3(mx[x / 2 % 4], __uint_as_float(s[c & 1][x]),
-                                                 __uint_as_float(s[c & 1][x + 1]));
+                        mx[x / 2 % 4] = tc::max3_nan(mx[x / 2 % 4], __uint_as_float(s[c & 1][x]),
+                                                     __uint_as_float(s[c & 1][x + 1]));
                     }
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const float top = tc::max3_nan(tc::max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
                 raise(top, jj > 0);
                 const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
                 const uint64_t c2 = tc::pair(p.c2, p.c2), nm2 = tc::pair(nm, nm);
@@ -1180,7 +1180,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&sm.pfull[st]);
                 const float2 z = tc::unpair(tc::add2(sum[0], sum[1]));
-                l += z.x + z.y;
+                l = top == top ? l + (z.x + z.y) : top;  // a NaN score: ex2_poly may have passed over it
             }
             if (!ok) break;
             // Accumulators done with this item, of either stream.
@@ -1332,9 +1332,10 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
             }
             float lse = l > 0.0f ? fmaf(m, p.c2, log2f(l)) : -INFINITY;
-            // A NaN somewhere, also seen as a sum no row can have (ex2_poly), or an infinity.
+            // A NaN or an infinity among the scores or the values. (Beside a score of +inf
+            // ex2_poly gives numbers.)
             const float2 bad = tc::unpair(bad2);
-            const bool again = mine && l != 0.0f && (!(l < 0x1p60f) || bad.x != 0.0f || bad.y != 0.0f);
+            const bool again = mine && l != 0.0f && (!(l < 0x1p60f) || m == INFINITY || bad.x != 0.0f || bad.y != 0.0f);
             const bool zeros = !kPartial && mine && l == 0.0f;
             const unsigned todo = __ballot_sync(0xffffffffu, again || zeros);
             if (todo != 0) {

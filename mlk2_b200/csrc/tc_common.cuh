@@ -429,7 +429,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // at an eighth of its rate): x = i + f with |f| <= 1/2 by adding and taking off
 // 1.5 * 2^23, 2^f by the degree-4 polynomial of least relative error there
 // (2.7e-6; coefficients from a Remez exchange), 2^i by adding i to the
-// exponent. x below -126 gives 2^-126; a NaN gives a NaN or about 3e38.
+// exponent. x below -126 gives 2^-126, and so does a NaN: who may meet one
+// looks for it apart.
 __device__ __forceinline__ uint64_t ex2_poly(uint64_t x2) {
     const float2 x = unpair(x2);
     const uint64_t v = pair(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
@@ -448,6 +449,13 @@ __device__ __forceinline__ uint64_t ex2_poly(uint64_t x2) {
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// The same where a NaN operand wins.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
