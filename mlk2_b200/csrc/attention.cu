@@ -38,12 +38,16 @@
 // in parts; a second issuing warp.
 //
 // Softmax: running row maximum m (of the raw scores) and sum in f32;
-// p = 2^(c s - c m), c = scale log2 e. The accumulator is rescaled only when a
-// row's maximum has grown by more than 2^8 since the last rescale: until then
-// p stays within 2^8 of 1, far inside the 16-bit formats' range, and the
-// factor cancels in the final division. The commit that makes Q K^T of tile
-// j + 1 visible also covers P V of tile j (one thread issues both), so a rescale
-// finds the accumulator at rest without another barrier.
+// p = 2^(c s - r), c = scale log2 e and r = c m rounded: one rounding to a p, and
+// what r is off by is a factor that all of a row's p share. Where results over
+// different keys meet they are scaled from r to r (in a block) or the factor is
+// taken out first (partial results). From |r| = 2^22 on it grows past what the
+// 16-bit formats hold: such a row is computed again from s - m (slowRow).
+// The accumulator is rescaled only when a row's maximum has grown by more than
+// 2^8 since the last rescale: until then p stays within 2^8 of 1, far inside the
+// 16-bit formats' range, and the factor cancels in the final division. The commit
+// that makes Q K^T of tile j + 1 visible also covers P V of tile j (one thread
+// issues both), so a rescale finds the accumulator at rest without another barrier.
 //
 // p is rounded to the inputs' 16-bit type for the product with V (the tensor
 // cores take equal operand types); its row sum is taken before that rounding.
@@ -83,6 +87,7 @@ constexpr int kConsumers = 10;                  // warps that read an item
 constexpr uint64_t kLimitNs = 2000000000ull;  // of a wait, and its share for each key an item may have:
 constexpr uint64_t kKeyNs = 16000, kMostNs = 60000000000ull;  // 32 rows done again take up to 7 us a key
 constexpr float kRescale = 8.0f;  // log2 of the growth of a row maximum that forces a rescale
+constexpr float kFar = 0x1p22f;   // scaled row maxima up to which c m may be rounded
 constexpr int kPoly = 2;          // of 8 pairs of exponentials, how many go to the FMA pipe (0, 1, 3, 4: slower)
 constexpr int kMaxSlots = 128;    // partial results a row may have: 16 x 4 of the prefix, as many of its own keys
 constexpr int kOwnItems = 2;      // items of own keys an SM should get (4: more epilogues than the even end gives)
@@ -143,7 +148,7 @@ struct Params {
     int32_t pre_parts, suf_parts;               // slots of an item: 4 when spread, else 1
     int32_t* chunk;                                               // keys of a chunk, for the join
     float* part;
-    float* lse;
+    float2* lse;         // of each partial result: row maximum, log2 of the sum of 2^(c s - c m)
     int32_t slots;       // partial results of a row, side by side
     int32_t wide_store;  // they start at multiples of 32 bytes
 };
@@ -493,9 +498,10 @@ __device__ __forceinline__ int pageRow(const Params& p, const Item& it, int key)
 // Row `row` of the query tile from the definition, over the item's keys that
 // the row sees (of a spread item, those of `part`), by a warp: a lane scores
 // one of 32 keys and then owns four columns of the result. o: those columns
-// (normalised); returns the log2 of the row's sum. All lanes have one row.
+// (normalised); returns the row's maximum and the log2 of its sum. All lanes
+// have one row.
 template <typename T>
-__device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, int row, int part,
+__device__ __noinline__ float2 slowRow(const Params& p, const Item& it, int st, int row, int part,
                                       float (&o)[4]) {
     const int lane = threadIdx.x & 31;
     const int token = row / p.group, head = it.kvh * p.group + row % p.group;
@@ -561,11 +567,11 @@ __device__ __noinline__ float slowRow(const Params& p, const Item& it, int st, i
         }
         if (m != m) break;
     }
-    if (m == -INFINITY) return -INFINITY;  // nothing to see: zeros
+    if (m == -INFINITY) return make_float2(-INFINITY, -INFINITY);  // nothing to see: zeros
     const float inv = 1.0f / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= inv;
-    return fmaf(m, p.c2, log2f(l));
+    return make_float2(m, log2f(l));
 }
 
 // 8 floats, in one store where `wide` says that the address is a multiple of 32.
@@ -1045,11 +1051,13 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                               token < (spread ? p.spread_tt : p.tt);
             const bool idle = !__any_sync(0xffffffffu, mine);  // no row of the warp is wanted
             float m = -INFINITY, l = 0.0f;
+            // What the row's exponents are counted from (r above).
+            auto scaled = [&](float x) { return __fmul_rn(x, p.c2); };
             // Takes a tile's row maximum into m, the sum and the accumulator (`begun`).
             auto raise = [&](float top, bool begun) {
                 const bool grow = top > m + p.grow;
                 if (!__any_sync(0xffffffffu, grow)) return;
-                const float f = grow ? tc::ex2((m - top) * p.c2) : 1.0f;
+                const float f = grow ? tc::ex2(scaled(m) - scaled(top)) : 1.0f;
                 m = grow ? top : m;
                 l *= f;
                 if (!begun) return;
@@ -1091,7 +1099,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                                                  __uint_as_float(v[x + 1]));
                     }
                     raise(fmaxf(mx[0], mx[1]), jj > 0);
-                    const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
+                    const float nm = m == -INFINITY ? 0.0f : -scaled(m);
                     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
@@ -1141,7 +1149,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
                 const float top = tc::max3_nan(tc::max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
                 raise(top, jj > 0);
-                const float nm = m == -INFINITY ? 0.0f : -m * p.c2;
+                const float nm = m == -INFINITY ? 0.0f : -scaled(m);
                 const uint64_t c2 = tc::pair(p.c2, p.c2), nm2 = tc::pair(nm, nm);
                 uint64_t sum[2] = {0, 0};
                 auto probabilities = [&](auto plain) {
@@ -1206,8 +1214,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 const float2 o = sm.xch[st ^ 1][quarter * 32 + lane];
                 if (theirs > 0 && !tc::mbar_wait(&sm.ofull[st ^ 1], o_other & 1u, abort, p.limit)) break;
                 const float both = fmaxf(m, o.x);
-                f0 = l == 0.0f ? 0.0f : tc::ex2((m - both) * p.c2);
-                f1 = o.y == 0.0f ? 0.0f : tc::ex2((o.x - both) * p.c2);
+                f0 = l == 0.0f ? 0.0f : tc::ex2(scaled(m) - scaled(both));
+                f1 = o.y == 0.0f ? 0.0f : tc::ex2(scaled(o.x) - scaled(both));
                 l = l * f0 + o.y * f1;
                 m = both;
                 from = st * (D / 2);
@@ -1228,7 +1236,9 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 ? reinterpret_cast<Out*>(p.part) + ((tok_row * p.heads + head) * p.slots + slot) * p.d
                 : static_cast<Out*>(p.y) + tok_row * p.y_row + head * p.y_head;
             // Four lanes store four rows together, 64 bytes of one row at a time. A
-            // row that sees nothing is left to the end.
+            // row that sees nothing is left to the end. (Every p of a row may
+            // underflow where its maximum is far from 0.)
+            const bool far = m != -INFINITY && !(fabsf(scaled(m)) < kFar);
             const bool store = mine && l != 0.0f;
             const int end = to < p.d ? to : p.d;
             const uint64_t f02 = tc::pair(f0, f0), f12 = tc::pair(f1, f1);
@@ -1331,12 +1341,13 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     }
                 }
             }
-            float lse = l > 0.0f ? fmaf(m, p.c2, log2f(l)) : -INFINITY;
-            // A NaN or an infinity among the scores or the values. (Beside a score of +inf
-            // ex2_poly gives numbers.)
+            float2 lse = l > 0.0f ? make_float2(m, log2f(l) - fmaf(m, p.c2, -scaled(m)))
+                                  : make_float2(-INFINITY, -INFINITY);
+            // A NaN or an infinity among the scores or the values (beside a score of +inf
+            // ex2_poly gives numbers), or a maximum too far from 0.
             const float2 bad = tc::unpair(bad2);
-            const bool again = mine && l != 0.0f && (!(l < 0x1p60f) || m == INFINITY || bad.x != 0.0f || bad.y != 0.0f);
-            const bool zeros = !kPartial && mine && l == 0.0f;
+            const bool again = mine && (far || (l != 0.0f && (!(l < 0x1p60f) || bad.x != 0.0f || bad.y != 0.0f)));
+            const bool zeros = !kPartial && mine && l == 0.0f && !far;
             const unsigned todo = __ballot_sync(0xffffffffu, again || zeros);
             if (todo != 0) {
                 __syncwarp();  // after the other lanes' stores
@@ -1347,7 +1358,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                         __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(out), src));
                     float o[4] = {};
                     if (slow >> src & 1u) {
-                        const float z = slowRow<T>(p, it, st, __shfl_sync(0xffffffffu, row, src), quarter, o);
+                        const float2 z = slowRow<T>(p, it, st, __shfl_sync(0xffffffffu, row, src), quarter, o);
                         if (lane == src) lse = z;
                     }
                     if (4 * lane >= from && 4 * lane < end) {
@@ -1361,10 +1372,10 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
             }
             if (kPartial && mine && from == 0) {
-                float* out_lse = p.lse + (tok_row * p.heads + head) * p.slots;
+                float2* out_lse = p.lse + (tok_row * p.heads + head) * p.slots;
                 out_lse[slot] = lse;
                 if (!kPrefix && it.slot == 0) {  // slots without a chunk
-                    for (int x = it.parts; x < p.slots; ++x) out_lse[x] = -INFINITY;
+                    for (int x = it.parts; x < p.slots; ++x) out_lse[x] = make_float2(-INFINITY, -INFINITY);
                 }
             }
             tc::tc_fence_before();  // the reads above come before the next item's products
@@ -1386,11 +1397,13 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
 // Bound by latency at the sizes there are (13 slots of 2560 rows: 17 MB out of
 // L2), so slots lie side by side and eight are loaded at a time (a slot's rows
 // side by side, one load at a time: 171 us instead of 153 for a whole call over
-// a prefix of 32768). One warp per result row: y = sum_i 2^(lse_i - top) o_i / sum_i 2^(lse_i - top)
-// over the row's slots; those that saw no key have lse = -inf and are not read.
+// a prefix of 32768). One warp per result row: y = sum_i w_i o_i / sum_i w_i over
+// the row's slots, w_i = 2^(c (m_i - top) + log2 of slot i's sum) with the largest
+// of the maxima m_i as top; slots that saw no key have m = -inf and are not read.
 struct JoinParams {
     const float* part;
-    const float* lse;
+    const float2* lse;
+    float c2;
     int64_t rows, y_row, y_head;
     int32_t slots, heads, d;
     // prefix: slots of the prefix, of a chunk of own keys, and the chunk
@@ -1419,12 +1432,13 @@ attention_join(const __grid_constant__ JoinParams p, const __grid_constant__ Par
         if (!__any_sync(0xffffffffu, mine)) return;
     }
     // The prefix' slots are all written; of its own keys those of chunks that exist.
-    const float* mine = p.lse + row * slots;
+    const float2* mine = p.lse + row * slots;
     const float* part = p.part + row * slots * d;
-    float e[kMaxSlots / 32];
+    const float2 none = make_float2(-INFINITY, -INFINITY);
+    float2 z[kMaxSlots / 32];
 #pragma unroll
     for (int i = 0; i < kMaxSlots / 32; ++i) {
-        e[i] = lane + 32 * i < slots ? mine[lane + 32 * i] : -INFINITY;
+        z[i] = lane + 32 * i < slots ? mine[lane + 32 * i] : none;
     }
     if (kPrefix && slots > p.prefix_slots) {
         const int keys = *p.chunk;
@@ -1435,14 +1449,14 @@ attention_join(const __grid_constant__ JoinParams p, const __grid_constant__ Par
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kMaxSlots / 32; ++i) {
-        if (lane + 32 * i >= slots) e[i] = -INFINITY;
-        top = fmaxf(top, e[i]);
+        if (lane + 32 * i >= slots) z[i] = none;
+        top = fmaxf(top, z[i].x);
     }
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.0f;
+    float sum = 0.0f, e[kMaxSlots / 32];
 #pragma unroll
     for (int i = 0; i < kMaxSlots / 32; ++i) {
-        e[i] = e[i] == -INFINITY ? 0.0f : tc::ex2(e[i] - top);
+        e[i] = z[i].x == -INFINITY ? 0.0f : tc::ex2(fmaf(z[i].x - top, p.c2, z[i].y));
         sum += e[i];
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -1596,7 +1610,7 @@ KeySource keySource(const mlkb_heads& k, const mlkb_heads& v) {
 // How attention_packed cuts its work.
 struct PackedPlan {
     int64_t items, slots, rows;
-    int64_t bytes(int64_t d) const { return slots * rows * (d + 1) * 4; }
+    int64_t bytes(int64_t d) const { return slots * rows * (d + 2) * 4; }
 };
 
 PackedPlan planPacked(int64_t rows, int64_t key_rows, int64_t seqs, int64_t heads, int64_t kv_heads,
@@ -1628,8 +1642,8 @@ struct PrefixPlan {
     int64_t suf_mt, suf_slots, tickets, slots;
     int64_t spread_tt, pre_spread, suf_spread;
 
-    // The partial results, their log-sums, and the chunk length.
-    int64_t bytes(int64_t d) const { return slots * rows * (d + 1) * 4 + 32; }
+    // The partial results, their maxima and log-sums, and the chunk length.
+    int64_t bytes(int64_t d) const { return slots * rows * (d + 2) * 4 + 32; }
 };
 
 PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_heads,
@@ -1741,11 +1755,12 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
     p.sms = smCount();
     p.slots = static_cast<int32_t>(r.slots);
     p.part = static_cast<float*>(workspace);
-    p.lse = p.part + r.slots * r.rows * d;
+    p.lse = reinterpret_cast<float2*>(p.part + r.slots * r.rows * d);
     if (int st = launchAttention<false, true>(m, p, elem_dtype, grid, asStream(stream))) return st;
     JoinParams j = {};
     j.part = p.part;
     j.lse = p.lse;
+    j.c2 = p.c2;
     j.rows = r.rows;
     j.y_row = hy.row_stride;
     j.y_head = hy.head_stride;
@@ -1879,7 +1894,7 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     p.chunk = static_cast<int32_t*>(workspace);
     p.part = static_cast<float*>(workspace) + 8;
     p.wide_store = (reinterpret_cast<uintptr_t>(p.part) & 31u) == 0;
-    p.lse = p.part + r.slots * r.rows * d;
+    p.lse = reinterpret_cast<float2*>(p.part + r.slots * r.rows * d);
     Maps m;
     const int box = pages != nullptr && page_size < kTile ? static_cast<int>(page_size) : kTile;
     if (int st = headsMap(&m.q, hq, heads, d, elem_dtype, p.group, p.tt, nullptr)) return st;
@@ -1899,6 +1914,7 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
     JoinParams j = {};
     j.part = p.part;
     j.lse = p.lse;
+    j.c2 = p.c2;
     j.rows = r.rows;
     j.y_row = hy.row_stride;
     j.y_head = hy.head_stride;

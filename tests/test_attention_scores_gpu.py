@@ -1,9 +1,10 @@
 """Scores at the ends of their range in attention_packed and attention_prefix:
-NaN and infinities in visible keys."""
+NaN and infinities in visible keys, and scores whose products with
+scale log2 e are far from 0."""
 import pytest
 import torch
 
-from attention_util import check, packed, prefix, starts
+from attention_util import check, half_step, packed, prefix, starts
 from mlk2_b200 import api
 
 pytestmark = pytest.mark.gpu
@@ -22,6 +23,15 @@ def normal(g, *shape, dtype=BF16):
 
 def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def mean_bound(y, size, n, dtype):
+    """Error of a mean over n values of which `size` is the largest magnitude,
+    from probabilities that differ by exactly known factors: each is rounded to
+    the element type (u), taken by an exponential of at most 2.7e-6, summed in
+    f32 (n 2^-24, twice), and the result is rounded (u |y|)."""
+    u = half_step(dtype)
+    return (u + 2 * 2.7e-6 + 2 * (n + 16) * 2.0 ** -24) * size + u * (1 + u) * y.abs() + u * u * size
 
 
 # ---- NaN and infinities in keys that are seen -------------------------------------
@@ -99,3 +109,87 @@ def test_prefix_key(cuda, what, batch, steps):
         check(y[1:], want[1:], bound[1:])
         check(y[:, :, 4:], want[:, :, 4:], bound[:, :, 4:])
     assert api.take_device_error() == 0
+
+
+# ---- large scores ------------------------------------------------------------------
+
+SIZES = [(F16, 64), (F16, 300), (F16, 725), (F16, 1100), (F16, 5736), (F16, 12128), (F16, 60000),
+         (BF16, 2.0 ** 11), (BF16, 2.0 ** 30), (BF16, 1.5 * 2.0 ** 58)]
+
+
+def large_inputs(g, nq, nk, kv, d, dtype, size):
+    """Queries and keys of one value each in all elements: every third key points the other way."""
+    q = torch.full((nq, 2 * kv, d), size, device="cuda", dtype=dtype)
+    k = torch.full((nk, kv, d), size, device="cuda", dtype=dtype)
+    away = torch.arange(nk, device="cuda") % 3 == 1
+    k[away] *= -1
+    return q, k, normal(g, nk, kv, d, dtype=dtype), away
+
+
+def means(q, v, away, nq, nk, causal):
+    """The mean of the values seen that have the largest score, for each query."""
+    seen = torch.arange(nk, device="cuda")[None] <= torch.arange(nq, device="cuda")[:, None] + nk - nq if causal \
+        else torch.ones(nq, nk, dtype=torch.bool, device="cuda")
+    near = seen & ~away
+    near = torch.where(near.any(-1, keepdim=True), near, seen)
+    w = near.double() / near.sum(-1, keepdim=True)
+    y = torch.einsum("qk,kcd->qcd", w, v.double())
+    return y.repeat_interleave(q.shape[1] // v.shape[1], 1)
+
+
+@pytest.mark.parametrize("dtype,size", SIZES)
+@pytest.mark.parametrize("nq,nk,causal", [(300, 300, True), (90, 300, False), (300, 700, False), (1, 5000, True)])
+def test_packed_large_scores(cuda, nq, nk, causal, dtype, size):
+    q, k, v, away = large_inputs(gen(4), nq, nk, 1, 128, dtype, size)
+    want = means(q, v, away, nq, nk, causal)
+    bound = mean_bound(want, v.abs().max().double(), nk, dtype)
+    for workspace in (None, torch.empty(0, device="cuda")):
+        y = torch.empty_like(q)
+        api.attention_packed(q, k, v, y, starts([nq], "cuda"), starts([nk], "cuda"), 128 ** -0.5, causal=causal,
+                             workspace=workspace)
+        check(y, want, bound)
+
+
+@pytest.mark.parametrize("dtype,size", SIZES)
+@pytest.mark.parametrize("batch", [2, 40])
+def test_prefix_large_scores(cuda, batch, dtype, size):
+    g = gen(5)
+    length, own, kv, d = 500, 300, 1, 128
+    q, k, v, away = large_inputs(g, batch, length + own, kv, d, dtype, size)
+    kp = k[length:, None].transpose(0, 1).repeat(batch, 1, 1, 1)
+    vp = v[length:, None].transpose(0, 1).repeat(batch, 1, 1, 1)
+    y = torch.empty_like(q[:, None])
+    api.attention_prefix(q[:, None], k[:length], v[:length], kp, vp, y, ints([own] * batch), 128 ** -0.5)
+    want = means(q, v, away, 1, length + own, True)[:1].expand(batch, -1, -1)
+    check(y[:, 0], want, mean_bound(want, v.abs().max().double(), length + own, dtype))
+
+
+@pytest.mark.parametrize("dtype,base", [(F16, 0), (F16, 256), (F16, 1024), (F16, 1700), (F16, 1920), (BF16, 1024),
+                                        (BF16, 1920)])
+@pytest.mark.parametrize("nq,nk", [(300, 700), (90, 400), (1, 5000)])
+def test_packed_small_differences_of_large_scores(cuda, nq, nk, dtype, base):
+    """Scores base^2 + t, exact in f32: the weights are e^t whatever the base, across tiles,
+    streams and joined chunks."""
+    g = gen(6)
+    d = 64
+    q = torch.zeros(nq, 2, d, device="cuda", dtype=dtype)
+    k = torch.zeros(nk, 1, d, device="cuda", dtype=dtype)
+    q[:, :, 0], k[:, :, 0] = base, base
+    q[:, :, 1] = 1
+    t = torch.randint(-8, 4, (nk,), generator=g, device="cuda").double() / 2 + torch.arange(nk, device="cuda") // 100 % 3
+    k[:, 0, 1] = t.to(dtype)
+    v = normal(g, nk, 1, d, dtype=dtype)
+    p = torch.softmax(t, 0)
+    want = torch.einsum("k,kcd->cd", p, v.double()).expand(nq, 2, d)
+    weight = torch.einsum("k,kcd->cd", p, v.double().abs()).expand(nq, 2, d)
+    # u for each probability; the exponent's product is rounded once, |t - max| 2^-23 at most
+    # beside the exponential's 2.7e-6; the f32 sums; log-sums of chunks of up to 2^14 keys,
+    # 15 2^-23 in the exponent; the result's rounding
+    u = half_step(dtype)
+    e = 2 * (2.7e-6 + 16 * 2.0 ** -23 + 15 * 2.0 ** -23) + 4 * (nk + 16) * 2.0 ** -24
+    bound = (u + e) * (1 + u) * weight + u * want.abs() + e * weight
+    for workspace in (None, torch.empty(0, device="cuda")):
+        y = torch.empty_like(q)
+        api.attention_packed(q, k, v, y, starts([nq], "cuda"), starts([nk], "cuda"), 1.0, causal=False,
+                             workspace=workspace)
+        check(y, want, bound)
