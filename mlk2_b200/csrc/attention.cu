@@ -51,6 +51,10 @@
 //
 // p is rounded to the inputs' 16-bit type for the product with V (the tensor
 // cores take equal operand types); its row sum is taken before that rounding.
+// f16 has few bits below 2^-14 and none below 2^-25, where the many small p of a
+// long row may lie, so there p is held 2^7 times its value: at most 2^15, and the
+// smallest step is 2^-31 of the row's largest (2^18 keys at e^-17.5 of the largest
+// came to nothing without it). The factor cancels like the others.
 //
 // Keys past an item's end are masked in the scores and zeroed in V's tile (a
 // zero probability times a NaN would be NaN). Values that only some rows of a
@@ -1051,7 +1055,9 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                               token < (spread ? p.spread_tt : p.tt);
             const bool idle = !__any_sync(0xffffffffu, mine);  // no row of the warp is wanted
             float m = -INFINITY, l = 0.0f;
-            // What the row's exponents are counted from (r above).
+            // What the row's exponents are counted from (r above), and by how much p is
+            // held larger.
+            constexpr float kUp = kBf16 ? 0.0f : 7.0f;
             auto scaled = [&](float x) { return __fmul_rn(x, p.c2); };
             // Takes a tile's row maximum into m, the sum and the accumulator (`begun`).
             auto raise = [&](float top, bool begun) {
@@ -1099,7 +1105,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                                                  __uint_as_float(v[x + 1]));
                     }
                     raise(fmaxf(mx[0], mx[1]), jj > 0);
-                    const float nm = m == -INFINITY ? 0.0f : -scaled(m);
+                    const float nm = m == -INFINITY ? 0.0f : kUp - scaled(m);
                     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
@@ -1149,7 +1155,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 }
                 const float top = tc::max3_nan(tc::max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
                 raise(top, jj > 0);
-                const float nm = m == -INFINITY ? 0.0f : -scaled(m);
+                const float nm = m == -INFINITY ? 0.0f : kUp - scaled(m);
                 const uint64_t c2 = tc::pair(p.c2, p.c2), nm2 = tc::pair(nm, nm);
                 uint64_t sum[2] = {0, 0};
                 auto probabilities = [&](auto plain) {
@@ -1341,7 +1347,7 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                     }
                 }
             }
-            float2 lse = l > 0.0f ? make_float2(m, log2f(l) - fmaf(m, p.c2, -scaled(m)))
+            float2 lse = l > 0.0f ? make_float2(m, log2f(l) - kUp - fmaf(m, p.c2, -scaled(m)))
                                   : make_float2(-INFINITY, -INFINITY);
             // A NaN or an infinity among the scores or the values (beside a score of +inf
             // ex2_poly gives numbers), or a maximum too far from 0.

@@ -1,6 +1,6 @@
 """Scores at the ends of their range in attention_packed and attention_prefix:
-NaN and infinities in visible keys, and scores whose products with
-scale log2 e are far from 0."""
+NaN and infinities in visible keys, scores whose rounded products with
+scale log2 e are far from 0, and small probabilities of long flat tails."""
 import pytest
 import torch
 
@@ -193,3 +193,31 @@ def test_packed_small_differences_of_large_scores(cuda, nq, nk, dtype, base):
         api.attention_packed(q, k, v, y, starts([nq], "cuda"), starts([nk], "cuda"), 1.0, causal=False,
                              workspace=workspace)
         check(y, want, bound)
+
+
+# ---- small probabilities ---------------------------------------------------------------
+
+@pytest.mark.parametrize("gap", [14.0, 17.5, 19.0])
+@pytest.mark.parametrize("nq", [1, 300])
+def test_packed_flat_tail(cuda, nq, gap):
+    """One key far above 2^18 equal others: each of those has a probability at the
+    lower end of f16 (e^-17.5 = 2^-25.2), all together a visible share."""
+    n, d = 2 ** 18, 16
+    q = torch.zeros(nq, 1, d, device="cuda", dtype=F16)
+    k = torch.zeros(n, 1, d, device="cuda", dtype=F16)
+    v = torch.ones(n, 1, d, device="cuda", dtype=F16)
+    q[:, :, 0] = 1
+    k[77, 0, 0] = gap
+    v[77] = 0
+    y = torch.empty_like(q)
+    api.attention_packed(q, k, v, y, starts([nq], "cuda"), starts([n], "cuda"), 1.0, causal=False,
+                         workspace=torch.empty(0, device="cuda"))
+    tail = (n - 1) * torch.exp(torch.tensor(-gap, dtype=torch.float64, device="cuda"))
+    want = (tail / (1 + tail)).expand(y.shape)
+    # Probabilities are held 2^7 above their value against the largest: a step of 2^-24
+    # there is 2^-31, half of it an error; u where they are normal. The f32 sums: the
+    # tile's sum joins a running one each 128 keys, 2^-24 a join and 128 2^-24 within;
+    # the product with V adds 16 keys at a time, at most 2^-23 an addition if truncated.
+    u = half_step(F16)
+    sums = (n / 128 + 128) * 2.0 ** -24 + n / 16 * 2.0 ** -23
+    check(y, want, n * 2.0 ** -32 + (2 * u + 2.7e-6 + sums) * want)
