@@ -481,10 +481,10 @@ int64_t mlkb_attention_packed_workspace(int64_t rows, int64_t key_rows, int64_t 
  *                       in use until the call's work on `stream` is done: calls
  *                       (and captured graphs) that may run at the same time
  *                       need workspaces of their own. Its contents do not matter
- * Types, sizes, rounding and masked keys as in mlkb_attention_packed. A
- * length outside [0, page_size * pages_per_request] is taken as the nearer
- * end, and a page index outside the pages reads as zeros; both raise
- * MLKB_ERR_INVALID in the status word.
+ * Types, sizes, rounding and masked keys as in mlkb_attention_packed, steps *
+ * heads below 2^31. A length outside [0, page_size * pages_per_request] is
+ * taken as the nearer end, and a page index outside the pages reads as zeros;
+ * both raise MLKB_ERR_INVALID in the status word.
  */
 int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* prefix_k,
                           const mlkb_heads* prefix_v, const mlkb_heads* k_pages,

@@ -1554,12 +1554,12 @@ int launchAttention(const Maps& m, const Params& p, int dtype, int grid, cudaStr
                      : launchKernel<128, __nv_bfloat16, kPrefix, kPartial>(m, p, grid, s);
 }
 
+int64_t joinBlocks(int64_t rows) { return (rows + 7) / 8; }
+
 template <bool kPrefix>
 int launchJoin(const JoinParams& j, const Params& p, void* y, int dtype, cudaStream_t s) {
-    const int64_t blocks = (j.rows + 7) / 8;
-    if (blocks > INT_MAX) return setError(MLKB_ERR_INVALID, "attention: too many rows");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.gridDim = dim3(static_cast<unsigned>(joinBlocks(j.rows)));
     cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute pdl[1];
@@ -1575,17 +1575,23 @@ int launchJoin(const JoinParams& j, const Params& p, void* y, int dtype, cudaStr
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "attention join launch");
 }
 
+bool headsFit(int64_t heads, int64_t kv_heads) {
+    return heads >= 1 && kv_heads >= 1 && kv_heads <= 65536 && heads % kv_heads == 0 &&
+           heads / kv_heads <= kTile;
+}
+bool sizeFits(int64_t d) { return d >= 8 && d <= 128 && d % 8 == 0; }
+bool shapeFits(int64_t heads, int64_t kv_heads, int64_t d) { return headsFit(heads, kv_heads) && sizeFits(d); }
+
 // Checks what both entries share.
 int checkShape(int64_t heads, int64_t kv_heads, int64_t d, double scale, int32_t dtype) {
     if (dtype != MLKB_F16 && dtype != MLKB_BF16) {
         return setError(MLKB_ERR_INVALID, "attention: dtype must be f16 or bf16");
     }
-    if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads / kv_heads > kTile ||
-        kv_heads > 65536) {
+    if (!headsFit(heads, kv_heads)) {
         return setError(MLKB_ERR_INVALID,
                         "attention: heads must be a multiple of kv heads, at most 128 to each");
     }
-    if (d < 8 || d > 128 || d % 8 != 0) {
+    if (!sizeFits(d)) {
         return setError(MLKB_ERR_INVALID, "attention: d must be a multiple of 8, 8 to 128");
     }
     const float c2 = static_cast<float>(scale * 1.4426950408889634);
@@ -1650,6 +1656,14 @@ struct PrefixPlan {
 
     // The partial results, their maxima and log-sums, and the chunk length.
     int64_t bytes(int64_t d) const { return slots * rows * (d + 2) * 4 + 32; }
+
+    // Whether the kernels' 32-bit counts hold it: items, those of a request, and the
+    // join's rows of a request and blocks.
+    bool fits(int64_t steps, int64_t heads, int64_t kv_heads) const {
+        return pre_items + tickets <= INT_MAX && slots <= kMaxSlots &&
+               kv_heads * suf_mt * suf_slots <= INT_MAX && steps * heads <= INT_MAX &&
+               joinBlocks(rows) <= INT_MAX;
+    }
 };
 
 PrefixPlan planPrefix(int64_t batch, int64_t steps, int64_t heads, int64_t kv_heads,
@@ -1779,9 +1793,8 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
 extern "C" int64_t mlkb_attention_packed_workspace(int64_t rows, int64_t key_rows, int64_t n_seqs,
                                                    int64_t heads, int64_t kv_heads, int64_t d) {
     using namespace mlkb;
-    if (rows < 0 || key_rows < 0 || n_seqs < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
-        heads / kv_heads > kTile || d < 8 || d > 128 || rows > kMaxHeadRows ||
-        key_rows > kMaxHeadRows || n_seqs > kMaxHeadRows || heads > (1 << 23) || rows * heads > kMaxHeadTotal) {
+    if (!shapeFits(heads, kv_heads, d) || rows < 0 || key_rows < 0 || n_seqs < 0 || rows > kMaxHeadRows ||
+        key_rows > kMaxHeadRows || n_seqs > kMaxHeadRows || rows * heads > kMaxHeadTotal) {
         return -1;
     }
     return planPacked(rows, key_rows, n_seqs, heads, kv_heads, d).bytes(d);
@@ -1791,16 +1804,16 @@ extern "C" int64_t mlkb_attention_prefix_workspace(int64_t batch, int64_t steps,
                                                    int64_t kv_heads, int64_t d, int64_t prefix_rows,
                                                    int64_t page_size, int64_t pages_per_request) {
     using namespace mlkb;
-    if (batch < 0 || steps < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
-        heads / kv_heads > kTile || d < 8 || d > 128 || prefix_rows < 0 || page_size < 0 ||
-        pages_per_request < 0 || batch > kMaxHeadRows || steps > kMaxHeadRows || heads > (1 << 23) ||
+    if (!shapeFits(heads, kv_heads, d) || batch < 0 || steps < 1 || prefix_rows < 0 || page_size < 0 ||
+        pages_per_request < 0 || batch > kMaxHeadRows || steps > kMaxHeadRows ||
         prefix_rows > kMaxHeadRows || page_size > kMaxHeadRows || pages_per_request > kMaxHeadRows ||
-        batch * steps > kMaxHeadRows || batch * steps * heads > kMaxHeadTotal) {
+        page_size * pages_per_request > kMaxHeadRows || batch * steps > kMaxHeadRows ||
+        batch * steps * heads > kMaxHeadTotal) {
         return -1;
     }
     const PrefixPlan r =
         planPrefix(batch, steps, heads, kv_heads, prefix_rows, page_size * pages_per_request);
-    return r.bytes(d);
+    return r.fits(steps, heads, kv_heads) ? r.bytes(d) : -1;
 }
 
 extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* prefix_k,
@@ -1853,8 +1866,7 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
         return setError(MLKB_ERR_INVALID, "attention: lens needed");
     }
     const PrefixPlan r = planPrefix(batch, steps, heads, kv_heads, hpk.rows, cap);
-    if (r.pre_items + r.tickets > INT_MAX || r.slots > kMaxSlots ||
-        kv_heads * r.suf_mt * r.suf_slots > INT_MAX) {
+    if (!r.fits(steps, heads, kv_heads)) {
         return setError(MLKB_ERR_INVALID, "attention: too much work for one call");
     }
     if (workspace_bytes < r.bytes(d) || workspace == nullptr || !aligned16(workspace)) {

@@ -1,0 +1,37 @@
+"""Calls of norm_rope and the attention entries that are refused before any
+device work, through the C ABI; no GPU needed."""
+import pytest
+
+import mlk2_b200 as mb
+from test_attention_abi import Y, accepted, heads, no_device, packed, prefix, refused
+
+
+# ---- rows of one request ----------------------------------------------------------
+
+def many(steps, heads_, batch=1):
+    q = heads(steps * batch, row=8 * heads_, head=8)
+    y = heads(steps * batch, row=8 * heads_, head=8, data=Y)
+    return {"batch": batch, "steps": steps, "heads_": heads_, "kv": heads_ // 2, "d": 8, "q": q, "y": y,
+            "pk": heads(30, row=4 * heads_, head=8), "pv": heads(30, row=4 * heads_, head=8),
+            "kp": heads(320, row=4 * heads_, head=8), "vp": heads(320, row=4 * heads_, head=8),
+            "size": 2 ** 62}
+
+
+@pytest.mark.parametrize("steps,heads_", [(2 ** 29, 4), (2 ** 30, 4), (2 ** 27, 64), (2 ** 22, 2 ** 10)])
+def test_prefix_rows_of_a_request_fit_32_bits(steps, heads_):
+    refused(prefix(**many(steps, heads_)), "too much work")
+
+
+@no_device
+def test_prefix_most_rows_of_a_request():
+    accepted(prefix(**many(2 ** 29 - 1, 4)))
+
+
+def test_workspace_of_refused_shapes_is_negative():
+    packed_size, prefix_size = mb.lib().mlkb_attention_packed_workspace, mb.lib().mlkb_attention_prefix_workspace
+    for bad in ((1, 16384, 1, 8, 2, 12), (1, 16384, 1, 2 ** 18, 2 ** 17, 64)):
+        assert packed_size(*bad) < 0
+    for bad in ((1, 2 ** 29, 4, 2, 8, 30, 16, 3), (4, 1, 8, 2, 12, 5, 16, 1), (4, 1, 2 ** 18, 2 ** 17, 64, 5, 16, 1),
+                (4, 1, 8, 2, 64, 5, 2 ** 20, 2 ** 20)):
+        assert prefix_size(*bad) < 0
+    assert prefix_size(1, 2 ** 29 - 1, 4, 2, 8, 30, 16, 3) > 0
