@@ -1737,7 +1737,7 @@ extern "C" int mlkb_attention_packed(const mlkb_heads* q, const mlkb_heads* k, c
         ((reinterpret_cast<uintptr_t>(q_starts) | reinterpret_cast<uintptr_t>(k_starts)) & 3u) != 0) {
         return setError(MLKB_ERR_INVALID, "attention: q_starts and k_starts needed");
     }
-    if (hy.data == hq.data || (hk.rows > 0 && (hy.data == hk.data || hy.data == hv.data))) {
+    if (sameStart(hy, hq) || sameStart(hy, hk) || sameStart(hy, hv)) {
         return setError(MLKB_ERR_INVALID, "attention: y may not overlap the inputs");
     }
     if (int st = needDevice()) return st;
@@ -1874,7 +1874,10 @@ extern "C" int mlkb_attention_prefix(const mlkb_heads* q, const mlkb_heads* pref
                         "attention: workspace (16-byte aligned) smaller than "
                         "mlkb_attention_prefix_workspace says");
     }
-    if (hy.data == hq.data) return setError(MLKB_ERR_INVALID, "attention: y may not overlap the inputs");
+    if (sameStart(hy, hq) || sameStart(hy, hpk) || sameStart(hy, hpv) || sameStart(hy, hk) ||
+        sameStart(hy, hv)) {
+        return setError(MLKB_ERR_INVALID, "attention: y may not overlap the inputs");
+    }
     if (int st = needDevice()) return st;
     Params p = {};
     setShape(p, heads, kv_heads, d, scale, (hpk.rows > cap ? hpk.rows : cap) + batch);

@@ -53,6 +53,12 @@ inline int checkHeads(const mlkb_heads* t, int64_t heads, int64_t d, bool output
     return setError(MLKB_ERR_INVALID, msg);
 }
 
+// Whether two operands have an element in common at their start. (Views may lie
+// between one another's rows, so addresses alone show no other overlap.)
+inline bool sameStart(const mlkb_heads& a, const mlkb_heads& b) {
+    return a.rows > 0 && b.rows > 0 && a.data == b.data;
+}
+
 // MLKB_ERR_NO_DEVICE where no CUDA device can be used.
 inline int needDevice() {
     int dev = 0;

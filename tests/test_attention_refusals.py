@@ -35,3 +35,17 @@ def test_workspace_of_refused_shapes_is_negative():
                 (4, 1, 8, 2, 64, 5, 2 ** 20, 2 ** 20)):
         assert prefix_size(*bad) < 0
     assert prefix_size(1, 2 ** 29 - 1, 4, 2, 8, 30, 16, 3) > 0
+
+
+# ---- outputs that are inputs --------------------------------------------------------
+
+@pytest.mark.parametrize("operand,rows", [("pk", 30), ("pv", 30), ("kp", 320), ("vp", 320)])
+def test_prefix_y_may_not_be_a_cache(operand, rows):
+    refused(prefix(**{operand: heads(rows, data=Y)}), "overlap")
+
+
+@no_device
+def test_prefix_empty_caches_have_no_address():
+    none = heads(0, data=Y)
+    accepted(prefix(pk=none, pv=none))
+    accepted(prefix(kp=none, vp=none, page=0, wide=0, pages=None, lens=None))
