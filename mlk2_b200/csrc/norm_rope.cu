@@ -299,6 +299,13 @@ int launchNormRope(RopeParams& p, bool interleaved, cudaStream_t s) {
     return e == cudaSuccess ? okStatus() : setCudaError(MLKB_ERR_LAUNCH, e, "norm_rope launch");
 }
 
+// Whether an output starts where its own input does but runs on otherwise, or
+// starts where the other side's input does.
+bool overlaps(const mlkb_heads& in, const mlkb_heads& out, const RopeSide& other) {
+    if (sameStart(in, out)) return in.row_stride != out.row_stride || in.head_stride != out.head_stride;
+    return sameStart(out, other.in);
+}
+
 }  // namespace
 }  // namespace mlkb
 
@@ -337,6 +344,10 @@ extern "C" int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const ml
     const int64_t tokens = qs.in.rows;
     if (qs.out.rows != tokens || (kv_heads > 0 && (ks.in.rows != tokens || ks.out.rows != tokens))) {
         return setError(MLKB_ERR_INVALID, "norm_rope: q, k and their outputs must have equal rows");
+    }
+    if (overlaps(qs.in, qs.out, ks) || (kv_heads > 0 && overlaps(ks.in, ks.out, qs)) ||
+        (sameStart(qs.out, ks.out) && !sameStart(qs.in, ks.in))) {
+        return setError(MLKB_ERR_INVALID, "norm_rope: outputs may be their own inputs, and overlap nothing else");
     }
     if (n_axes < 1 || n_axes > kMaxAxes || (n_axes > 1 && sections == nullptr)) {
         return setError(MLKB_ERR_INVALID, "norm_rope: 1 to 4 position axes, with their sections");

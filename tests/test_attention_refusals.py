@@ -3,7 +3,9 @@ device work, through the C ABI; no GPU needed."""
 import pytest
 
 import mlk2_b200 as mb
-from test_attention_abi import Y, accepted, heads, no_device, packed, prefix, refused
+from test_attention_abi import P, Y, accepted, heads, no_device, norm_rope, packed, prefix, refused
+
+K = P + (1 << 22)
 
 
 # ---- rows of one request ----------------------------------------------------------
@@ -49,3 +51,24 @@ def test_prefix_empty_caches_have_no_address():
     none = heads(0, data=Y)
     accepted(prefix(pk=none, pv=none))
     accepted(prefix(kp=none, vp=none, page=0, wide=0, pages=None, lens=None))
+
+
+@pytest.mark.parametrize("kw", [
+    {"qo": heads(row=2048)},                    # q's address, other strides
+    {"qo": heads(row=1024, head=256)},
+    {"ko": heads(row=512, data=K)},             # k's
+    {"qo": heads(data=K)}, {"ko": heads(data=P)},  # the other operand's
+    {"qo": heads(data=Y), "ko": heads(data=Y)}])
+def test_norm_rope_outputs_over_other_operands(kw):
+    refused(norm_rope(**{"k": heads(data=K), "ko": heads(data=K), "heads_": 2, **kw}), "overlap")
+
+
+@no_device
+def test_norm_rope_outputs_in_place_or_apart():
+    apart = {"k": heads(data=K), "ko": heads(data=K)}
+    accepted(norm_rope(**apart))
+    accepted(norm_rope(**{**apart, "qo": heads(data=Y, row=2048)}))
+    # strides of dimensions with one entry do not count
+    accepted(norm_rope(**{**apart, "heads_": 1, "qo": heads(head=4096)}))
+    one = {"k": heads(rows=1, data=K), "ko": heads(rows=1, data=K, row=8)}
+    accepted(norm_rope(**one, q=heads(rows=1), qo=heads(rows=1, row=4096)))
