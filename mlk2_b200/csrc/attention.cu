@@ -227,6 +227,7 @@ struct Walker {
     int np, ge, parts;
 };
 
+// Sequence `s`; without queries past the last and where the starts are bad (k0 -1 there).
 __device__ __forceinline__ Seq loadSeq(const Params& p, int s) {
     Seq r = {0, 0, 0, 0};
     if (s < p.seqs) {
@@ -234,6 +235,7 @@ __device__ __forceinline__ Seq loadSeq(const Params& p, int s) {
         const int c = p.k_starts[s], e = p.k_starts[s + 1];
         if (a < 0 || b < a || b > p.q_rows || c < 0 || e < c || e > p.k_rows) {
             if (p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
+            r.k0 = -1;
         } else {
             r = {a, b - a, c, e - c};
         }
@@ -692,16 +694,23 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         // ---------------- scheduler ----------------
         Walker w = {};
         OwnKeys own = {};
+        // A grid has as many blocks as there can be items, but starts that fall may
+        // claim rows again and make more of them: then a number stands for those a
+        // grid further on too.
+        int64_t wrap = 0;
         if constexpr (!kPrefix) {
+            bool bad = false;
             int most = 0;
             int64_t tiles = 0;  // of all pairs, about: a pair in the middle for each
             for (int s = lane; s - lane < p.seqs; s += 32) {
                 const Seq q = loadSeq(p, s);
                 w.seq = q;
+                bad = bad || q.k0 < 0;
                 if (q.nq > 0 && q.nk > most) most = q.nk;
                 const int middle = p.causal ? max(q.nk - q.nq / 2, 0) : q.nk;
                 tiles += static_cast<int64_t>(ceilDiv(q.nq, 2 * p.tt)) * ceilDiv(middle, kTile);
             }
+            if (__any_sync(0xffffffffu, bad)) wrap = gridDim.x;
             most = __reduce_max_sync(0xffffffffu, most);
             w.top = ceilDiv(most, kTile);
             w.step = 1;
@@ -744,8 +753,10 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 // The next number is asked for towards the end of this item's loads:
                 // earlier would take work that another block is free for.
                 if (!tc::mbar_wait(&sm.cnext, n++ & 1u, abort, p.limit)) break;
-                if (kPrefix && at >= p.pre_items) {  // every `tickets`-th item of the requests
-                    at += p.tickets;
+                // every `tickets`-th item of the requests
+                const int64_t stride = kPrefix ? (at >= p.pre_items ? p.tickets : 0) : wrap;
+                if (stride > 0) {
+                    at += stride;
                     continue;
                 }
             }

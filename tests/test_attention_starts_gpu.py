@@ -1,0 +1,61 @@
+"""attention_packed where the starts of its sequences fall, and with very many
+empty sequences."""
+import pytest
+import torch
+
+import mlk2_b200 as mb
+from attention_util import check, packed, starts
+from mlk2_b200 import api
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, dtype=BF16):
+    return torch.randn(shape, generator=g, device="cuda").to(dtype)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("again,heads", [(1, 1), (1, 4), (9, 1), (40, 2)])
+def test_starts_that_fall_over_long_sequences(cuda, again, heads, causal):
+    """The first 2000 rows claimed many times over, more work than the rows could hold:
+    the sequences behind them are computed all the same."""
+    g = gen(1)
+    n, last = 2000, [5, 1, 40]
+    rows = n + sum(last)
+    q, k, v = normal(g, rows, heads, 64), normal(g, rows, 1, 64), normal(g, rows, 1, 64)
+    s = [0, n] * (again + 1)
+    for m in last:
+        s.append(s[-1] + m)
+    y = torch.full_like(q, 5)
+    assert api.take_device_error() == 0
+    api.attention_packed(q, k, v, y, ints(s), ints(s), 0.125, causal=causal)
+    assert api.take_device_error() == mb.ERR_INVALID
+    want, bound = packed(q, k, v, [n, *last], [n, *last], 0.125, causal)
+    # every claim of the first rows is the same sequence
+    check(y, want, bound)
+
+
+@pytest.mark.parametrize("again", [3, 30])
+def test_starts_that_fall_over_cut_keys(cuda, again):
+    """The same with few queries over many keys, which are cut and joined."""
+    g = gen(2)
+    nq, nk, last = 300, 4000, [2, 1]
+    q, k, v = normal(g, nq + 3, 1, 64), normal(g, nk + 300, 1, 64), normal(g, nk + 300, 1, 64)
+    qs, ks = [0, nq] * (again + 1) + [nq + 2, nq + 3], [0, nk] * (again + 1) + [nk + 250, nk + 300]
+    assert api.attention_packed_workspace(q, k, ints(qs)) > 0
+    need = api.attention_packed_workspace(q, k, ints(qs))
+    y = torch.full_like(q, 5)
+    api.attention_packed(q, k, v, y, ints(qs), ints(ks), 0.125,
+                         workspace=torch.full((need // 4,), torch.nan, device="cuda"))
+    assert api.take_device_error() == mb.ERR_INVALID
+    check(y, *packed(q, k, v, [nq, *last], [nk, 250, 50], 0.125))
