@@ -72,3 +72,14 @@ def test_norm_rope_outputs_in_place_or_apart():
     accepted(norm_rope(**{**apart, "heads_": 1, "qo": heads(head=4096)}))
     one = {"k": heads(rows=1, data=K), "ko": heads(rows=1, data=K, row=8)}
     accepted(norm_rope(**one, q=heads(rows=1), qo=heads(rows=1, row=4096)))
+
+
+# ---- when keys are cut -----------------------------------------------------------------
+
+def test_packed_keys_are_not_cut_among_very_many_sequences():
+    """Every block looks through the sequences for each key count there may be."""
+    size = mb.lib().mlkb_attention_packed_workspace
+    assert size(1, 16384, 8192, 8, 1, 128) == size(1, 16384, 1, 8, 1, 128) > 0
+    assert size(1, 16384, 8193, 8, 1, 128) == 0
+    assert size(40, 16384, 40, 8, 1, 128) > 0
+    assert size(8, 16384, 2000, 8, 2, 128) == 0

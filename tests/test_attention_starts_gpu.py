@@ -59,3 +59,24 @@ def test_starts_that_fall_over_cut_keys(cuda, again):
                          workspace=torch.full((need // 4,), torch.nan, device="cuda"))
     assert api.take_device_error() == mb.ERR_INVALID
     check(y, *packed(q, k, v, [nq, *last], [nk, 250, 50], 0.125))
+
+
+@pytest.mark.parametrize("rows,heads,kv,seqs", [(1, 8, 1, 3000), (7, 3, 3, 700), (5, 8, 8, 40), (4, 1, 1, 1500),
+                                                (3, 8, 2, 50000)])
+def test_few_rows_among_empty_sequences(cuda, rows, heads, kv, seqs):
+    """Single tokens over many keys (cut where the sequences are not too many), each a
+    sequence among empty ones; rows of none are left."""
+    g = gen(3)
+    keys, pad = 4000, 9
+    q = normal(g, rows + pad, heads, 64, dtype=F16)
+    k, v = normal(g, keys, kv, 64, dtype=F16), normal(g, keys, kv, 64, dtype=F16)
+    nq, nk = torch.zeros(seqs, dtype=torch.int64), torch.zeros(seqs, dtype=torch.int64)
+    at = [1 + i * (seqs - 2) // rows for i in range(rows)]
+    lengths = [1 + (keys - rows) * (i + 1) // (rows * (rows + 1) // 2) for i in range(rows)]
+    for i, n in zip(at, lengths):
+        nq[i], nk[i] = 1, n
+    qs, ks = starts(nq.tolist(), "cuda"), starts(nk.tolist(), "cuda")
+    y = torch.full_like(q, 5)
+    api.attention_packed(q, k, v, y, qs, ks, 0.125)
+    check(y[:rows], *packed(q[:rows], k, v, [1] * rows, lengths, 0.125))
+    assert (y[rows:] == 5).all() and api.take_device_error() == 0
