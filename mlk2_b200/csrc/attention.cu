@@ -722,7 +722,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 w.chunk = max(static_cast<int>(min(want, static_cast<int64_t>(w.top) + 1)), 4);
                 w.chunk = max(w.chunk, ceilDiv(w.top, p.slots));
             } else {
-                // With many sequences a level is several key tiles: the walk has kWalk steps at most.
+                // With many sequences a level is several key tiles: the walk has fewer than
+                // 2 kWalk steps, and up to two more for each group of 32 sequences.
                 const int64_t steps = static_cast<int64_t>(w.top) * ceilDiv(p.seqs, 32);
                 w.step = steps <= kWalk ? 1 : static_cast<int>(min(steps / kWalk, static_cast<int64_t>(max(w.top, 1))));
                 w.top = ceilDiv(w.top, w.step);

@@ -103,10 +103,4 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-    return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
-                      pack2<T>(x[6], x[7]));
-}
-
 }  // namespace mlkb
