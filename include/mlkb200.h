@@ -404,6 +404,7 @@ int mlkb_qk_softmax_kt_f16(const void* q, const void* kt, float* y, int64_t batc
  *   heads, kv_heads  1 to 65536; kv_heads 0 leaves k and k_out out
  *   d, rot           multiples of 16, rot <= d <= 512
  *   q_weight, k_weight  [d] in the element type, or both NULL: no norm
+ *   eps              0 to 3e38
  *   table            f32 [table_rows, rot]: cosines, then sines
  *   positions        int32, axis a of token t at [a * position_stride + t];
  *                    a token with a position outside the table is left as it

@@ -45,6 +45,7 @@ struct RopeParams {
     int32_t tokens, d, rot, axes;
     int32_t steps, chunks;   // steps a warp does; warps that share a token
     float eps, inv_d;
+    float eps_up, eps_down;  // eps scaled by 2^140 and by 2^-140, from 64 bits
     int* status;
 };
 
@@ -217,7 +218,7 @@ norm_rope_kernel(const __grid_constant__ RopeParams p) {
             if (__any_sync(0xffffffffu, large || small)) {
                 // The squares left the f32 range (bf16 values past 2^63, or below 2^-63
                 // with an eps that does not hide them): once more on values scaled by
-                // 2^-70 or 2^70, exact in f32. (eps has no weight beside large ones.)
+                // 2^-70 or 2^70, exact in f32.
                 const float f = large ? 0x1p-70f : 0x1p70f;
                 float t = 0.0f;
 #pragma unroll
@@ -227,8 +228,8 @@ norm_rope_kernel(const __grid_constant__ RopeParams p) {
                     t += fmaf(u0, u0, u1 * u1) + fmaf(v0, v0, v1 * v1);
                 }
                 t = sum(mine ? t : 0.0f);
-                if (large) r = rsqrtf(t * p.inv_d) * 0x1p-70f;
-                if (small) r = rsqrtf(fmaf(t, p.inv_d, p.eps * 0x1p70f * 0x1p70f));
+                if (large) r = rsqrtf(fmaf(t, p.inv_d, p.eps_down)) * 0x1p-70f;
+                if (small) r = rsqrtf(fmaf(t, p.inv_d, p.eps_up));
                 const uint64_t keep = small ? tc::pair(f, f) : tc::pair(1.0f, 1.0f);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -326,7 +327,7 @@ extern "C" int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const ml
         return setError(MLKB_ERR_INVALID,
                         "norm_rope: d and rot must be multiples of 16, rot <= d <= 512");
     }
-    if (!std::isfinite(eps) || eps < 0) return setError(MLKB_ERR_INVALID, "norm_rope: bad eps");
+    if (!(eps >= 0 && eps <= 3e38)) return setError(MLKB_ERR_INVALID, "norm_rope: eps must be 0 to 3e38");
     if ((q_weight == nullptr) != (k_weight == nullptr) && kv_heads > 0) {
         return setError(MLKB_ERR_INVALID, "norm_rope: weights of both q and k, or of neither");
     }
@@ -386,6 +387,11 @@ extern "C" int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const ml
     p.rot = static_cast<int32_t>(rot);
     p.axes = n_axes;
     p.eps = static_cast<float>(eps);
+    // An eps above 0 stays above it, so that rows of zeros stay zeros (nothing else is
+    // as small: the least square of a bf16 value is 2^-266).
+    const double up = std::ldexp(eps, 140);
+    p.eps_up = eps > 0 && up < 1.5e-45 ? 1.5e-45f : static_cast<float>(up < 3e38 ? up : 3e38);
+    p.eps_down = static_cast<float>(std::ldexp(eps, -140));
     p.inv_d = 1.0f / static_cast<float>(d);
     p.status = deviceStatusPtr();
     return elem_dtype == MLKB_F16 ? launchNormRope<__half>(p, interleaved != 0, asStream(stream))

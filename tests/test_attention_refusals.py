@@ -74,6 +74,11 @@ def test_norm_rope_outputs_in_place_or_apart():
     accepted(norm_rope(**one, q=heads(rows=1), qo=heads(rows=1, row=4096)))
 
 
+@pytest.mark.parametrize("eps", [3.1e38, 1e300, float("inf"), -1e-300])
+def test_norm_rope_eps(eps):
+    refused(norm_rope(eps=eps), "eps")
+
+
 # ---- when keys are cut -----------------------------------------------------------------
 
 def test_packed_keys_are_not_cut_among_very_many_sequences():
