@@ -162,6 +162,7 @@ norm_rope_kernel(const __grid_constant__ RopeParams p) {
     }
     if (bad) {  // a position outside the table: the token's rows are left as they are
         if (lane == 0 && p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
+        asm volatile("cp.async.wait_all;" ::: "memory");  // the block's memory may go to another
         return;
     }
     // As pairs: for split pairs those of two neighbours, else one value twice
