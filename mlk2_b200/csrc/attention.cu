@@ -61,7 +61,7 @@
 // tile may see (the causal edge) cannot be zeroed: a row whose result has a
 // NaN or an infinity is computed again from its own keys (slowRow), which costs
 // about 7 us a key and warp where all rows of a tile need it (a prompt of 8192
-// whose values are all NaN: 182 ms; one such value: 52 ms).
+// whose values are all NaN: 186 ms; one such value: 52 ms).
 //
 // Every mbarrier wait is bounded; on a timeout the CTA raises the device
 // status word, drains its copies, frees TMEM and returns.
