@@ -439,9 +439,10 @@ int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* q
  * Scores, row maxima, sums and outputs are held in f32; the probabilities are
  * rounded to the element type before the product with v. A query that sees no
  * key (or only scores of -inf) gets zeros, one with a NaN or +inf among the
- * scores it sees gets NaN. Rows of y outside every sequence are left as they were. Keys a query does not see have no effect on it,
- * whatever they or their values hold. A sequence whose starts fall or leave
- * the operands is skipped and raises MLKB_ERR_INVALID in the status word that
+ * scores it sees gets NaN. Rows of y outside every sequence are left as they
+ * were. Keys a query does not see have no effect on it, whatever they or
+ * their values hold. A sequence whose starts fall or leave the operands is
+ * skipped and raises MLKB_ERR_INVALID in the status word that
  * mlkb_take_device_error returns; the others are computed (a row that two of
  * them claim around it holds either's result, or a mixture of both where the
  * keys are cut). y may not overlap the inputs.
