@@ -442,10 +442,9 @@ int mlkb_norm_rope(const mlkb_heads* q, const mlkb_heads* k, const mlkb_heads* q
  * scores it sees gets NaN. Rows of y outside every sequence are left as they
  * were. Keys a query does not see have no effect on it, whatever they or
  * their values hold. A sequence whose starts fall or leave the operands is
- * skipped and raises MLKB_ERR_INVALID in the status word that
- * mlkb_take_device_error returns; the others are computed (a row that two of
- * them claim around it holds either's result, or a mixture of both where the
- * keys are cut). y may not overlap the inputs.
+ * skipped, and so is one whose queries begin below an earlier start; they
+ * raise MLKB_ERR_INVALID in the status word that mlkb_take_device_error
+ * returns, the others are computed. y may not overlap the inputs.
  *   workspace  few queries over many keys are cut along the keys and joined,
  *              with at least mlkb_attention_packed_workspace bytes of device
  *              memory (16-byte aligned); NULL or less: they are not cut. In use

@@ -225,22 +225,47 @@ struct Walker {
     int64_t total, upto, mine;
     Seq seq;
     int np, ge, parts;
+    bool falls;          // some starts fall; then the highest start before the next group
+    int floor;
 };
 
-// Sequence `s`; without queries past the last and where the starts are bad (k0 -1 there).
-__device__ __forceinline__ Seq loadSeq(const Params& p, int s) {
+// Sequence `s` (its starts fall or leave the operands: without queries, and
+// refused); `falls`: whether those of the queries fall.
+__device__ __forceinline__ Seq loadSeq(const Params& p, int s, bool& falls) {
     Seq r = {0, 0, 0, 0};
     if (s < p.seqs) {
         const int a = p.q_starts[s], b = p.q_starts[s + 1];
         const int c = p.k_starts[s], e = p.k_starts[s + 1];
+        falls = falls || b < a;
         if (a < 0 || b < a || b > p.q_rows || c < 0 || e < c || e > p.k_rows) {
             if (p.status != nullptr) atomicExch(p.status, MLKB_ERR_INVALID);
-            r.k0 = -1;
         } else {
             r = {a, b - a, c, e - c};
         }
     }
     return r;
+}
+
+// The start of sequence `s` where it lies inside the operands, else 0.
+__device__ __forceinline__ int startOf(const Params& p, int s) {
+    const int start = s < p.seqs ? p.q_starts[s] : 0;
+    return start >= 0 && start <= p.q_rows ? start : 0;
+}
+
+// Where some starts fall: a sequence that begins below an earlier start is
+// refused too, so that no row is claimed twice. `s`, `r`: the lane's sequence, of
+// 32; floor: the highest start (inside the operands) before those, and then before
+// the next 32.
+__device__ __forceinline__ void keepOrder(const Params& p, int s, int lane, int& floor, Seq& r) {
+    int high = startOf(p, s);
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, high, o);
+        if (lane >= o) high = max(high, t);
+    }
+    high = max(high, floor);
+    floor = __shfl_sync(0xffffffffu, high, 31);
+    if (r.q0 < high) r.nq = 0;  // a start that falls was refused already
 }
 
 // Pair of query tiles that has token `t`.
@@ -272,12 +297,17 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
         w.next = -1;
         w.before = 0;
         w.known = false;
+        w.floor = 0;
     }
     for (;;) {
         if (w.level < 0) return false;
         if (!w.known) {
             w.known = true;
-            if (p.seqs > 32) w.seq = loadSeq(p, w.base + lane);
+            if (p.seqs > 32) {
+                bool falls = false;
+                w.seq = loadSeq(p, w.base + lane, falls);
+                if (w.falls) keepOrder(p, w.base + lane, lane, w.floor, w.seq);
+            }
             const Seq& s = w.seq;
             w.np = s.nq > 0 ? pairOf(p, s.nq - 1) + 1 : 0;
             w.ge = pairsFrom(p, s, w.np, w.level, w.step);
@@ -350,6 +380,7 @@ __device__ bool nextPacked(const Params& p, Walker& w, int64_t idx, Item& it, in
             w.base = 0;
             w.level = __reduce_max_sync(0xffffffffu, w.next);
             w.next = -1;
+            w.floor = 0;
         }
     }
 }
@@ -694,23 +725,27 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
         // ---------------- scheduler ----------------
         Walker w = {};
         OwnKeys own = {};
-        // A grid has as many blocks as there can be items, but starts that fall may
-        // claim rows again and make more of them: then a number stands for those a
-        // grid further on too.
-        int64_t wrap = 0;
         if constexpr (!kPrefix) {
-            bool bad = false;
             int most = 0;
             int64_t tiles = 0;  // of all pairs, about: a pair in the middle for each
-            for (int s = lane; s - lane < p.seqs; s += 32) {
-                const Seq q = loadSeq(p, s);
+            auto add = [&](const Seq& q) {
                 w.seq = q;
-                bad = bad || q.k0 < 0;
                 if (q.nq > 0 && q.nk > most) most = q.nk;
                 const int middle = p.causal ? max(q.nk - q.nq / 2, 0) : q.nk;
                 tiles += static_cast<int64_t>(ceilDiv(q.nq, 2 * p.tt)) * ceilDiv(middle, kTile);
+            };
+            bool falls = false;
+            for (int s = lane; s - lane < p.seqs; s += 32) add(loadSeq(p, s, falls));
+            w.falls = __any_sync(0xffffffffu, falls);
+            if (w.falls) {
+                most = 0;
+                tiles = 0;
+                for (int s = lane, floor = 0; s - lane < p.seqs; s += 32) {
+                    Seq q = loadSeq(p, s, falls);
+                    keepOrder(p, s, lane, floor, q);
+                    add(q);
+                }
             }
-            if (__any_sync(0xffffffffu, bad)) wrap = gridDim.x;
             most = __reduce_max_sync(0xffffffffu, most);
             w.top = ceilDiv(most, kTile);
             w.step = 1;
@@ -754,10 +789,8 @@ attention_tcgen05(const __grid_constant__ CUtensorMap map_q,
                 // The next number is asked for towards the end of this item's loads:
                 // earlier would take work that another block is free for.
                 if (!tc::mbar_wait(&sm.cnext, n++ & 1u, abort, p.limit)) break;
-                // every `tickets`-th item of the requests
-                const int64_t stride = kPrefix ? (at >= p.pre_items ? p.tickets : 0) : wrap;
-                if (stride > 0) {
-                    at += stride;
+                if (kPrefix && at >= p.pre_items) {  // every `tickets`-th item of the requests
+                    at += p.tickets;
                     continue;
                 }
             }
@@ -1442,9 +1475,14 @@ attention_join(const __grid_constant__ JoinParams p, const __grid_constant__ Par
     const int d = p.d;
     if constexpr (!kPrefix) {  // a row of no sequence was not computed
         const int token = static_cast<int>(row / p.heads);
-        bool mine = false;
-        for (int s = lane; s < seqs.seqs; s += 32) {
-            const Seq q = loadSeq(seqs, s);
+        bool mine = false, falls = false;
+#pragma unroll 1
+        for (int s = lane, floor = 0; s - lane < seqs.seqs; s += 32) {
+            Seq q = loadSeq(seqs, s, falls);
+            const int high = __reduce_max_sync(0xffffffffu, startOf(seqs, s));
+            int before = floor;
+            if (__any_sync(0xffffffffu, falls)) keepOrder(seqs, s, lane, before, q);
+            floor = max(floor, high);
             mine = mine || (token >= q.q0 && token < q.q0 + q.nq);
         }
         if (!__any_sync(0xffffffffu, mine)) return;

@@ -80,3 +80,29 @@ def test_few_rows_among_empty_sequences(cuda, rows, heads, kv, seqs):
     api.attention_packed(q, k, v, y, qs, ks, 0.125)
     check(y[:rows], *packed(q[:rows], k, v, [1] * rows, lengths, 0.125))
     assert (y[rows:] == 5).all() and api.take_device_error() == 0
+
+
+@pytest.mark.parametrize("rows,heads,extra", [(2000, 2, 0), (300, 1, 4000)])  # whole; cut and joined
+@pytest.mark.parametrize("again", [1, 20, 500])
+def test_rows_belong_to_the_first_sequence_that_claims_them(cuda, again, rows, heads, extra):
+    """Sequences that begin below an earlier start are refused, in the same 32 and far behind."""
+    g = gen(4)
+    keys = rows + extra
+    q = normal(g, rows + 20, heads, 64)
+    k, v = normal(g, 2 * keys + 20, 1, 64), normal(g, 2 * keys + 20, 1, 64)
+    qs, ks = [0, rows], [0, keys]
+    for i in range(again):  # the same rows, all or a part, with other keys
+        qs += [i % 7 * 10, rows - i % 3]
+        ks += [keys, 2 * keys]
+    qs += [rows + 3, rows + 10, rows + 10, rows + 13]
+    ks += [2 * keys, 2 * keys + 7, 2 * keys + 7, 2 * keys + 10]
+    y = torch.full_like(q, 5)
+    assert api.take_device_error() == 0
+    api.attention_packed(q, k, v, y, ints(qs), ints(ks), 0.125)
+    assert api.take_device_error() == mb.ERR_INVALID
+    check(y[:rows], *packed(q[:rows], k, v, [rows], [keys], 0.125))
+    # once, the sequence behind it begins on the highest start (and has no keys), else one below
+    assert (y[rows:rows + 3] == (0 if again == 1 else 5)).all()
+    check(y[rows + 3:rows + 10], *packed(q[rows + 3:rows + 10], k[2 * keys:], v[2 * keys:], [7], [7], 0.125))
+    check(y[rows + 10:rows + 13], *packed(q[rows + 10:rows + 13], k[2 * keys + 7:], v[2 * keys + 7:], [3], [3], 0.125))
+    assert (y[rows + 13:] == 5).all()
