@@ -106,3 +106,32 @@ def test_rows_belong_to_the_first_sequence_that_claims_them(cuda, again, rows, h
     check(y[rows + 3:rows + 10], *packed(q[rows + 3:rows + 10], k[2 * keys:], v[2 * keys:], [7], [7], 0.125))
     check(y[rows + 10:rows + 13], *packed(q[rows + 10:rows + 13], k[2 * keys + 7:], v[2 * keys + 7:], [3], [3], 0.125))
     assert (y[rows + 13:] == 5).all()
+
+
+def test_captured_call_with_cut_keys_follows_the_starts(cuda):
+    """One graph, replayed with other sequences, with none, and with refused ones."""
+    g = gen(5)
+    q, k, v = normal(g, 6, 8, 64), normal(g, 6000, 2, 64), normal(g, 6000, 2, 64)
+    qs, ks = ints([0, 1, 2, 6]), ints([0, 2000, 2500, 6000])
+    assert api.attention_packed_workspace(q, k, qs) > 0
+    y = torch.zeros_like(q)
+    api.attention_packed(q, k, v, y, qs, ks, 0.125)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        api.attention_packed(q, k, v, y, qs, ks, 0.125)
+    for nq, nk in (([1, 1, 4], [2000, 500, 3500]), ([0, 0, 1], [0, 0, 6000]), ([6, 0, 0], [1, 0, 5]),
+                   ([0, 0, 0], [0, 0, 0]), ([2, 2, 2], [6000, 0, 0])):
+        qs.copy_(starts(nq, "cuda"))
+        ks.copy_(starts(nk, "cuda"))
+        y.fill_(5)
+        graph.replay()
+        n = sum(nq)
+        check(y[:n], *packed(q[:n], k, v, nq, nk, 0.125))
+        assert (y[n:] == 5).all() and api.take_device_error() == 0
+    qs.copy_(ints([0, 4, 2, 6]))
+    ks.copy_(ints([0, 3000, 3000, 6000]))
+    y.fill_(5)
+    graph.replay()
+    check(y[:4], *packed(q[:4], k, v, [4], [3000], 0.125))
+    assert (y[4:] == 5).all() and api.take_device_error() == mb.ERR_INVALID
