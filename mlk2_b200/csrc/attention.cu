@@ -61,7 +61,7 @@
 // tile may see (the causal edge) cannot be zeroed: a row whose result has a
 // NaN or an infinity is computed again from its own keys (slowRow), which costs
 // about 7 us a key and warp where all rows of a tile need it (a prompt of 8192
-// whose values are all NaN: 186 ms; one such value: 52 ms).
+// whose values are all NaN: 180 ms; one such value: 51 ms).
 //
 // Every mbarrier wait is bounded; on a timeout the CTA raises the device
 // status word, drains its copies, frees TMEM and returns.
@@ -581,9 +581,11 @@ __device__ __noinline__ float2 slowRow(const Params& p, const Item& it, int st, 
         const float e = key < lim ? tc::ex2((s - m) * p.c2) : 0.0f;
         float sum = e;
         for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        l = fmaf(l, f, sum);
+        // o stays a weighted mean: sums of the largest bf16 values would leave the f32 range
+        const float all = fmaf(l, f, sum), inv = 1.0f / all, keep = l * f * inv, share = e * inv;
+        l = all;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= f;
+        for (int i = 0; i < 4; ++i) o[i] *= keep;
         for (int j = 0; j < 32; j += 8) {  // eight loads at a time
             uint2 u[8];
 #pragma unroll
@@ -594,7 +596,7 @@ __device__ __noinline__ float2 slowRow(const Params& p, const Item& it, int st, 
             }
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                const float w = __shfl_sync(0xffffffffu, e, j + x);
+                const float w = __shfl_sync(0xffffffffu, share, j + x);
                 const float2 a = unpack2<T>(u[x].x), b = unpack2<T>(u[x].y);
                 o[0] = fmaf(w, a.x, o[0]);
                 o[1] = fmaf(w, a.y, o[1]);
@@ -605,9 +607,6 @@ __device__ __noinline__ float2 slowRow(const Params& p, const Item& it, int st, 
         if (m != m) break;
     }
     if (m == -INFINITY) return make_float2(-INFINITY, -INFINITY);  // nothing to see: zeros
-    const float inv = 1.0f / l;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] *= inv;
     return make_float2(m, log2f(l));
 }
 
@@ -1517,6 +1516,8 @@ attention_join(const __grid_constant__ JoinParams p, const __grid_constant__ Par
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < kMaxSlots / 32; ++i) e[i] *= inv;  // first: sums of large values may leave the f32 range
     const bool live = 4 * lane < d;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -1545,7 +1546,7 @@ attention_join(const __grid_constant__ JoinParams p, const __grid_constant__ Par
     if (live) {
         T* out = y + (row / p.heads) * p.y_row + (row % p.heads) * p.y_head + 4 * lane;
         *reinterpret_cast<uint2*>(out) =
-            make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+            make_uint2(pack2<T>(acc.x, acc.y), pack2<T>(acc.z, acc.w));
     }
 }
 

@@ -221,3 +221,35 @@ def test_packed_flat_tail(cuda, nq, gap):
     u = half_step(F16)
     sums = (n / 128 + 128) * 2.0 ** -24 + n / 16 * 2.0 ** -23
     check(y, want, n * 2.0 ** -32 + (2 * u + 2.7e-6 + sums) * want)
+
+
+# ---- large values -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("size", [2.0 ** 118, 3.3895313892515355e38])
+@pytest.mark.parametrize("nq,nk,causal", [(300, 300, True), (90, 300, False), (1, 5000, True)])
+def test_packed_values_near_the_largest(cuda, nq, nk, causal, size):
+    """Sums of such values leave the f32 range; their weighted mean does not."""
+    g = gen(7)
+    q, k = normal(g, nq, 2, 64), normal(g, nk, 1, 64)
+    v = torch.full((nk, 1, 64), size, device="cuda", dtype=BF16)
+    v[:, :, 1] = -size
+    v[:, 0, 2] *= torch.where(torch.arange(nk, device="cuda") % 3 == 1, -1, 1)
+    want, bound = packed(q, k, v, [nq], [nk], 0.125, causal)
+    for workspace in (None, torch.empty(0, device="cuda")):
+        y = torch.empty_like(q)
+        api.attention_packed(q, k, v, y, starts([nq], "cuda"), starts([nk], "cuda"), 0.125, causal=causal,
+                             workspace=workspace)
+        check(y, want, bound)
+
+
+@pytest.mark.parametrize("batch,steps", [(2, 1), (40, 1), (3, 9)])
+def test_prefix_values_near_the_largest(cuda, batch, steps):
+    g = gen(8)
+    q, pk, kp = normal(g, batch, steps, 4, 64), normal(g, 600, 2, 64), normal(g, batch, 300, 2, 64)
+    top = torch.finfo(BF16).max
+    pv, vp = torch.full_like(pk, top), torch.full_like(kp, top)
+    vp[1::2] = -top
+    lens = [300 - 7 * b for b in range(batch)]
+    y = torch.empty_like(q)
+    api.attention_prefix(q, pk, pv, kp, vp, y, ints(lens), 0.125)
+    check(y, *prefix(q, pk, pv, kp, vp, lens, 0.125))
